@@ -334,6 +334,46 @@ typedef struct svdq_attention_args {
 int svdq_attention(const svdq_attention_args* args, void* stream);
 
 /*
+ * 16-bit rows -> signed 8-bit codes with one fp32 scale per row, optionally behind a residual addition and an RMSNorm:
+ *   h = x (+ residual);  y = h / sqrt(mean(h^2) + eps) * weight  (y = h when weight is NULL);
+ *   scale = max|y| / 127;  code = rint(y / scale).
+ * fp32 arithmetic on the sum before its rounding to `hidden`.  A row of zeros has scale 0; a row whose sum of squares or
+ * maximum is not finite has scale NaN and codes 0.  The same call quantises a weight [N, K] per output channel.  Reference:
+ * quantize_w8a8_act (src/kernels/zgemm/gemm_w8a8.cu), there with a 16-bit scale and no norm.
+ */
+typedef struct svdq_quantize_w8a8_args {
+    const void* x;            /* bf16 / fp16 (`dtype`) [rows, cols], row stride x_stride elements  */
+    const void* residual;     /* NULL, or [rows, cols] of x's type                               */
+    const void* weight;       /* NULL (no norm), or [cols] of x's type                           */
+    void* codes;              /* int8 [rows, cols]                                               */
+    float* scales;            /* fp32 [rows]                                                     */
+    void* hidden;             /* x + residual, x's type [rows, cols] (fp16 saturates); goes with `residual`, may be x or residual
+                                 when that one is contiguous                                     */
+    int64_t rows, x_stride, residual_stride;   /* strides: multiples of 8, at least cols          */
+    int32_t cols;             /* multiple of 16, at most 16384                                   */
+    float eps;
+    int32_t dtype;
+} svdq_quantize_w8a8_args;
+int svdq_quantize_w8a8(const svdq_quantize_w8a8_args* args, void* stream);
+
+/*
+ * out[m][n] = ascales[m] * wscales[n] * sum_k act[m][k] wgt[n][k] (+ bias[n]): 8-bit integer GEMM, int32 accumulation (exact),
+ * scales and bias in fp32, one rounding to the 16-bit output.  Reference: gemm_w8a8 (src/kernels/zgemm/gemm_w8a8.cu).
+ */
+typedef struct svdq_gemm_w8a8_args {
+    const void* act;          /* int8 [M, K]                                                     */
+    const void* wgt;          /* int8 [N, K]                                                     */
+    const float* ascales;     /* fp32 [M]                                                        */
+    const float* wscales;     /* fp32 [N]                                                        */
+    const void* bias;         /* NULL, or [N] of the output's type                               */
+    void* out;                /* bf16 / fp16 (`dtype`) [M, N], row stride out_stride elements     */
+    int64_t out_stride;       /* multiple of 8, at least N                                       */
+    int32_t M, N, K;          /* N a multiple of 8, K of 16 (at most 131056)                     */
+    int32_t dtype;
+} svdq_gemm_w8a8_args;
+int svdq_gemm_w8a8(const svdq_gemm_w8a8_args* args, void* stream);
+
+/*
  * Device-side status word of the current device: 0, or the SVDQ_ERR_TIMEOUT code a
  * kernel recorded when one of its bounded waits ran out.  Synchronises the device.
  * `detail` (may be NULL) receives a kernel-specific location code.  Reading clears it.

@@ -219,6 +219,39 @@ class AttentionArgs(Structure):
     ]
 
 
+class QuantizeW8A8Args(Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("residual", c_void_p),
+        ("weight", c_void_p),
+        ("codes", c_void_p),
+        ("scales", c_void_p),
+        ("hidden", c_void_p),
+        ("rows", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("cols", c_int32),
+        ("eps", c_float),
+        ("dtype", c_int32),
+    ]
+
+
+class GemmW8A8Args(Structure):
+    _fields_ = [
+        ("act", c_void_p),
+        ("wgt", c_void_p),
+        ("ascales", c_void_p),
+        ("wscales", c_void_p),
+        ("bias", c_void_p),
+        ("out", c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("M", c_int32),
+        ("N", c_int32),
+        ("K", c_int32),
+        ("dtype", c_int32),
+    ]
+
+
 class LiteLAArgs(Structure):
     _fields_ = [
         ("qkv", c_void_p),
@@ -248,6 +281,8 @@ EXPORTS = {
     "svdq_litela": (c_int32, [POINTER(LiteLAArgs), c_void_p]),
     "svdq_attention": (c_int32, [POINTER(AttentionArgs), c_void_p]),
     "svdq_quantize_w4a4_wgt": (c_int32, [POINTER(QuantizeWgtArgs), c_void_p]),
+    "svdq_quantize_w8a8": (c_int32, [POINTER(QuantizeW8A8Args), c_void_p]),
+    "svdq_gemm_w8a8": (c_int32, [POINTER(GemmW8A8Args), c_void_p]),
     "svdq_device_status": (c_int32, [POINTER(c_int32), POINTER(c_int32)]),
     "svdq_last_error_string": (c_char_p, []),
     "svdq_version": (c_int32, []),

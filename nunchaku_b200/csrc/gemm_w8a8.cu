@@ -1,0 +1,520 @@
+// 8-bit integer GEMM with a scale per token and per output channel on the tcgen05 tensor cores, sm_100a.
+//
+//   out[m][n] = ascales[m] * wscales[n] * sum_k act[m][k] * wgt[n][k] (+ bias[n])
+//
+// act int8 [M, K] and wgt int8 [N, K] row-major (both K-major operands as they lie in memory), the sum exact in int32
+// (K <= 131071: 2^14 * K stays below 2^31), scales and bias applied in fp32 with one rounding to the 16-bit output.
+// Reference: gemm_w8a8 / quantize_w8a8_act (src/kernels/zgemm/gemm_w8a8.cu), there on mma.sync with 16-bit scales.
+//
+// Two kernels.
+//
+// w8a8_pair_kernel (many tokens): the two SMs of a CTA pair walk 256 x BN output tiles (tcgen05.mma cta_group::2 kind::i8,
+// M 256, K 32), each CTA holding its 128 token rows and half of the weight rows of a 128-deep K stage (128B-swizzled TMA
+// boxes) in a ring; two accumulators of up to 256 columns alternate in TMEM, so that the epilogue of a tile runs under the
+// next tile's products.  Warps: 0 tokens' producer, 1 weights' producer, 2 MMA issuer (leader CTA), 4-11 epilogue (two per
+// lane quadrant, alternating 32-column chunks).
+//
+// w8a8_skinny_kernel (few tokens, the serving form): there every weight is used for a handful of rows and the kernel streams
+// weights.  The operands change places: 128 weight rows are the M side of the product, the tokens (16 to 128) its N side,
+// so that a tile of weights is 16 KB whatever the token count, and K is split over a cluster of up to 8 CTAs to fill the
+// SMs.  The int32 partial sums are exchanged through distributed shared memory (integers: the order does not matter).
+//
+// Every wait is bounded; a role whose wait runs out records SVDQ_ERR_TIMEOUT and leaves its loop.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "host_common.h"
+#include "ptx.cuh"
+
+namespace svdq {
+
+constexpr int W8_BK = 128;                        // K bytes per stage (one 128-byte swizzle row)
+constexpr int W8_BM = 128;                        // token rows per CTA of a pair
+constexpr int W8_BN_MAX = 256;
+constexpr int W8_A_BYTES = W8_BM * W8_BK;         // 16384
+constexpr int W8_B_BYTES = (W8_BN_MAX / 2) * W8_BK;
+constexpr int W8_STAGE_BYTES = W8_A_BYTES + W8_B_BYTES;
+constexpr int W8_STAGES = 6;
+constexpr int W8_EPI_WARPS = 8;
+constexpr int W8_THREADS = (4 + W8_EPI_WARPS) * 32;
+constexpr int W8_COL_BYTES = 2 * W8_BN_MAX * 4;   // column scales and bias of one tile
+constexpr int W8_SMEM = 1024 + W8_STAGES * W8_STAGE_BYTES + W8_COL_BYTES + 256;
+constexpr int W8_MAX_K = 131071;
+constexpr long long W8_WAIT_CYCLES = 4000000000ll;   // ~2 s
+
+struct W8Params {
+    const float* ascales;
+    const float* wscales;
+    const void* bias;
+    void* out;
+    long long out_stride;
+    int M, N, K;
+    int bn, tiles_m, tiles_n;
+    int* status;
+};
+
+struct W8Shared {
+    uint64_t full[W8_STAGES];     // leader: the stage's operands of both CTAs have landed
+    uint64_t empty[W8_STAGES];    // each CTA: the MMAs of the stage are done
+    uint64_t tfull[2];            // each CTA: accumulator complete
+    uint64_t tempty[2];           // leader: accumulator drained by the epilogue warps of both CTAs
+    uint64_t drain;
+    uint32_t tmem_base;
+    volatile int abort_flag;
+};
+
+__device__ __forceinline__ bool w8_wait(uint64_t* bar, uint32_t parity, W8Shared* sh, int* status, int where) {
+#pragma unroll 1
+    for (int i = 0; i < 512; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i) {
+            if (mbar_try_wait(bar, parity)) return true;
+            __nanosleep(32);
+        }
+        if (sh->abort_flag) return false;
+        if (clock64() - t0 > W8_WAIT_CYCLES) {
+            sh->abort_flag = 1;
+            st_shared_cluster_u32(mapa_shared(smem_u32(const_cast<int*>(&sh->abort_flag)), cluster_ctarank() ^ 1u), 1u);
+            atomicExch(&status[0], SVDQ_ERR_TIMEOUT);
+            atomicExch(&status[1], where);
+            return false;
+        }
+    }
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t w8_pack(float lo, float hi) {
+    uint32_t r;
+    if constexpr (F16) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));   // saturates as the W4A4 GEMM's output does
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <bool F16>
+__device__ __forceinline__ float w8_load16(const void* p, int i) {
+    if constexpr (F16) return __half2float(static_cast<const __half*>(p)[i]);
+    else return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+template <bool F16>
+__global__ void __launch_bounds__(W8_THREADS, 1)
+w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const W8Params p) {
+    extern __shared__ __align__(1024) uint8_t w8_smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(w8_smem_raw) + 1023) & ~uintptr_t(1023));
+    float* colv = reinterpret_cast<float*>(smem + W8_STAGES * W8_STAGE_BYTES);     // [0, 256) scales, [256, 512) bias
+    W8Shared* sh = reinterpret_cast<W8Shared*>(reinterpret_cast<uint8_t*>(colv) + W8_COL_BYTES);
+    static_assert(sizeof(W8Shared) <= 256, "barrier block");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int kstages = (p.K + W8_BK - 1) / W8_BK;
+    const int ntiles = p.tiles_m * p.tiles_n;
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int bnh = p.bn >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < W8_STAGES; ++s) {
+            mbar_init(&sh->full[s], 4);       // two producers in each CTA
+            mbar_init(&sh->empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->tfull[i], 1);
+            mbar_init(&sh->tempty[i], 2 * W8_EPI_WARPS);
+        }
+        mbar_init(&sh->drain, 1);
+        sh->abort_flag = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tm_a);
+        prefetch_tmap(&tm_b);
+    }
+    if (warp == 2) {
+        tmem_alloc_pair(&sh->tmem_base, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    cluster_sync_all();   // barriers of both CTAs are initialised before anything remote touches them
+    tc_fence_after_sync();
+    const uint32_t tmem = sh->tmem_base;
+
+    if (warp < 2) {
+        // ------------------------------------------------------------------ producers: 0 = tokens, 1 = weights
+        uint32_t slot = 0, phase = 1;
+        bool ok = true;
+        const uint32_t bytes = warp == 0 ? W8_A_BYTES : bnh * W8_BK;
+        for (int tile = pair; tile < ntiles && ok; tile += npairs) {
+            const int row = warp == 0 ? (tile % p.tiles_m) * (2 * W8_BM) + rank * W8_BM : (tile / p.tiles_m) * p.bn + rank * bnh;
+            for (int ks = 0; ks < kstages; ++ks) {
+                ok = __all_sync(0xffffffffu, w8_wait(&sh->empty[slot], phase, sh, p.status, 810 + warp));
+                if (!ok) break;
+                uint8_t* dst = smem + slot * W8_STAGE_BYTES + (warp ? W8_A_BYTES : 0);
+                const uint32_t lfull = mapa_shared(smem_u32(&sh->full[slot]), 0);
+                if (elect_one()) {
+                    mbar_arrive_expect_tx_cluster(lfull, bytes);
+                    tma_load_2d_pair(dst, warp == 0 ? &tm_a : &tm_b, lfull, ks * W8_BK, row);
+                }
+                __syncwarp();
+                if (++slot == W8_STAGES) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 2 && rank == 0) {
+        // ------------------------------------------------------------------ MMA issuer
+        const uint32_t idesc = idesc_i8(2 * W8_BM, p.bn, true);
+        const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
+        const uint32_t hi = static_cast<uint32_t>(desc0 >> 32), lo0 = static_cast<uint32_t>(desc0);
+        const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]);
+        uint32_t slot = 0, phase = 0, off = 0;
+        bool ok = true;
+        int ti = 0;
+        for (int tile = pair; tile < ntiles && ok; tile += npairs, ++ti) {
+            const uint32_t as = ti & 1;
+            ok = __all_sync(0xffffffffu, w8_wait(&sh->tempty[as], ((ti >> 1) & 1) ^ 1, sh, p.status, 820));
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t d_tmem = tmem + as * W8_BN_MAX;
+            for (int ks = 0; ks < kstages; ++ks) {
+                if (!mbar_try_wait_addr(full0 + 8 * slot, phase)) ok = w8_wait(&sh->full[slot], phase, sh, p.status, 821);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after_sync();
+                if (elect_one()) {
+                    const uint32_t a_lo = lo0 + off, b_lo = a_lo + (W8_A_BYTES >> 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)   // four K = 32 steps; the columns past K are zeros
+                        tc_mma_pair_i8(d_tmem, a_lo + 2 * j, b_lo + 2 * j, hi, idesc, (ks | j) ? 1u : 0u);
+                    tc_commit_pair_addr(empty0 + 8 * slot, 3);
+                }
+                __syncwarp();
+                if (++slot == W8_STAGES) {
+                    slot = 0;
+                    phase ^= 1;
+                    off = 0;
+                } else {
+                    off += W8_STAGE_BYTES >> 4;
+                }
+            }
+            if (ok) {
+                if (elect_one()) tc_commit_pair(&sh->tfull[as], 3);
+                __syncwarp();
+            }
+        }
+        if (sh->abort_flag) {   // let whatever was issued finish before TMEM is released
+            if (lane == 0) {
+                tc_commit_pair(&sh->drain, 1);
+                mbar_wait(&sh->drain, 0, 400000000ll);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------------ epilogue
+        const int quad = warp & 3, set = (warp - 4) >> 2;
+        const int et = threadIdx.x - 128;
+        int ti = 0;
+        for (int tile = pair; tile < ntiles; tile += npairs, ++ti) {
+            const uint32_t as = ti & 1;
+            const int m = (tile % p.tiles_m) * (2 * W8_BM) + rank * W8_BM + quad * 32 + lane;
+            const int n0 = (tile / p.tiles_m) * p.bn;
+            // this tile's column scales and bias (every epilogue warp has left the previous tile at the first barrier)
+            named_barrier_sync(1, W8_EPI_WARPS * 32);
+            if (et < p.bn) {
+                const int n = n0 + et;
+                colv[et] = n < p.N ? p.wscales[n] : 0.f;
+                colv[W8_BN_MAX + et] = (p.bias && n < p.N) ? w8_load16<F16>(p.bias, n) : 0.f;
+            }
+            const float sa = m < p.M ? p.ascales[m] : 0.f;
+            named_barrier_sync(1, W8_EPI_WARPS * 32);
+            const bool ok = __all_sync(0xffffffffu, w8_wait(&sh->tfull[as], (ti >> 1) & 1, sh, p.status, 830));
+            if (ok) {
+                tc_fence_after_sync();
+                uint8_t* orow = static_cast<uint8_t*>(p.out) + 2 * (static_cast<long long>(m) * p.out_stride + n0);
+                for (int c = set * 32; c < p.bn; c += 64) {
+                    uint32_t r[32];
+                    tc_ld_32x32b_x32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + as * W8_BN_MAX + c, r);
+                    tc_wait_ld();
+                    if (m < p.M) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            if (n0 + c + u * 8 < p.N) {   // N is a multiple of 8
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int i = u * 8 + 2 * e;
+                                    const float2 sc = *reinterpret_cast<const float2*>(colv + c + i);
+                                    const float2 bi = *reinterpret_cast<const float2*>(colv + W8_BN_MAX + c + i);
+                                    w[e] = w8_pack<F16>(fmaf(static_cast<float>(static_cast<int>(r[i])) * sa, sc.x, bi.x),
+                                                        fmaf(static_cast<float>(static_cast<int>(r[i + 1])) * sa, sc.y, bi.y));
+                                }
+                                *reinterpret_cast<uint4*>(orow + 2 * (c + u * 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&sh->tempty[as]), 0));
+            }
+            // a warp that gave up still takes part in the block's named barriers, tile by tile
+        }
+    }
+    // Neither CTA may leave (or give up its TMEM) while the other can still signal its barriers or the leader's MMAs can
+    // still read its shared memory: both have passed all their tiles here.
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 2) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- few tokens
+constexpr int W8S_BW = 128;                       // weight rows per CTA (the M side)
+constexpr int W8S_W_BYTES = W8S_BW * W8_BK;
+constexpr int W8S_THREADS = 6 * 32;
+constexpr int W8S_MAX_STAGES = 4;
+constexpr int W8S_MAX_TOKENS = 128;               // tokens per CTA (the N side)
+constexpr int W8S_MAX_SPLIT = 8;
+
+struct W8SShared {
+    uint64_t full[W8S_MAX_STAGES], empty[W8S_MAX_STAGES], done;
+    uint32_t tmem_base;
+    int failed;
+};
+
+__host__ __device__ constexpr int w8s_stages(int bt) { return bt <= 64 ? 4 : 3; }
+__host__ __device__ constexpr int w8s_smem(int bt) { return 1024 + w8s_stages(bt) * (W8S_W_BYTES + bt * W8_BK) + 256; }
+static_assert(w8s_stages(128) * (W8S_W_BYTES + 128 * W8_BK) >= 128 * W8S_BW * 4 && w8s_stages(16) * W8S_W_BYTES >= 16 * W8S_BW * 4,
+              "the exchange buffer lies over the ring");
+
+// grid (weight tiles * split, token tiles), cluster (split, 1, 1)
+template <bool F16>
+__global__ void __launch_bounds__(W8S_THREADS)
+w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t, const W8Params p, const int bt,
+                   const int split) {
+    extern __shared__ __align__(1024) uint8_t w8_smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(w8_smem_raw) + 1023) & ~uintptr_t(1023));
+    const int stages = w8s_stages(bt), stage_bytes = W8S_W_BYTES + bt * W8_BK;
+    W8SShared* sh = reinterpret_cast<W8SShared*>(smem + stages * stage_bytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int n0 = (blockIdx.x / split) * W8S_BW, m0 = blockIdx.y * bt;
+    const int kstages = (p.K + W8_BK - 1) / W8_BK;
+    const int ks0 = kstages * rank / split, ks1 = kstages * (rank + 1) / split;
+    const uint32_t tcols = bt <= 32 ? 32 : bt;    // TMEM columns: a power of two from 32 on
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&sh->full[s], 1);
+            mbar_init(&sh->empty[s], 1);
+        }
+        mbar_init(&sh->done, 1);
+        sh->failed = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tm_w);
+        prefetch_tmap(&tm_t);
+    }
+    if (warp == 1) {
+        tmem_alloc(&sh->tmem_base, tcols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh->tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int i = 0; i < ks1 - ks0; ++i) {
+                const int s = i % stages;
+                if (!mbar_wait(&sh->empty[s], ((i / stages) & 1) ^ 1, W8_WAIT_CYCLES)) {
+                    atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
+                    atomicExch(&p.status[1], 840);
+                    break;
+                }
+                uint8_t* st = smem + s * stage_bytes;
+                mbar_arrive_expect_tx(&sh->full[s], stage_bytes);
+                tma_load_2d(st, &tm_w, &sh->full[s], (ks0 + i) * W8_BK, n0);
+                tma_load_2d(st + W8S_W_BYTES, &tm_t, &sh->full[s], (ks0 + i) * W8_BK, m0);
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = idesc_i8(W8S_BW, bt, true);
+        bool ok = true;
+        for (int i = 0; i < ks1 - ks0; ++i) {
+            const int s = i % stages;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh->full[s], (i / stages) & 1, W8_WAIT_CYCLES));
+            if (!ok) {
+                if (lane == 0) {
+                    atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
+                    atomicExch(&p.status[1], 841);
+                }
+                break;
+            }
+            tc_fence_after_sync();
+            if (elect_one()) {
+                const uint64_t wd = smem_desc_sw128(smem_u32(smem + s * stage_bytes));
+                const uint64_t td = smem_desc_sw128(smem_u32(smem + s * stage_bytes + W8S_W_BYTES));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tc_mma_i8(tmem, wd + 2 * j, td + 2 * j, idesc, (i | j) ? 1u : 0u);
+                tc_commit(&sh->empty[s]);
+            }
+            __syncwarp();
+        }
+        if (elect_one()) tc_commit(&sh->done);
+        __syncwarp();
+    }
+    // ---- partial sums [token][weight row] into shared memory over the ring (all copies and products are done)
+    int* red = reinterpret_cast<int*>(smem);
+    const bool done = mbar_wait(&sh->done, 0, 2 * W8_WAIT_CYCLES);
+    if (!done && lane == 0) {
+        atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
+        atomicExch(&p.status[1], 842);
+    }
+    if (done && warp >= 2) {
+        tc_fence_after_sync();
+        const int quad = warp & 3;
+        for (int c = 0; c < bt; c += 16) {
+            uint32_t r[16];
+            tc_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + c, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) red[(c + i) * W8S_BW + quad * 32 + lane] = static_cast<int>(r[i]);
+        }
+    }
+    tc_fence_before_sync();
+    if (split > 1) cluster_sync_all();
+    else __syncthreads();
+    if (warp >= 2) {
+        const int row = (warp & 3) * 32 + lane, n = n0 + row;
+        const float sw = n < p.N ? p.wscales[n] : 0.f;
+        const float bias = p.bias && n < p.N ? w8_load16<F16>(p.bias, n) : 0.f;
+        for (int t = rank; t < bt && m0 + t < p.M; t += split) {
+            int sum = 0;
+            if (split > 1) {
+#pragma unroll 1
+                for (int q = 0; q < split; ++q) sum += ld_shared_cluster_s32(mapa_shared(smem_u32(red + t * W8S_BW + row), q));
+            } else {
+                sum = red[t * W8S_BW + row];
+            }
+            if (n < p.N) {
+                const float v = fmaf(static_cast<float>(sum) * p.ascales[m0 + t], sw, bias);
+                const uint32_t w = w8_pack<F16>(v, 0.f);
+                static_cast<uint16_t*>(p.out)[static_cast<long long>(m0 + t) * p.out_stride + n] = static_cast<uint16_t>(w);
+            }
+        }
+    }
+    if (split > 1) cluster_sync_all();   // peers may still read this CTA's partial sums
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, tcols);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+static int w8_tmap(CUtensorMap* map, const void* base, int rows, int K, int box_rows) {
+    return make_tmap_2d(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, static_cast<uint64_t>(K), static_cast<uint64_t>(rows),
+                        static_cast<uint64_t>(K), W8_BK, static_cast<uint32_t>(box_rows), true);
+}
+
+template <bool F16>
+static int launch_w8_pair(const CUtensorMap& ta, const CUtensorMap& tb, const W8Params& p, int pairs, cudaStream_t stream) {
+    static std::atomic<uint64_t> attr_done{0};
+    if (int rc = ensure_dynamic_smem(w8a8_pair_kernel<F16>, W8_SMEM, attr_done)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * pairs, 1, 1);
+    cfg.blockDim = dim3(W8_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = W8_SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, w8a8_pair_kernel<F16>, ta, tb, p));
+    return SVDQ_OK;
+}
+
+template <bool F16>
+static int launch_w8_skinny(const CUtensorMap& tw, const CUtensorMap& tt, const W8Params& p, int bt, int split, cudaStream_t stream) {
+    static std::atomic<uint64_t> attr_done{0};
+    if (int rc = ensure_dynamic_smem(w8a8_skinny_kernel<F16>, w8s_smem(W8S_MAX_TOKENS), attr_done)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((p.N + W8S_BW - 1) / W8S_BW * split, (p.M + bt - 1) / bt, 1);
+    cfg.blockDim = dim3(W8S_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = w8s_smem(bt);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, w8a8_skinny_kernel<F16>, tw, tt, p, bt, split));
+    return SVDQ_OK;
+}
+
+}  // namespace svdq
+
+extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args* a, void* stream) {
+    using namespace svdq;
+    SVDQ_CHECK_ARG(a && a->act && a->wgt && a->ascales && a->wscales && a->out, "gemm_w8a8: null pointer");
+    SVDQ_CHECK_ARG(a->M > 0 && a->N > 0 && a->N % 8 == 0, "gemm_w8a8: M (%d) must be positive and N (%d) a positive multiple of 8", a->M, a->N);
+    SVDQ_CHECK_ARG(a->K > 0 && a->K % 16 == 0 && a->K <= W8_MAX_K, "gemm_w8a8: K (%d) must be a positive multiple of 16, at most %d", a->K, W8_MAX_K);
+    SVDQ_CHECK_ARG(a->dtype == SVDQ_DTYPE_BF16 || a->dtype == SVDQ_DTYPE_FP16, "gemm_w8a8: bad dtype %d", a->dtype);
+    SVDQ_CHECK_ARG(a->out_stride >= a->N && a->out_stride % 8 == 0, "gemm_w8a8: the output's row stride must be a multiple of 8, at least N");
+    SVDQ_CHECK_ARG(aligned(a->act, 16) && aligned(a->wgt, 16) && aligned(a->out, 16) && aligned(a->ascales, 4) && aligned(a->wscales, 4) &&
+                       aligned(a->bias, 2),
+                   "gemm_w8a8: act, wgt and out must be 16-byte aligned");
+    if (int rc = check_arch()) return rc;
+    W8Params p = {};
+    p.ascales = a->ascales;
+    p.wscales = a->wscales;
+    p.bias = a->bias;
+    p.out = a->out;
+    p.out_stride = a->out_stride;
+    p.M = a->M;
+    p.N = a->N;
+    p.K = a->K;
+    if (int rc = status_words(&p.status)) return rc;
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool f16 = a->dtype == SVDQ_DTYPE_FP16;
+    const int kstages = (a->K + W8_BK - 1) / W8_BK;
+    CUtensorMap ta, tb;
+    if (a->M <= W8S_MAX_TOKENS) {
+        const int bt = a->M <= 16 ? 16 : a->M <= 32 ? 32 : a->M <= 64 ? 64 : 128;
+        const int tiles = (a->N + W8S_BW - 1) / W8S_BW;
+        int split = 1;
+        while (split < W8S_MAX_SPLIT && tiles * split < 2 * sms && 2 * split <= kstages) split *= 2;
+        if (int rc = w8_tmap(&ta, a->wgt, a->N, a->K, W8S_BW)) return rc;
+        if (int rc = w8_tmap(&tb, a->act, a->M, a->K, bt)) return rc;
+        return f16 ? launch_w8_skinny<true>(ta, tb, p, bt, split, st) : launch_w8_skinny<false>(ta, tb, p, bt, split, st);
+    }
+    const int max_pairs = sms / 2;
+    p.tiles_m = (a->M + 2 * W8_BM - 1) / (2 * W8_BM);
+    // tile width: the one whose rounds over the pairs take the least, a round costing its width plus a fixed part
+    long long best = -1;
+    for (int bn = W8_BN_MAX; bn >= 64; bn -= 32) {
+        const long long tiles = static_cast<long long>(p.tiles_m) * ((a->N + bn - 1) / bn);
+        const long long cost = (tiles + max_pairs - 1) / max_pairs * (bn + 16);
+        if (best < 0 || cost < best) {
+            best = cost;
+            p.bn = bn;
+        }
+    }
+    p.tiles_n = (a->N + p.bn - 1) / p.bn;
+    const int ntiles = p.tiles_m * p.tiles_n;
+    if (int rc = w8_tmap(&ta, a->act, a->M, a->K, W8_BM)) return rc;
+    if (int rc = w8_tmap(&tb, a->wgt, a->N, a->K, p.bn / 2)) return rc;
+    const int pairs = ntiles < max_pairs ? ntiles : max_pairs;
+    return f16 ? launch_w8_pair<true>(ta, tb, p, pairs, st) : launch_w8_pair<false>(ta, tb, p, pairs, st);
+}

@@ -1,0 +1,136 @@
+"""The 8-bit path: 16-bit rows -> int8 codes with one scale per token (optionally behind a residual addition and an RMSNorm), and
+the int8 GEMM with a scale per token and per output channel.
+
+Counterparts in the reference: ``quantize_w8a8_act`` and ``gemm_w8a8`` (src/kernels/zgemm/gemm_w8a8.cu), there with 16-bit scales.
+Forward only, as the rest of the package.
+"""
+from __future__ import annotations
+
+from ctypes import byref
+
+import torch
+
+from .. import _lib
+from ..utils import HALF_DTYPES, dtype_code, on_device, stream_ptr
+
+
+def _rows(name: str, t: torch.Tensor, cols: int) -> tuple[int, int]:
+    """(number of rows, row stride) of ``t`` [..., cols] as a 2-D matrix; raises when its rows have no common stride."""
+    if t.is_contiguous():
+        return t.numel() // cols, cols
+    if t.stride(-1) == 1 or cols == 1:
+        rows, stride = 1, None
+        for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if stride is None:
+                stride = st
+            elif st != stride * rows:
+                break
+            rows *= size
+        else:
+            stride = cols if stride is None else stride
+            if stride >= cols and stride % 8 == 0:
+                return rows, stride
+    raise ValueError(f"{name} must be rows of contiguous columns, one row stride (a multiple of 8 elements) apart")
+
+
+def _check_half(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
+    if not t.is_cuda or t.dtype not in HALF_DTYPES:
+        raise ValueError(f"{name} must be a CUDA bf16 / fp16 tensor (this library has no CPU path)")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must have x's dtype and device")
+
+
+def _quantize(x, weight, residual, eps):
+    _check_half("x", x)
+    cols = x.shape[-1] if x.dim() else 0
+    if x.numel() == 0 or cols % 16:
+        raise ValueError("x must be [..., C] with at least one row and C a positive multiple of 16")
+    rows, x_stride = _rows("x", x, cols)
+    hidden, res_stride = None, 0
+    if weight is not None:
+        _check_half("weight", weight, x)
+        if weight.shape != (cols,) or not weight.is_contiguous():
+            raise ValueError("weight must be a contiguous [C]")
+    if residual is not None:
+        _check_half("residual", residual, x)
+        if residual.shape != x.shape:
+            raise ValueError("residual must have x's shape")
+        res_stride = _rows("residual", residual, cols)[1]
+        hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    args = _lib.QuantizeW8A8Args(x.data_ptr(), None if residual is None else residual.data_ptr(), None if weight is None else weight.data_ptr(),
+                                 codes.data_ptr(), scales.data_ptr(), None if hidden is None else hidden.data_ptr(), rows, x_stride,
+                                 res_stride, cols, eps, dtype_code(x.dtype))
+    with on_device(x.device):
+        _lib.check(_lib.load().svdq_quantize_w8a8(byref(args), stream_ptr(x.device)))
+    return codes, scales, hidden
+
+
+def quantize_w8a8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Symmetric 8-bit codes of bf16 / fp16 ``x`` [..., C] with one scale per row: ``scale = max|x| / 127``, ``code = rint(x / scale)``.
+    Returns (codes int8 like x, scales fp32 [...]).  For activations (one scale per token) and for weights [N, K] (one per output
+    channel) alike.  C: a multiple of 16 up to 16384; the rows of x may be strided.  A row of zeros has scale 0; a row with a NaN or an
+    infinity has scale NaN (and codes 0)."""
+    codes, scales, _ = _quantize(x, None, None, 0.0)
+    return codes, scales
+
+
+def rms_norm_quantize_w8a8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None,
+                           eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``quantize_w8a8(rms_norm(x + residual) * weight)`` in one pass: h = x (+ residual), y = h / sqrt(mean(h^2) + eps) * weight.
+
+    x, residual: bf16 or fp16 [..., C] (rows may be strided), weight [C] of the same dtype.  Returns (codes int8 like x, scales fp32
+    [...], hidden): hidden = x + residual rounded to x's dtype (the residual stream; fp16 saturates), None without a residual.  The norm
+    works on the fp32 sum.  A row whose sum of squares is not finite has scale NaN (and codes 0)."""
+    if weight is None:
+        raise ValueError("weight is required (quantize_w8a8 is the form without the norm)")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    return _quantize(x, weight, residual, eps)
+
+
+def gemm_w8a8(act: torch.Tensor, wgt: torch.Tensor, ascales: torch.Tensor, wscales: torch.Tensor, bias: torch.Tensor | None = None,
+              out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``(act @ wgt.T) * ascales[:, None] * wscales (+ bias)`` for int8 ``act`` [..., K] and ``wgt`` [N, K], fp32 ``ascales`` [...] (one
+    per token) and ``wscales`` [N].  The integer sum is exact; scales and bias are applied in fp32 with one rounding to the output's type.
+
+    K: a multiple of 16 up to 131056; N: a multiple of 8; any number of rows from one on.  ``out`` [..., N] bf16 / fp16 may be rows of a
+    wider buffer (unit column stride, one row stride that is a multiple of 8); by default a new tensor of ``out_dtype`` (bias's dtype,
+    else bf16)."""
+    for name, t in (("act", act), ("wgt", wgt)):
+        if not t.is_cuda or t.dtype != torch.int8 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous CUDA int8 tensor")
+    for name, t in (("ascales", ascales), ("wscales", wscales)):
+        if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous CUDA fp32 tensor")
+    if wgt.dim() != 2 or act.dim() < 1 or act.shape[-1] != wgt.shape[1] or act.numel() == 0:
+        raise ValueError("act must be [..., K] with at least one row and wgt [N, K]")
+    N, K = wgt.shape
+    lead = act.shape[:-1]
+    if ascales.shape != lead or wscales.shape != (N,):
+        raise ValueError("ascales must be act's shape without K and wscales [N]")
+    dev = act.device
+    if wgt.device != dev or ascales.device != dev or wscales.device != dev:
+        raise ValueError("all tensors must be on act's device")
+    if out is not None:
+        if out.shape != (*lead, N) or out.device != dev or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError("out must be [..., N] on act's device (of out_dtype, where that is given)")
+        dtype = out.dtype
+    else:
+        dtype = out_dtype if out_dtype is not None else bias.dtype if bias is not None else torch.bfloat16
+    code = dtype_code(dtype)
+    if bias is not None and (bias.shape != (N,) or bias.dtype != dtype or not bias.is_contiguous() or bias.device != dev):
+        raise ValueError("bias must be a contiguous [N] of the output's dtype on act's device")
+    if out is None:
+        out = torch.empty((*lead, N), dtype=dtype, device=dev)
+        stride = N
+    else:
+        stride = _rows("out", out, N)[1]
+    args = _lib.GemmW8A8Args(act.data_ptr(), wgt.data_ptr(), ascales.data_ptr(), wscales.data_ptr(), None if bias is None else bias.data_ptr(),
+                             out.data_ptr(), stride, act.numel() // K, N, K, code)
+    with on_device(dev):
+        _lib.check(_lib.load().svdq_gemm_w8a8(byref(args), stream_ptr(dev)))
+    return out
