@@ -205,10 +205,6 @@ def _plain_cross(s):
 
 
 # ------------------------------------------------------------------------------------------------------------------ run
-def _values(codes, scales, dtype):
-    return torch.mul(codes, scales[:, None], out=torch.empty(codes.shape, dtype=dtype, device=codes.device))
-
-
 def run(state):
     s, op = state, state["op"]
     if own:
@@ -216,10 +212,10 @@ def run(state):
 
         if op == "norm":
             codes, scales, hidden = ops.rms_norm_quantize_w8a8(s["x"], s["weight"], residual=s["residual"], eps=_EPS)
-            return _values(codes, scales, s["dtype"]), scales, hidden
+            return ops.dequantize_w8a8(codes, scales, out_dtype=s["dtype"]), scales, hidden
         if op == "quant":
             codes, scales = ops.quantize_w8a8(s["x"])
-            return _values(codes, scales, s["dtype"]), scales
+            return ops.dequantize_w8a8(codes, scales, out_dtype=s["dtype"]), scales
         if op == "gemm":
             return ops.gemm_w8a8(s["act"], s["wgt"], s["ascales"], s["wscales"], bias=s["bias"], out_dtype=s["dtype"])
         return ops.cross_attention(s["q"], s["k"], s["v"], kv_lens=s["kv_lens"], mask=s["mask"], kv_offsets=s["kv_offsets"],
