@@ -356,6 +356,17 @@ typedef struct svdq_quantize_w8a8_args {
 } svdq_quantize_w8a8_args;
 int svdq_quantize_w8a8(const svdq_quantize_w8a8_args* args, void* stream);
 
+/* The values such codes stand for: out = code * scale of its row, rounded once.  No counterpart in the reference. */
+typedef struct svdq_dequantize_w8a8_args {
+    const void* codes;        /* int8 [rows, cols]                                               */
+    const float* scales;      /* fp32 [rows]                                                     */
+    void* out;                /* bf16 / fp16 (`dtype`) [rows, cols]                               */
+    int64_t rows;
+    int32_t cols;             /* multiple of 16                                                  */
+    int32_t dtype;
+} svdq_dequantize_w8a8_args;
+int svdq_dequantize_w8a8(const svdq_dequantize_w8a8_args* args, void* stream);
+
 /*
  * out[m][n] = ascales[m] * wscales[n] * sum_k act[m][k] wgt[n][k] (+ bias[n]): 8-bit integer GEMM, int32 accumulation (exact),
  * scales and bias in fp32, one rounding to the 16-bit output.  Reference: gemm_w8a8 (src/kernels/zgemm/gemm_w8a8.cu).

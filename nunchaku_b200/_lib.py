@@ -236,6 +236,17 @@ class QuantizeW8A8Args(Structure):
     ]
 
 
+class DequantizeW8A8Args(Structure):
+    _fields_ = [
+        ("codes", c_void_p),
+        ("scales", c_void_p),
+        ("out", c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", c_int32),
+        ("dtype", c_int32),
+    ]
+
+
 class GemmW8A8Args(Structure):
     _fields_ = [
         ("act", c_void_p),
@@ -282,6 +293,7 @@ EXPORTS = {
     "svdq_attention": (c_int32, [POINTER(AttentionArgs), c_void_p]),
     "svdq_quantize_w4a4_wgt": (c_int32, [POINTER(QuantizeWgtArgs), c_void_p]),
     "svdq_quantize_w8a8": (c_int32, [POINTER(QuantizeW8A8Args), c_void_p]),
+    "svdq_dequantize_w8a8": (c_int32, [POINTER(DequantizeW8A8Args), c_void_p]),
     "svdq_gemm_w8a8": (c_int32, [POINTER(GemmW8A8Args), c_void_p]),
     "svdq_device_status": (c_int32, [POINTER(c_int32), POINTER(c_int32)]),
     "svdq_last_error_string": (c_char_p, []),

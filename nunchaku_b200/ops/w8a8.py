@@ -92,6 +92,23 @@ def rms_norm_quantize_w8a8(x: torch.Tensor, weight: torch.Tensor, residual: torc
     return _quantize(x, weight, residual, eps)
 
 
+def dequantize_w8a8(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values codes stand for: ``codes * scales[..., None]`` rounded once to ``out_dtype`` (bf16 or fp16), for int8 ``codes`` [..., C]
+    (C a multiple of 16) and fp32 ``scales`` [...], both contiguous."""
+    if not codes.is_cuda or codes.dtype != torch.int8 or not codes.is_contiguous():
+        raise ValueError("codes must be a contiguous CUDA int8 tensor")
+    if scales.dtype != torch.float32 or scales.device != codes.device or not scales.is_contiguous():
+        raise ValueError("scales must be a contiguous fp32 tensor on codes' device")
+    cols = codes.shape[-1] if codes.dim() else 0
+    if codes.numel() == 0 or cols % 16 or scales.shape != codes.shape[:-1]:
+        raise ValueError("codes must be [..., C] with at least one row and C a positive multiple of 16, scales [...]")
+    out = torch.empty(codes.shape, dtype=out_dtype, device=codes.device)
+    args = _lib.DequantizeW8A8Args(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel() // cols, cols, dtype_code(out_dtype))
+    with on_device(codes.device):
+        _lib.check(_lib.load().svdq_dequantize_w8a8(byref(args), stream_ptr(codes.device)))
+    return out
+
+
 def gemm_w8a8(act: torch.Tensor, wgt: torch.Tensor, ascales: torch.Tensor, wscales: torch.Tensor, bias: torch.Tensor | None = None,
               out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``(act @ wgt.T) * ascales[:, None] * wscales (+ bias)`` for int8 ``act`` [..., K] and ``wgt`` [N, K], fp32 ``ascales`` [...] (one

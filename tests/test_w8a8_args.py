@@ -21,7 +21,8 @@ def lib():
 
 
 def test_struct_layout_matches_c(lib, tmp_path):
-    structs = {"svdq_quantize_w8a8_args": lib.QuantizeW8A8Args, "svdq_gemm_w8a8_args": lib.GemmW8A8Args}
+    structs = {"svdq_quantize_w8a8_args": lib.QuantizeW8A8Args, "svdq_gemm_w8a8_args": lib.GemmW8A8Args,
+               "svdq_dequantize_w8a8_args": lib.DequantizeW8A8Args}
     lines = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{HEADER}"', "int main(void){"]
     for cname, cls in structs.items():
         lines.append(f'printf("{cname} %zu\\n", sizeof({cname}));')
@@ -55,6 +56,12 @@ def test_quantiser_refuses_null_and_too_wide(lib):
     assert lib.load().svdq_quantize_w8a8(None, None) == lib.SVDQ_ERR_INVALID_ARGUMENT
     assert lib.load().svdq_quantize_w8a8(ctypes.byref(_q(lib, cols=16400, x_stride=16400)), None) == lib.SVDQ_ERR_UNSUPPORTED
     assert b"16384" in lib.load().svdq_last_error_string()
+
+
+@pytest.mark.parametrize("bad", [dict(codes=None), dict(scales=None), dict(out=None), dict(rows=0), dict(cols=8), dict(out=8), dict(dtype=3)])
+def test_dequantiser_refuses(lib, bad):
+    d = dict(codes=64, scales=64, out=64, rows=2, cols=32)
+    assert lib.load().svdq_dequantize_w8a8(ctypes.byref(lib.DequantizeW8A8Args(**{**d, **bad})), None) == lib.SVDQ_ERR_INVALID_ARGUMENT
 
 
 @pytest.mark.parametrize("bad", [dict(act=None), dict(wgt=None), dict(ascales=None), dict(wscales=None), dict(out=None), dict(M=0), dict(N=0),

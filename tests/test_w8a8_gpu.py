@@ -113,6 +113,21 @@ def test_smallest_and_largest_magnitudes():
     assert codes[0, 3] == 127 and codes.abs().sum() == 127
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(16,), (1, 48), (3, 5, 272), (4000, 2240)])
+def test_dequantize(shape, dtype):
+    from nunchaku_b200.ops import dequantize_w8a8
+
+    g = torch.Generator().manual_seed(len(shape))
+    c = torch.randint(-128, 128, shape, generator=g, dtype=torch.int8)
+    s = torch.rand(shape[:-1], generator=g) * 0.1
+    got = dequantize_w8a8(c.cuda(), s.cuda(), out_dtype=dtype).cpu()
+    assert torch.equal(got, (c.float() * s[..., None]).to(dtype))
+    for bad in ((c.cuda().half(), s.cuda()), (c.cuda(), s.cuda().double()), (c.cuda(), torch.zeros(*shape[:-1], 1, device="cuda"))):
+        with pytest.raises(ValueError):
+            dequantize_w8a8(*bad)
+
+
 # ------------------------------------------------------------------------------------------------------------------ GEMM
 def _gemm_case(M, N, K, seed, dtype, bias):
     g = torch.Generator().manual_seed(seed)
