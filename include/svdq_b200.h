@@ -385,6 +385,32 @@ typedef struct svdq_gemm_w8a8_args {
 int svdq_gemm_w8a8(const svdq_gemm_w8a8_args* args, void* stream);
 
 /*
+ * Softmax attention of queries over an encoder's states of another length, heads of 8 to 128 channels: out = softmax(scale q k^T) v
+ * per (batch, head) over the states that exist for the sample; query head h reads stored head h / (heads / kv_heads).  A sample
+ * without states gets zeros; states that do not take part may hold anything (NaN included).  fp32 scores and sums, probabilities
+ * rounded to the 16-bit type before the second product, one rounding of the output.  Reference: MultiHeadCrossAttention
+ * (src/SanaModel.cpp:138-190: packed captions through a varlen library kernel).
+ */
+typedef struct svdq_cross_attention_args {
+    const void* q;            /* element (b, h, t, c) at b*q_stride[0] + h*q_stride[1] + t*q_stride[2] + c; likewise k, v, out     */
+    const void* k;
+    const void* v;
+    void* out;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];   /* batch, head, token: elements, multiples of 8, at least
+                                 head_dim; the batch and head strides of q, k, v may be 0 (broadcast); ignored where the size is 1 */
+    const int32_t* kv_lens;   /* NULL, or [batch] on the device: the first kv_lens[b] states of sample b exist (clamped to 0..kv_len)  */
+    const int32_t* kv_offsets;/* NULL, or [batch + 1] on the device: sample b has rows kv_offsets[b] .. kv_offsets[b + 1] of k and v,
+                                 which then have no batch dimension (clamped to 0..kv_len, the number of rows)                  */
+    const void* mask;         /* NULL, or bytes [batch, kv_len] on the device: states whose byte is not 0 exist              */
+    int64_t mask_stride;      /* bytes between the mask's rows                                   */
+    int32_t batch, heads, kv_heads, q_len, kv_len, head_dim;      /* at most one of kv_lens, kv_offsets, mask; kv_len <= 65536
+                                                                     with a mask                 */
+    float scale;              /* positive                                                        */
+    int32_t dtype;            /* SVDQ_DTYPE_* of q, k, v and out                                 */
+} svdq_cross_attention_args;
+int svdq_cross_attention(const svdq_cross_attention_args* args, void* stream);
+
+/*
  * Device-side status word of the current device: 0, or the SVDQ_ERR_TIMEOUT code a
  * kernel recorded when one of its bounded waits ran out.  Synchronises the device.
  * `detail` (may be NULL) receives a kernel-specific location code.  Reading clears it.

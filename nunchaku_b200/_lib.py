@@ -236,6 +236,31 @@ class QuantizeW8A8Args(Structure):
     ]
 
 
+class CrossAttentionArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("out", c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("o_stride", ctypes.c_int64 * 3),
+        ("kv_lens", c_void_p),
+        ("kv_offsets", c_void_p),
+        ("mask", c_void_p),
+        ("mask_stride", ctypes.c_int64),
+        ("batch", c_int32),
+        ("heads", c_int32),
+        ("kv_heads", c_int32),
+        ("q_len", c_int32),
+        ("kv_len", c_int32),
+        ("head_dim", c_int32),
+        ("scale", c_float),
+        ("dtype", c_int32),
+    ]
+
+
 class DequantizeW8A8Args(Structure):
     _fields_ = [
         ("codes", c_void_p),
@@ -292,6 +317,7 @@ EXPORTS = {
     "svdq_litela": (c_int32, [POINTER(LiteLAArgs), c_void_p]),
     "svdq_attention": (c_int32, [POINTER(AttentionArgs), c_void_p]),
     "svdq_quantize_w4a4_wgt": (c_int32, [POINTER(QuantizeWgtArgs), c_void_p]),
+    "svdq_cross_attention": (c_int32, [POINTER(CrossAttentionArgs), c_void_p]),
     "svdq_quantize_w8a8": (c_int32, [POINTER(QuantizeW8A8Args), c_void_p]),
     "svdq_dequantize_w8a8": (c_int32, [POINTER(DequantizeW8A8Args), c_void_p]),
     "svdq_gemm_w8a8": (c_int32, [POINTER(GemmW8A8Args), c_void_p]),

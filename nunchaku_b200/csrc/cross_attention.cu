@@ -1,0 +1,904 @@
+// Softmax attention of queries over an encoder's states of another length, sm_100a: out = softmax(scale * q k^T) v per (batch, head)
+// over the states that exist for the sample.
+//
+// Heads of 8 to 128 channels (multiples of 8), kv_heads dividing heads (query head h reads stored head h / (heads / kv_heads)),
+// states given as [batch, kv_len] rows (all of them, the first kv_lens[b], or those a byte mask keeps) or packed one sample after
+// the other (kv_offsets).  A sample without states gets zeros.  States that do not take part may hold anything, infinities and
+// NaN included: their scores are replaced, not added to, and their rows of V are zeroed before the second product.
+// Scores, running maximum, sums and the output accumulator are fp32; the probabilities are rounded to the 16-bit type before the
+// second product (the tensor cores take 16-bit operands; the row sum is taken before that rounding), the output once.
+// Reference: MultiHeadCrossAttention, src/SanaModel.cpp:138-190, which calls a varlen library kernel on packed captions.
+//
+// Two kernels.
+//
+// cross_tile_kernel (many queries): one CTA owns 128 query rows of one (batch, head) and walks the states in blocks of 128:
+// Q K^T and P V as tcgen05.mma kind::f16 with S, P and O in tensor memory (S: 128 columns, O: 128), as in attention.cu, but
+// sized for short state lists: 98 KB of shared memory and 256 TMEM columns, so that two CTAs share an SM and one's prologue,
+// exponentials and store run under the other's products (with 300 states a CTA only has three blocks; a CTA alone on its
+// SM, as attention.cu's, would spend half its life filling and draining).  One K and one V slot suffice: K is free as soon as
+// its Q K^T is done, a block ahead of the softmax, V is first needed behind it.  The last block's products, loads and
+// exponentials are cut to the states that exist (N of Q K^T and K-steps of P V in sixteens, the rest in halves of 64).
+// Warps 0-3: softmax, one query row per thread; 4: producer; 5: MMA issuer; 6: zeroes rows of V whose state is not to be seen.
+//
+// cross_rows_kernel (few query rows per stored head: the serving form for single tokens): bound by streaming K and V once.
+// Up to 16 rows (queries x heads that share a stored head) are the M side of mma.sync m16n8k16; four warps take 16 of every 64
+// states each, with their own running maximum; tiles come through a three-stage cp.async ring whose copies write zeros for states that
+// are not to be seen; the states are split over a cluster of up to 8 CTAs and joined through distributed shared memory in one launch.
+//
+// Every wait is bounded; a role whose wait runs out records SVDQ_ERR_TIMEOUT and leaves its loop.
+#include "attention_common.cuh"
+#include "host_common.h"
+
+namespace svdq {
+
+struct CrossStates {
+    const int* kv_lens;       // or NULL
+    const int* kv_offsets;    // or NULL: packed, k / v have no batch dimension
+    const uint8_t* mask;      // or NULL: [batch, kv_len], row stride mask_stride bytes
+    long long mask_stride;
+    int kv_len;               // padded length, or the number of packed rows
+};
+
+// first row and number of rows of sample b; whatever the device arrays hold, inside [0, kv_len]
+__device__ __forceinline__ void cross_range(const CrossStates& s, int b, int& start, int& len) {
+    start = 0;
+    len = s.kv_len;
+    if (s.kv_offsets) {
+        const int a = min(max(s.kv_offsets[b], 0), s.kv_len), e = min(max(s.kv_offsets[b + 1], 0), s.kv_len);
+        start = a;
+        len = max(e - a, 0);
+    } else if (s.kv_lens) {
+        len = min(max(s.kv_lens[b], 0), s.kv_len);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- many queries
+constexpr int CT_BM = 128, CT_BN = 128;
+constexpr int CT_HALF_BYTES = 128 * 128;            // 128 rows x 64 channels
+constexpr int CT_TILE_BYTES = 2 * CT_HALF_BYTES;
+constexpr int CT_THREADS = 256;
+constexpr int CT_PRODUCER_WARP = 4, CT_MMA_WARP = 5, CT_ZERO_WARP = 6;
+// registers move inside the pool the CTA was launched with (256 threads x 128)
+constexpr int CT_REGS_SOFTMAX = 208, CT_REGS_OTHER = 48;
+static_assert(4 * CT_REGS_SOFTMAX + 4 * CT_REGS_OTHER <= 8 * 128, "register budget");
+constexpr int CT_MASK_STATES = 65536;               // longest state list a mask may cover (its bits are kept in shared memory)
+constexpr int CT_BAR_BYTES = 128;
+constexpr int CT_SMEM = 1024 + 3 * CT_TILE_BYTES + CT_BAR_BYTES;   // 98 KB: two CTAs per SM
+constexpr int CT_TMEM_COLS = 256;
+constexpr long long CT_WAIT_CYCLES = 600000000ll;   // ~0.3 s
+constexpr float CT_RESCALE_STEP = 8.f;
+static_assert(2 * (CT_SMEM + CT_MASK_STATES / 8 + 1024) <= 228 * 1024, "two CTAs per SM");
+
+struct CrossTileShared {
+    uint64_t q_full, k_full, k_empty, s_full, p_half[2], pv_done;
+    // A block of V whose rows are all to be seen lands on v_full, which the issuer waits for; one with rows to be zeroed lands on
+    // vh_full, which warp 6 waits for, and the issuer waits for v_zeroed: so every barrier has one sequence of phases that
+    // its waiter follows without gaps.
+    uint64_t v_full, vh_full, v_zeroed, v_empty;
+    uint32_t tmem_base;
+};
+static_assert(sizeof(CrossTileShared) <= CT_BAR_BYTES, "barrier block");
+
+struct CrossTileParams {
+    CrossStates st;
+    int q_len, dim, group;
+    int q_bmul, q_hmul, k_bmul, k_hmul, v_bmul, v_hmul;   // 0 where that dimension is broadcast (stride 0): its coordinate is then 0
+    float scale_log2;
+    int* status;
+};
+
+__device__ __forceinline__ void tma_store_4d(const void* tmap, const void* src, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+                 ::"l"(tmap), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
+
+template <bool F16, bool MASK>
+__global__ void __launch_bounds__(CT_THREADS, 2)
+cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                  const __grid_constant__ CUtensorMap tm_o, const CrossTileParams p) {
+    extern __shared__ __align__(1024) uint8_t ct_smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ct_smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* q_s = smem;
+    uint8_t* k_s = q_s + CT_TILE_BYTES;
+    uint8_t* v_s = k_s + CT_TILE_BYTES;
+    CrossTileShared* sh = reinterpret_cast<CrossTileShared*>(v_s + CT_TILE_BYTES);
+    uint32_t* words = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(sh) + CT_BAR_BYTES);   // MASK: one bit per state
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int q0 = blockIdx.x * CT_BM, head = blockIdx.y, batch = blockIdx.z;
+    const int kv_head = head / p.group;
+    int kv_start, kv_count;
+    cross_range(p.st, batch, kv_start, kv_count);
+    const int nblocks = (kv_count + CT_BN - 1) / CT_BN;
+    const int halves = p.dim > 64 ? 2 : 1;
+
+    if (tid == 0) {
+        mbar_init(&sh->q_full, 1);
+        mbar_init(&sh->k_full, 1);
+        mbar_init(&sh->k_empty, 1);
+        mbar_init(&sh->v_full, 1);
+        mbar_init(&sh->vh_full, 1);
+        mbar_init(&sh->v_empty, 1);
+        mbar_init(&sh->v_zeroed, 1);
+        mbar_init(&sh->s_full, 1);
+        mbar_init(&sh->p_half[0], 4);
+        mbar_init(&sh->p_half[1], 4);
+        mbar_init(&sh->pv_done, 1);
+        fence_mbar_init();
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+        prefetch_tmap(&tm_o);
+    }
+    if (warp == CT_MMA_WARP) {
+        tmem_alloc(&sh->tmem_base, CT_TMEM_COLS);
+        tmem_relinquish();
+    }
+    if constexpr (MASK) {
+        const uint8_t* m = p.st.mask + batch * p.st.mask_stride;
+        for (int w = warp; w < nblocks * 4; w += CT_THREADS / 32) {
+            const int i = w * 32 + lane;
+            const uint32_t bits = __ballot_sync(0xffffffffu, i < kv_count && m[i] != 0);
+            if (lane == 0) words[w] = bits;
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh->tmem_base;
+
+    // States of block j that are looked at: its leading `valid` ones (0: the block is skipped).  `holes`: some of the rows of V
+    // that P V reads (valid rounded up to 16) must not be seen and are not zeros already.
+    auto block_valid = [&](int j) {
+        if constexpr (MASK) {
+#pragma unroll
+            for (int i = 3; i >= 0; --i)
+                if (words[4 * j + i]) return 32 * i + 32 - __clz(words[4 * j + i]);
+            return 0;
+        }
+        return min(kv_count - j * CT_BN, CT_BN);
+    };
+    auto block_holes = [&](int j, int valid) {
+        const int up = (valid + 15) & ~15;
+        if constexpr (MASK) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int bits = min(max(up - 32 * i, 0), 32);
+                const uint32_t want = bits == 32 ? 0xffffffffu : (1u << bits) - 1u;
+                any |= (words[4 * j + i] & want) != want;
+            }
+            return any;
+        }
+        return up != valid && (p.st.kv_lens || p.st.kv_offsets);   // without them the rows past the end are filled with zeros by the copy
+    };
+    auto timeout = [&](int code) {
+        atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
+        atomicExch(&p.status[1], code);
+    };
+
+    if (warp == CT_PRODUCER_WARP) {
+        reg_dealloc<CT_REGS_OTHER>();
+        // ------------------------------------------------------------------ producer
+        if (lane == 0) {
+            int n = 0;
+            bool ok = true;
+            uint32_t uses[3] = {0, 0, 0};   // of k_full, v_full, vh_full
+            for (int j = 0; j < nblocks && ok; ++j) {
+                const int valid = block_valid(j);
+                if (valid == 0) continue;
+                if (n == 0) {
+                    mbar_arrive_expect_tx(&sh->q_full, halves * CT_HALF_BYTES);
+                    for (int h = 0; h < halves; ++h)
+                        tma_load_4d(q_s + h * CT_HALF_BYTES, &tm_q, &sh->q_full, h * 64, q0, head * p.q_hmul, batch * p.q_bmul);
+                }
+                const int boxes = valid > 64 ? 2 : 1;   // of 64 rows
+                const int row = kv_start + j * CT_BN;
+                for (int kv = 0; kv < 2 && ok; ++kv) {
+                    const int which = kv == 0 ? 0 : block_holes(j, valid) ? 2 : 1;
+                    uint64_t* full = which == 0 ? &sh->k_full : which == 1 ? &sh->v_full : &sh->vh_full;
+                    if (!mbar_wait(kv ? &sh->v_empty : &sh->k_empty, (n & 1) ^ 1, CT_WAIT_CYCLES)) {
+                        timeout(900 + kv);
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_expect_tx(full, halves * boxes * (CT_HALF_BYTES / 2));
+                    ++uses[which];
+                    const int z = kv_head * (kv ? p.v_hmul : p.k_hmul), w = p.st.kv_offsets ? 0 : batch * (kv ? p.v_bmul : p.k_bmul);
+                    for (int h = 0; h < halves; ++h)
+                        for (int b = 0; b < boxes; ++b)
+                            tma_load_4d((kv ? v_s : k_s) + h * CT_HALF_BYTES + b * (CT_HALF_BYTES / 2), kv ? &tm_v : &tm_k, full, h * 64,
+                                        row + b * 64, z, w);
+                }
+                ++n;
+            }
+            if (!ok) {   // leave with no copy of this CTA in flight
+                mbar_wait(&sh->q_full, 0, CT_WAIT_CYCLES);
+                if (uses[0]) mbar_wait(&sh->k_full, (uses[0] - 1) & 1, CT_WAIT_CYCLES);
+                if (uses[1]) mbar_wait(&sh->v_full, (uses[1] - 1) & 1, CT_WAIT_CYCLES);
+                if (uses[2]) mbar_wait(&sh->vh_full, (uses[2] - 1) & 1, CT_WAIT_CYCLES);
+            }
+        }
+    } else if (warp == CT_MMA_WARP) {
+        reg_dealloc<CT_REGS_OTHER>();
+        // ------------------------------------------------------------------ MMA issuer (the whole warp walks the loop, one elected lane issues)
+        const int ksteps = (p.dim + 15) >> 4;                    // of 16 channels; channels past the head read as zeros
+        const uint32_t idesc_pv = idesc_h16(CT_BM, 0, F16, true) | (static_cast<uint32_t>(ksteps * 2) << 17);
+        const uint64_t qd = smem_desc_sw128(smem_u32(q_s)), kd = smem_desc_sw128(smem_u32(k_s));
+        const uint64_t vd = smem_desc_sw128_mn(smem_u32(v_s), CT_HALF_BYTES, 1024);
+        const uint32_t hi_k = static_cast<uint32_t>(qd >> 32), hi_v = static_cast<uint32_t>(vd >> 32);
+        const uint32_t q_lo = static_cast<uint32_t>(qd), k_lo = static_cast<uint32_t>(kd), v_lo = static_cast<uint32_t>(vd);
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+            if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity, CT_WAIT_CYCLES))) {
+                if (lane == 0) timeout(code);
+                ok = false;
+            }
+            return ok;
+        };
+        auto next_block = [&](int j) {
+            while (j < nblocks && block_valid(j) == 0) ++j;
+            return j;
+        };
+        // S = Q K_j^T over the block's states, rounded up to 16
+        auto issue_qk = [&](int valid) {
+            const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((valid + 15) >> 4) << 18);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+                if (kk < ksteps) {
+                    const uint32_t off = (kk >> 2) * (CT_HALF_BYTES >> 4) + (kk & 3) * 2;
+                    tc_mma_f16_lo(tmem, q_lo + off, k_lo + off, hi_k, idesc, kk > 0);
+                }
+            tc_commit(&sh->s_full);
+            tc_commit(&sh->k_empty);
+        };
+        int j = next_block(0), n = 0, plain = 0, zeroed = 0, second = 0;   // blocks; of those: V as it lies, V with zeroed rows, more than 64 states
+        if (j < nblocks && wait(&sh->q_full, 0, 910) && wait(&sh->k_full, 0, 911)) {
+            tc_fence_after_sync();
+            if (elect_one()) issue_qk(block_valid(j));
+            __syncwarp();
+        }
+        while (ok && j < nblocks) {
+            const int valid = block_valid(j), steps = (valid + 15) >> 4;
+            const int jn = next_block(j + 1);
+            if (block_holes(j, valid)) {
+                if (!wait(&sh->v_zeroed, zeroed++ & 1, 921)) break;
+            } else {
+                if (!wait(&sh->v_full, plain++ & 1, 920)) break;
+            }
+            for (int hf = 0; hf < (valid > 64 ? 2 : 1); ++hf) {
+                if (!wait(&sh->p_half[hf], hf ? second++ & 1 : n & 1, 930 + hf)) break;
+                tc_fence_after_sync();
+                if (elect_one()) {
+#pragma unroll
+                    for (int k4 = 0; k4 < 4; ++k4)
+                        if (hf * 4 + k4 < steps)
+                            tc_mma_f16_ts_lo(tmem + CT_BN, tmem + hf * 64 + k4 * 8, v_lo + (hf * 4 + k4) * 128, hi_v, idesc_pv, (n | hf | k4) ? 1u : 0u);
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (elect_one()) {
+                tc_commit(&sh->pv_done);
+                tc_commit(&sh->v_empty);
+            }
+            __syncwarp();
+            ++n;
+            j = jn;
+            if (j < nblocks) {
+                if (!wait(&sh->k_full, n & 1, 940)) break;
+                tc_fence_after_sync();
+                if (elect_one()) issue_qk(block_valid(j));   // overwrites P: behind P V in the tensor pipe's order
+                __syncwarp();
+            }
+        }
+    } else if (warp >= CT_ZERO_WARP) {
+        reg_dealloc<CT_REGS_OTHER>();
+        // ------------------------------------------------------------------ rows of V that must not be seen -> zeros
+        if (warp == CT_ZERO_WARP) {
+            int n = 0;   // blocks with such rows
+            for (int j = 0; j < nblocks; ++j) {
+                const int valid = block_valid(j);
+                if (valid == 0) continue;
+                if (block_holes(j, valid)) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(&sh->vh_full, n & 1, CT_WAIT_CYCLES))) {
+                        if (lane == 0) timeout(950);
+                        break;
+                    }
+                    const int up = (valid + 15) & ~15;
+                    // four rows a turn, eight lanes per row (and half)
+                    for (int r0 = MASK ? 0 : valid & ~3; r0 < up; r0 += 4) {
+                        const int r = r0 + (lane >> 3);
+                        bool zero = r >= valid;
+                        if constexpr (MASK) zero = !((words[4 * j + (r >> 5)] >> (r & 31)) & 1u);
+                        if (zero && r < up)
+                            for (int h = 0; h < halves; ++h)
+                                *reinterpret_cast<uint4*>(v_s + h * CT_HALF_BYTES + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->v_zeroed);
+                    ++n;
+                }
+            }
+        }
+    } else {
+        reg_alloc<CT_REGS_SOFTMAX>();
+        // ------------------------------------------------------------------ softmax: thread = one query row
+        const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
+        const uint32_t s_tmem = tmem + lane_addr, o_tmem = s_tmem + CT_BN;
+        float m_used = 0.f, l = 0.f;
+        bool ok = true;
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+        // 64 states (two 32-column chunks of S) -> 32 columns of packed 16-bit pairs, and their sum
+        auto exp_half = [&](const uint32_t (&a)[32], const uint32_t (&b)[32], float m, uint32_t (&w)[32]) {
+            const float2 nm2 = make_float2(-m, -m);
+            float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const int e = (i & 15) * 2;
+                const float2 v = i < 16 ? make_float2(__uint_as_float(a[e]), __uint_as_float(a[e + 1]))
+                                        : make_float2(__uint_as_float(b[e]), __uint_as_float(b[e + 1]));
+                const float2 x = __ffma2_rn(v, sc2, nm2);
+                float2 r;
+                if ((i & 3) == 3) {   // a quarter on the FMA pipe, as in attention.cu
+                    r = exp2_fma2(x);
+                } else {
+                    r.x = ex2(x.x);
+                    r.y = ex2(x.y);
+                }
+                sum2[i & 1] = __fadd2_rn(sum2[i & 1], r);
+                w[i] = pack_h16<F16>(r.x, r.y);
+            }
+            return (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+        };
+        auto max_half = [&](const uint32_t (&a)[32], const uint32_t (&b)[32]) {
+            float m0 = __uint_as_float(a[0]), m1 = __uint_as_float(b[0]);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                m0 = max3(m0, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
+                m1 = max3(m1, __uint_as_float(b[i]), __uint_as_float(b[i + 1]));
+            }
+            return fmaxf(m0, m1);
+        };
+        // scores that do not count -> -inf (selected, not added: they may be anything)
+        auto hide = [&](uint32_t (&a)[32], int j, int chunk, int valid) {
+            if constexpr (MASK) {
+                const uint32_t bits = words[4 * j + chunk];
+                if (bits != 0xffffffffu) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!((bits >> i) & 1u)) a[i] = 0xff800000u;
+                }
+            } else if (valid < (chunk + 1) * 32) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (chunk * 32 + i >= valid) a[i] = 0xff800000u;
+            }
+        };
+        auto publish = [&](int hf, const uint32_t (&w)[32]) {
+            tc_st_32x32b_x32(s_tmem + hf * 64, w);   // over this thread's own S values, which are all in registers by now
+            tc_wait_st();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->p_half[hf]);
+        };
+        int n = 0;
+        for (int j = 0; j < nblocks; ++j) {
+            const int valid = block_valid(j);
+            if (valid == 0) continue;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh->s_full, n & 1, CT_WAIT_CYCLES))) {
+                if (lane == 0) timeout(960);
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            const bool two = valid > 64;
+            uint32_t s0[32], s1[32], s2[32], s3[32], w[32];
+            tc_ld_32x32b_x32(s_tmem, s0);
+            tc_ld_32x32b_x32(s_tmem + 32, s1);
+            tc_wait_ld();
+            if (two) {
+                tc_ld_32x32b_x32(s_tmem + 64, s2);
+                tc_ld_32x32b_x32(s_tmem + 96, s3);
+            }
+            hide(s0, j, 0, valid);
+            hide(s1, j, 1, valid);
+            float mx = max_half(s0, s1);
+            float sum_a = 0.f;
+            if (n > 0) sum_a = exp_half(s0, s1, m_used, w);   // with the maximum in use while the second half is on its way
+            if (two) {
+                tc_wait_ld();
+                hide(s2, j, 2, valid);
+                hide(s3, j, 3, valid);
+                mx = fmaxf(mx, max_half(s2, s3));
+            }
+            const float ms = mx * p.scale_log2;
+            const bool grow = n == 0 || ms > m_used + CT_RESCALE_STEP;
+            if (__any_sync(0xffffffffu, grow)) {
+                if (n > 0) {
+                    // O is written by the previous P V product until it has completed
+                    if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done, (n - 1) & 1, CT_WAIT_CYCLES))) {
+                        if (lane == 0) timeout(970);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const float alpha = grow ? ex2(m_used - ms) : 1.f;
+                    l *= alpha;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (c * 32 >= p.dim) break;
+                        uint32_t o[32];
+                        tc_ld_32x32b_x32(o_tmem + c * 32, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tc_st_32x32b_x32(o_tmem + c * 32, o);
+                    }
+                    tc_wait_st();
+                }
+                if (grow) {
+                    m_used = ms;
+                    sum_a = exp_half(s0, s1, m_used, w);
+                }
+            }
+            publish(0, w);
+            if (two) {
+                sum_a += exp_half(s2, s3, m_used, w);
+                publish(1, w);
+            }
+            l += sum_a;
+            ++n;
+        }
+        // ---- O / l through shared memory (over Q, which every product has read) to global memory
+        if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh->pv_done, (n - 1) & 1, CT_WAIT_CYCLES))) {
+            if (lane == 0) timeout(980);
+            ok = false;
+        }
+        if (ok) {
+            tc_fence_after_sync();
+            const float inv = n > 0 ? 1.f / l : 0.f;
+            const int row = warp * 32 + lane;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (c * 32 >= p.dim) break;
+                uint32_t o[32];
+                if (n > 0) {
+                    tc_ld_32x32b_x32(o_tmem + c * 32, o);
+                    tc_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0u;   // no states: zeros
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t w4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w4[e] = pack_h16<F16>(__uint_as_float(o[u * 8 + 2 * e]) * inv, __uint_as_float(o[u * 8 + 2 * e + 1]) * inv);
+                    // 16-byte piece (c & 1) * 4 + u of the row's 128 bytes, where the 128-byte swizzle puts it
+                    *reinterpret_cast<uint4*>(q_s + (c >> 1) * CT_HALF_BYTES + row * 128 + ((((c & 1) * 4 + u) ^ (row & 7)) << 4)) =
+                        make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (q0 + warp * 32 < p.q_len)
+                    for (int h = 0; h < halves; ++h)
+                        tma_store_4d(&tm_o, q_s + h * CT_HALF_BYTES + warp * 32 * 128, h * 64, q0 + warp * 32, head, batch);
+                bulk_commit_group();
+                bulk_wait_group_read<0>();
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == CT_MMA_WARP) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, CT_TMEM_COLS);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- few query rows
+constexpr int CR_THREADS = 128, CR_KEYS = 64, CR_STAGES = 3, CR_ROWS = 16, CR_MAX_SPLIT = 8;
+
+struct CrossRowsParams {
+    CrossStates st;
+    const uint8_t *q, *k, *v;
+    uint8_t* out;
+    long long qs[3], ks[3], vs[3], os[3];   // batch, head, token strides in bytes
+    int kv_heads, group, q_rows, dim;       // q_rows = q_len * group: row r is query r / group, head kv_head * group + r % group
+    float scale_log2;
+};
+
+template <int NK>
+struct CrossRowsSizes {
+    static constexpr int ROW = (2 * NK + 1) * 16;           // bytes of a state's row: an odd number of 16-byte pieces, so that ldmatrix has no conflicts
+    static constexpr int TILE = CR_KEYS * ROW;
+    static constexpr int STAGE = 2 * TILE;
+    static constexpr int SMEM = CR_STAGES * STAGE;
+    static constexpr int COLS = NK * 16;
+    // afterwards: four warps' partial sums [4][16][COLS], the CTA's [16][COLS], maxima and sums [5][16] each
+    static_assert(SMEM >= 5 * CR_ROWS * COLS * 4 + 2 * 5 * CR_ROWS * 4, "the partial sums lie over the ring");
+};
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {   // writes zeros where not valid (src is not read)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const void* src) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(src)) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* src) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(src)) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma_16816_t(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t addr) { return __int_as_float(ld_shared_cluster_s32(addr)); }
+
+// grid (batch * kv_heads * split, row tiles), cluster (split, 1, 1)
+template <bool F16, int NK>
+__global__ void __launch_bounds__(CR_THREADS)
+cross_rows_kernel(const CrossRowsParams p, const int split) {
+    using S = CrossRowsSizes<NK>;
+    extern __shared__ __align__(1024) uint8_t cr_smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int pairix = blockIdx.x / split, batch = pairix / p.kv_heads, kv_head = pairix % p.kv_heads;
+    const int r0 = blockIdx.y * CR_ROWS;
+    int start, count;
+    cross_range(p.st, batch, start, count);
+    const int tiles = (count + CR_KEYS - 1) / CR_KEYS;
+    const int t0 = static_cast<int>(static_cast<long long>(tiles) * rank / split), t1 = static_cast<int>(static_cast<long long>(tiles) * (rank + 1) / split);
+    const uint8_t* kbase = p.k + kv_head * p.ks[1] + (p.st.kv_offsets ? start * p.ks[2] : batch * p.ks[0]);
+    const uint8_t* vbase = p.v + kv_head * p.vs[1] + (p.st.kv_offsets ? start * p.vs[2] : batch * p.vs[0]);
+    const uint8_t* mask = p.st.mask ? p.st.mask + batch * p.st.mask_stride : nullptr;
+
+    auto load_tile = [&](int tile, int slot) {
+        uint8_t* ks = cr_smem + slot * S::STAGE;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const int idx = tid + i * CR_THREADS, r = idx / (2 * NK), c = idx % (2 * NK);
+            const int key = tile * CR_KEYS + r;
+            bool valid = key < count && c * 8 < p.dim;
+            if (mask && valid) valid = mask[key] != 0;
+            const uint8_t* ksrc = valid ? kbase + key * p.ks[2] + c * 16 : p.k;
+            const uint8_t* vsrc = valid ? vbase + key * p.vs[2] + c * 16 : p.v;
+            cp_async16(ks + r * S::ROW + c * 16, ksrc, valid);
+            cp_async16(ks + S::TILE + r * S::ROW + c * 16, vsrc, valid);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < CR_STAGES - 1; ++s) {
+        if (t0 + s < t1) load_tile(t0 + s, s);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // query fragments: rows g and g + 8
+    uint32_t qf[NK][4];
+    {
+        const uint8_t* qrow[2];
+        bool there[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = r0 + g + 8 * i;
+            there[i] = r < p.q_rows;
+            qrow[i] = p.q + batch * p.qs[0] + (kv_head * p.group + (there[i] ? r % p.group : 0)) * p.qs[1] + (there[i] ? r / p.group : 0) * p.qs[2];
+        }
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int ch = kk * 16 + (i >> 1) * 8 + 2 * t;
+                qf[kk][i] = there[i & 1] && ch < p.dim ? *reinterpret_cast<const uint32_t*>(qrow[i & 1] + 2 * ch) : 0u;
+            }
+    }
+    float o[2 * NK][4];
+#pragma unroll
+    for (int i = 0; i < 2 * NK; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int tile = t0; tile < t1; ++tile) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(CR_STAGES - 2) : "memory");
+        __syncthreads();   // the tile has landed for every thread, and every warp has left the slot that is filled next
+        if (tile + CR_STAGES - 1 < t1) load_tile(tile + CR_STAGES - 1, (tile - t0 + CR_STAGES - 1) % CR_STAGES);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const uint8_t* ks = cr_smem + ((tile - t0) % CR_STAGES) * S::STAGE + warp * 16 * S::ROW;
+        const uint8_t* vs = ks + S::TILE;
+        const int key0 = tile * CR_KEYS + warp * 16;
+        if (key0 >= count) continue;
+        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+            uint32_t b[4];
+            ldmatrix_x4(b, ks + ((lane >> 4) * 8 + (lane & 7)) * S::ROW + (kk * 2 + ((lane >> 3) & 1)) * 16);
+            mma_16816_t<F16>(s[0], qf[kk], b[0], b[1]);
+            mma_16816_t<F16>(s[1], qf[kk], b[2], b[3]);
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = key0 + i * 8 + 2 * t + (e & 1);
+                const bool seen = key < count && (!mask || mask[key] != 0);
+                s[i][e] = seen ? s[i][e] * p.scale_log2 : -INFINITY;
+                top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
+            }
+        float alpha[2], base[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+            const float mn = fmaxf(m[i], top[i]);
+            base[i] = mn == -INFINITY ? 0.f : mn;         // nothing seen yet: every exponential below is 2^-inf = 0
+            alpha[i] = ex2(m[i] - base[i]);
+            m[i] = mn;
+            l[i] *= alpha[i];
+        }
+        uint32_t pf[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float e[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) e[q] = ex2(s[i][q] - base[q >> 1]);
+            l[0] += e[0] + e[1];
+            l[1] += e[2] + e[3];
+            pf[2 * i] = pack_h16<F16>(e[0], e[1]);
+            pf[2 * i + 1] = pack_h16<F16>(e[2], e[3]);
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < 2 * NK; ++i) {
+                o[i][0] *= alpha[0];
+                o[i][1] *= alpha[0];
+                o[i][2] *= alpha[1];
+                o[i][3] *= alpha[1];
+            }
+        }
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, vs + (((lane >> 3) & 1) * 8 + (lane & 7)) * S::ROW + (kk * 2 + (lane >> 4)) * 16);
+            mma_16816_t<F16>(o[2 * kk], pf, b[0], b[1]);
+            mma_16816_t<F16>(o[2 * kk + 1], pf, b[2], b[3]);
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    // ---- join the four warps, then the CTAs of the cluster
+    const int rows = min(CR_ROWS, p.q_rows - r0);
+    float* part = reinterpret_cast<float*>(cr_smem);               // [4][16][COLS]
+    float* mine = part + 4 * CR_ROWS * S::COLS;                    // [16][COLS]
+    float* pm = mine + CR_ROWS * S::COLS;                          // [5][16]: the warps' maxima, then the CTA's
+    float* pl = pm + 5 * CR_ROWS;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (t == 0) {
+            pm[warp * CR_ROWS + g + 8 * i] = m[i];
+            pl[warp * CR_ROWS + g + 8 * i] = l[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NK; ++i) {
+        *reinterpret_cast<float2*>(part + (warp * CR_ROWS + g) * S::COLS + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
+        *reinterpret_cast<float2*>(part + (warp * CR_ROWS + g + 8) * S::COLS + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
+    }
+    __syncthreads();
+    for (int idx = tid; idx < rows * S::COLS; idx += CR_THREADS) {
+        const int r = idx / S::COLS, c = idx % S::COLS;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, pm[w * CR_ROWS + r]);
+        const float b = mm == -INFINITY ? 0.f : mm;
+        float sum = 0.f, ls = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = ex2(pm[w * CR_ROWS + r] - b);
+            sum = fmaf(f, part[(w * CR_ROWS + r) * S::COLS + c], sum);
+            ls = fmaf(f, pl[w * CR_ROWS + r], ls);
+        }
+        mine[idx] = sum;
+        if (c == 0) {
+            pm[4 * CR_ROWS + r] = mm;
+            pl[4 * CR_ROWS + r] = ls;
+        }
+    }
+    if (split > 1) cluster_sync_all();
+    else __syncthreads();
+    const int half = p.dim >> 1;
+    for (int idx = rank * CR_THREADS + tid; idx < rows * half; idx += split * CR_THREADS) {
+        const int r = idx / half, c = (idx % half) * 2;
+        float mm = -INFINITY;
+        for (int q = 0; q < split; ++q) {
+            const float v = split > 1 ? ld_shared_cluster_f32(mapa_shared(smem_u32(pm + 4 * CR_ROWS + r), q)) : pm[4 * CR_ROWS + r];
+            mm = fmaxf(mm, v);
+        }
+        const float b = mm == -INFINITY ? 0.f : mm;
+        float x = 0.f, y = 0.f, ls = 0.f;
+        for (int q = 0; q < split; ++q) {
+            if (split > 1) {
+                const float f = ex2(ld_shared_cluster_f32(mapa_shared(smem_u32(pm + 4 * CR_ROWS + r), q)) - b);
+                const uint32_t a = mapa_shared(smem_u32(mine + r * S::COLS + c), q);
+                x = fmaf(f, ld_shared_cluster_f32(a), x);
+                y = fmaf(f, ld_shared_cluster_f32(a + 4), y);
+                ls = fmaf(f, ld_shared_cluster_f32(mapa_shared(smem_u32(pl + 4 * CR_ROWS + r), q)), ls);
+            } else {
+                x = mine[r * S::COLS + c];
+                y = mine[r * S::COLS + c + 1];
+                ls = pl[4 * CR_ROWS + r];
+            }
+        }
+        const float inv = mm == -INFINITY && ls == 0.f ? 0.f : 1.f / ls;   // nothing seen: zeros
+        const int row = r0 + r;
+        uint8_t* dst = p.out + batch * p.os[0] + (kv_head * p.group + row % p.group) * p.os[1] + (row / p.group) * p.os[2] + 2 * c;
+        *reinterpret_cast<uint32_t*>(dst) = pack_h16<F16>(x * inv, y * inv);
+    }
+    if (split > 1) cluster_sync_all();   // peers may still read this CTA's sums
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+struct CrossTensor {
+    const void* base;
+    int64_t stride[3];   // batch, head, token
+    int batch, heads, tokens;
+};
+
+// 4-D tiled map (channel, token, head, batch).  A dimension of one, or broadcast with stride 0, is encoded with one entry and some
+// valid stride; *bmul / *hmul say whether its coordinate counts.
+static int cross_tmap(CUtensorMap* map, const CrossTensor& t, int dim, int dtype, int box_rows, int* bmul, int* hmul) {
+    const int64_t any = dim;   // a multiple of 8
+    *bmul = t.batch > 1 && t.stride[0] != 0;
+    *hmul = t.heads > 1 && t.stride[1] != 0;
+    const uint64_t dims[4] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(t.tokens), static_cast<uint64_t>(*hmul ? t.heads : 1),
+                              static_cast<uint64_t>(*bmul ? t.batch : 1)};
+    const uint64_t strides[3] = {2 * static_cast<uint64_t>(t.tokens > 1 ? t.stride[2] : any), 2 * static_cast<uint64_t>(*hmul ? t.stride[1] : any),
+                                 2 * static_cast<uint64_t>(*bmul ? t.stride[0] : any)};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), 1, 1};
+    return make_tmap_nd(map, t.base, dtype == SVDQ_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims, strides,
+                        box, true);
+}
+
+template <bool F16, bool MASK>
+static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const CrossTileParams& p,
+                             dim3 grid, cudaStream_t stream) {
+    auto kern = cross_tile_kernel<F16, MASK>;
+    static std::atomic<uint64_t> attr_done{0};
+    if (int rc = ensure_dynamic_smem(kern, CT_SMEM + (MASK ? CT_MASK_STATES / 8 : 0), attr_done)) return rc;
+    const int smem = CT_SMEM + (MASK ? (p.st.kv_len + CT_BN - 1) / CT_BN * (CT_BN / 8) : 0);
+    kern<<<grid, CT_THREADS, smem, stream>>>(tq, tk, tv, to, p);
+    SVDQ_CUDA(cudaGetLastError());
+    return SVDQ_OK;
+}
+
+template <bool F16, int NK>
+static int launch_cross_rows(const CrossRowsParams& p, int pairs, int split, cudaStream_t stream) {
+    auto kern = cross_rows_kernel<F16, NK>;
+    static std::atomic<uint64_t> attr_done{0};
+    if (int rc = ensure_dynamic_smem(kern, CrossRowsSizes<NK>::SMEM, attr_done)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(pairs * split, (p.q_rows + CR_ROWS - 1) / CR_ROWS, 1);
+    cfg.blockDim = dim3(CR_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = CrossRowsSizes<NK>::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, p, split));
+    return SVDQ_OK;
+}
+
+template <bool F16>
+static int launch_cross_rows_dim(const CrossRowsParams& p, int pairs, int split, cudaStream_t stream) {
+    switch ((p.dim + 15) / 16) {
+        case 1: return launch_cross_rows<F16, 1>(p, pairs, split, stream);
+        case 2: return launch_cross_rows<F16, 2>(p, pairs, split, stream);
+        case 3: return launch_cross_rows<F16, 3>(p, pairs, split, stream);
+        case 4: return launch_cross_rows<F16, 4>(p, pairs, split, stream);
+        case 5: return launch_cross_rows<F16, 5>(p, pairs, split, stream);
+        case 6: return launch_cross_rows<F16, 6>(p, pairs, split, stream);
+        case 7: return launch_cross_rows<F16, 7>(p, pairs, split, stream);
+        default: return launch_cross_rows<F16, 8>(p, pairs, split, stream);
+    }
+}
+
+}  // namespace svdq
+
+extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* stream) {
+    using namespace svdq;
+    SVDQ_CHECK_ARG(a && a->q && a->k && a->v && a->out, "cross_attention: null tensor pointer");
+    SVDQ_CHECK_ARG(a->batch > 0 && a->heads > 0 && a->kv_heads > 0 && a->q_len > 0 && a->kv_len > 0 && a->batch <= 65535 && a->heads <= 65535,
+                   "cross_attention: bad sizes");
+    SVDQ_CHECK_ARG(a->heads % a->kv_heads == 0, "cross_attention: kv_heads (%d) must divide heads (%d)", a->kv_heads, a->heads);
+    SVDQ_CHECK_ARG(a->head_dim > 0 && a->head_dim <= 128 && a->head_dim % 8 == 0, "cross_attention: head_dim %d (multiples of 8 up to 128)", a->head_dim);
+    SVDQ_CHECK_ARG(a->dtype == SVDQ_DTYPE_BF16 || a->dtype == SVDQ_DTYPE_FP16, "cross_attention: bad dtype %d", a->dtype);
+    SVDQ_CHECK_ARG(a->scale > 0.f && a->scale < 3e38f, "cross_attention: scale must be positive");
+    SVDQ_CHECK_ARG((a->kv_lens != nullptr) + (a->kv_offsets != nullptr) + (a->mask != nullptr) <= 1,
+                   "cross_attention: at most one of kv_lens, kv_offsets and mask");
+    SVDQ_CHECK_ARG(!a->mask || a->mask_stride >= 0, "cross_attention: the mask's row stride must not be negative");
+    SVDQ_CHECK_ARG(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16) && aligned(a->kv_lens, 4) && aligned(a->kv_offsets, 4),
+                   "cross_attention: tensors must be 16-byte aligned");
+    const int kv_batch = a->kv_offsets ? 1 : a->batch;
+    const CrossTensor tq = {a->q, {a->q_stride[0], a->q_stride[1], a->q_stride[2]}, a->batch, a->heads, a->q_len};
+    const CrossTensor tk = {a->k, {a->k_stride[0], a->k_stride[1], a->k_stride[2]}, kv_batch, a->kv_heads, a->kv_len};
+    const CrossTensor tv = {a->v, {a->v_stride[0], a->v_stride[1], a->v_stride[2]}, kv_batch, a->kv_heads, a->kv_len};
+    const CrossTensor to = {a->out, {a->o_stride[0], a->o_stride[1], a->o_stride[2]}, a->batch, a->heads, a->q_len};
+    for (const CrossTensor* t : {&tq, &tk, &tv, &to}) {
+        const int size[3] = {t->batch, t->heads, t->tokens};
+        for (int i = 0; i < 3; ++i) {
+            const int64_t s = t->stride[i];
+            SVDQ_CHECK_ARG(size[i] == 1 || (s % 8 == 0 && s >= 0 && s < (1ll << 38)), "cross_attention: strides must be multiples of 8 elements");
+            SVDQ_CHECK_ARG(size[i] == 1 || s >= a->head_dim || (s == 0 && i < 2 && t != &to),
+                           "cross_attention: strides must be at least head_dim (batch and head strides of q, k and v may be 0)");
+        }
+    }
+    const int group = a->heads / a->kv_heads;
+    const long long q_rows = static_cast<long long>(a->q_len) * group;
+    if (a->mask && a->kv_len > CT_MASK_STATES)
+        return fail(SVDQ_ERR_UNSUPPORTED, "cross_attention: a mask covers at most %d states (got %d)", CT_MASK_STATES, a->kv_len);
+    if (int rc = check_arch()) return rc;
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool f16 = a->dtype == SVDQ_DTYPE_FP16;
+    const CrossStates states = {a->kv_lens, a->kv_offsets, static_cast<const uint8_t*>(a->mask), a->mask_stride, a->kv_len};
+    const float scale_log2 = a->scale * 1.4426950408889634f;
+    const long long kv_pairs = static_cast<long long>(a->batch) * a->kv_heads;
+    if (q_rows <= CR_ROWS && kv_pairs * CR_MAX_SPLIT < (1ll << 31)) {
+        CrossRowsParams p = {};
+        p.st = states;
+        p.q = static_cast<const uint8_t*>(a->q);
+        p.k = static_cast<const uint8_t*>(a->k);
+        p.v = static_cast<const uint8_t*>(a->v);
+        p.out = static_cast<uint8_t*>(a->out);
+        for (int i = 0; i < 3; ++i) {
+            p.qs[i] = 2 * a->q_stride[i];
+            p.ks[i] = 2 * a->k_stride[i];
+            p.vs[i] = 2 * a->v_stride[i];
+            p.os[i] = 2 * a->o_stride[i];
+        }
+        p.kv_heads = a->kv_heads;
+        p.group = group;
+        p.q_rows = static_cast<int>(q_rows);
+        p.dim = a->head_dim;
+        p.scale_log2 = scale_log2;
+        // states per sample as far as the host knows
+        const long long len = a->kv_offsets ? (a->kv_len + a->batch - 1) / a->batch : a->kv_len;
+        const long long tiles = (len + CR_KEYS - 1) / CR_KEYS, ctas = kv_pairs * ((q_rows + CR_ROWS - 1) / CR_ROWS);
+        int split = 1;
+        while (split < CR_MAX_SPLIT && ctas * split < 2ll * sms && 2 * split <= tiles) split *= 2;
+        return f16 ? launch_cross_rows_dim<true>(p, static_cast<int>(kv_pairs), split, st) : launch_cross_rows_dim<false>(p, static_cast<int>(kv_pairs), split, st);
+    }
+    CrossTileParams p = {};
+    p.st = states;
+    p.q_len = a->q_len;
+    p.dim = a->head_dim;
+    p.group = group;
+    p.scale_log2 = scale_log2;
+    if (int rc = status_words(&p.status)) return rc;
+    CUtensorMap mq, mk, mv, mo;
+    int obm, ohm;
+    if (int rc = cross_tmap(&mq, tq, a->head_dim, a->dtype, CT_BM, &p.q_bmul, &p.q_hmul)) return rc;
+    if (int rc = cross_tmap(&mk, tk, a->head_dim, a->dtype, CT_BN / 2, &p.k_bmul, &p.k_hmul)) return rc;
+    if (int rc = cross_tmap(&mv, tv, a->head_dim, a->dtype, CT_BN / 2, &p.v_bmul, &p.v_hmul)) return rc;
+    if (int rc = cross_tmap(&mo, to, a->head_dim, a->dtype, 32, &obm, &ohm)) return rc;
+    const dim3 grid((a->q_len + CT_BM - 1) / CT_BM, a->heads, a->batch);
+    if (a->mask) return f16 ? launch_cross_tile<true, true>(mq, mk, mv, mo, p, grid, st) : launch_cross_tile<false, true>(mq, mk, mv, mo, p, grid, st);
+    return f16 ? launch_cross_tile<true, false>(mq, mk, mv, mo, p, grid, st) : launch_cross_tile<false, false>(mq, mk, mv, mo, p, grid, st);
+}

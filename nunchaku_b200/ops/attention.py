@@ -62,3 +62,79 @@ def attention_fp16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.T
     """The reference's call (nunchaku/csrc/ops.h:112-118): q, k, v packed [B, H, T, 128], o [B, Tq, H*128], written in place.
     The reference takes fp16 inputs with a bf16 or fp16 output; here all four share one 16-bit type."""
     attention(q, k, v, out=o, scale=scale)
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: torch.Tensor | None = None,
+                    mask: torch.Tensor | None = None, kv_offsets: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    scale: float | None = None) -> torch.Tensor:
+    """``softmax(scale * q k^T) v`` of queries over an encoder's states of another length (``MultiHeadCrossAttention``,
+    src/SanaModel.cpp:138-190), over the states that exist for each sample.
+
+    q: [B, H, Tq, D]; k, v: [B, Hk, T, D] views with any (batch, head, token) strides (multiples of 8 elements; batch and head may be
+    expanded), bf16 or fp16, D a multiple of 8 up to 128, H a multiple of Hk (query head h reads stored head h // (H // Hk)).
+    Which states exist, at most one of: ``kv_lens`` int32 [B] (the first so many of each sample), ``mask`` bool [B, T] (those that are
+    True; T up to 65536), ``kv_offsets`` int32 [B + 1] (k and v are then packed [total, Hk, D], sample b owning rows
+    ``kv_offsets[b]:kv_offsets[b + 1]``); all on q's device, read there (lengths outside 0..T are clamped).  None: all T.  A sample without
+    states gets zeros; states that do not exist may hold anything, NaN included.
+    out: [B, Tq, H*D] (default: a new tensor) or a [B, H, Tq, D] view of one.  scale defaults to D ** -0.5 and must be positive."""
+    dtype, dev = q.dtype, q.device
+    if not q.is_cuda or dtype not in HALF_DTYPES:
+        raise ValueError("q must be a CUDA bf16 / fp16 tensor (this library has no CPU path)")
+    if k.dtype != dtype or v.dtype != dtype or k.device != dev or v.device != dev:
+        raise ValueError("k and v must have q's dtype and device")
+    if q.dim() != 4:
+        raise ValueError("q must be [batch, heads, tokens, D]")
+    B, H, Tq, D = q.shape
+    if (kv_lens is not None) + (mask is not None) + (kv_offsets is not None) > 1:
+        raise ValueError("at most one of kv_lens, mask and kv_offsets")
+    if k.shape != v.shape:
+        raise ValueError("k and v must have the same shape")
+    lens_ptr = off_ptr = mask_ptr = None
+    mask_stride = 0
+    if kv_offsets is not None:
+        if k.dim() != 3 or k.shape[2] != D:
+            raise ValueError("with kv_offsets, k and v are packed [total, kv_heads, D]")
+        T, Hk = k.shape[0], k.shape[1]
+        ks, vs = (0, k.stride(1), k.stride(0)), (0, v.stride(1), v.stride(0))
+        if kv_offsets.dtype != torch.int32 or kv_offsets.device != dev or kv_offsets.shape != (B + 1,) or not kv_offsets.is_contiguous():
+            raise ValueError("kv_offsets must be a contiguous int32 [batch + 1] on q's device")
+        off_ptr = kv_offsets.data_ptr()
+    else:
+        if k.dim() != 4 or k.shape[0] != B or k.shape[3] != D:
+            raise ValueError("k and v must be [batch, kv_heads, tokens, D] with q's batch and D")
+        Hk, T = k.shape[1], k.shape[2]
+        ks, vs = k.stride()[:3], v.stride()[:3]
+        if kv_lens is not None:
+            if kv_lens.dtype != torch.int32 or kv_lens.device != dev or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
+                raise ValueError("kv_lens must be a contiguous int32 [batch] on q's device")
+            lens_ptr = kv_lens.data_ptr()
+        elif mask is not None:
+            if mask.dtype != torch.bool or mask.device != dev or mask.shape != (B, T) or (mask.stride(1) != 1 and T > 1):
+                raise ValueError("mask must be bool [batch, tokens] on q's device with unit token stride")
+            mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0)
+    if q.stride(3) != 1 or k.stride(-1) != 1 or v.stride(-1) != 1:
+        raise ValueError("the last dimension of q, k and v must be contiguous")
+    if min(B, H, Tq, D, Hk, T) == 0:
+        raise ValueError("cross_attention: empty tensors (where no sample has states, k and v still need one row, of any content)")
+    ret = out
+    if out is None:
+        ret = torch.empty((B, Tq, H * D), dtype=dtype, device=dev)
+        os = (Tq * H * D, D, H * D)
+    else:
+        if out.dtype != dtype or out.device != dev:
+            raise ValueError("out must have q's dtype and device")
+        if out.dim() == 3:
+            if out.shape != (B, Tq, H * D) or out.stride(2) != 1:
+                raise ValueError("out must be [batch, tokens_q, heads*D] with unit channel stride")
+            os = (out.stride(0), D, out.stride(1))
+        else:
+            if out.shape != q.shape or out.stride(3) != 1:
+                raise ValueError("out must be [batch, tokens_q, heads*D] or [batch, heads, tokens_q, D]")
+            os = out.stride()[:3]
+    i3 = ctypes.c_int64 * 3
+    args = _lib.CrossAttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), ret.data_ptr(), i3(*q.stride()[:3]), i3(*ks), i3(*vs), i3(*os),
+                                   lens_ptr, off_ptr, mask_ptr, mask_stride, B, H, Hk, Tq, T, D,
+                                   float(D ** -0.5 if scale is None else scale), dtype_code(dtype))
+    with on_device(dev):
+        _lib.check(_lib.load().svdq_cross_attention(ctypes.byref(args), stream_ptr(dev)))
+    return ret

@@ -1,0 +1,266 @@
+"""Cross attention against fp64 softmax attention on the CPU.
+
+Tolerance, per output element o = sum_i p_i v_i / sum_i p_i with A = sum_i p_i |v_i| / sum_i p_i: the probabilities are rounded to the
+16-bit type (half a step: eps / 2 relative), a quarter of the exponentials is a cubic good to 7.6e-5 (it acts on p and on the sum),
+a score is off by at most d = (D + 3) 2^-24 scale max_i sum_c |q_c k_c| (fp32 accumulation over D channels, scale, exponent), which moves
+p and the sum; the fp32 sums over blocks, warps and CTAs add less than 2^-16.  fp16 probabilities below 2^-14 lose at most 2^-25
+each, against a sum of at least 1 (the maximum in use is one of the row's own scores and never above the largest).  The output itself: half a step of o."""
+import pytest
+import torch
+
+from nunchaku_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _keep(B, T, kv_lens=None, mask=None):
+    if mask is not None:
+        return mask.cpu()
+    if kv_lens is not None:
+        return torch.arange(T) < kv_lens.cpu().clamp(0, T)[:, None]
+    return torch.ones(B, T, dtype=torch.bool)
+
+
+def _exact(q, k, v, keep, scale):
+    """q [B, H, Tq, D], k, v [B, Hk, T, D], keep [B, T]; returns the output and its tolerance, both [B, Tq, H*D] in fp64."""
+    B, H, Tq, D = q.shape
+    eps = torch.finfo(q.dtype).eps
+    out, tol = torch.zeros(B, Tq, H, D, dtype=torch.float64), torch.zeros(B, Tq, H, D, dtype=torch.float64)
+    group = H // k.shape[1]
+    for b in range(B):
+        idx = keep[b].nonzero().squeeze(1)
+        if len(idx) == 0:
+            continue
+        kb, vb = k[b][:, idx].double().repeat_interleave(group, 0), v[b][:, idx].double().repeat_interleave(group, 0)
+        qb = q[b].double()
+        w = torch.softmax(scale * (qb @ kb.transpose(1, 2)), dim=-1)
+        d = (D + 3) * 2.0 ** -24 * scale * (qb.abs() @ kb.abs().transpose(1, 2)).amax(-1, keepdim=True)
+        o, a = w @ vb, w @ vb.abs()
+        t = a * (eps / 2 + 2 * 7.6e-5 + 2.0 ** -16 + 2 * d) + o.abs() * eps / 2
+        if q.dtype == torch.float16:
+            t += 2.0 ** -25 * vb.abs().sum(1, keepdim=True) + 2.0 ** -25
+        out[b], tol[b] = o.transpose(0, 1), t.transpose(0, 1) + 1e-30
+    return out.reshape(B, Tq, H * D), tol.reshape(B, Tq, H * D)
+
+
+def _check(got, q, k, v, keep, scale):
+    torch.cuda.synchronize()
+    assert _lib.device_status() == (0, 0)
+    exp, tol = _exact(q.cpu(), k.cpu(), v.cpu(), keep, scale)
+    got = got.cpu()
+    assert got.shape == exp.shape and got.dtype == q.dtype
+    err = (got.double() - exp).abs()
+    assert (err <= tol).all(), f"largest error over tolerance {(err / tol).max().item()}"
+    assert (got[~keep.any(1)] == 0).all()
+
+
+def _inputs(B, H, Hk, Tq, T, D, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(B, Tq, H, D, generator=g).to(dtype).cuda().transpose(1, 2)
+    kv = torch.randn(B, T, 2, Hk, D, generator=g).to(dtype).cuda()
+    return q, kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+
+
+# few query rows, one tile, ragged tiles; one state, ragged blocks, exact blocks, many blocks; head widths of every step count
+SIZES = [(1, 1, 1, 1, 1, 8), (1, 20, 20, 1, 300, 112), (3, 4, 2, 1, 65, 128), (2, 6, 2, 5, 129, 40), (2, 2, 2, 16, 64, 64), (1, 3, 1, 2, 1000, 72),
+         (1, 2, 2, 17, 1, 16), (2, 3, 3, 128, 128, 64), (1, 4, 2, 129, 300, 112), (2, 2, 1, 33, 77, 8), (1, 2, 2, 300, 16, 128), (2, 2, 2, 200, 257, 96),
+         (1, 2, 1, 64, 190, 24), (1, 1, 1, 100, 1153, 80), (3, 1, 1, 40, 64, 48), (1, 2, 2, 70, 192, 104)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,Hk,Tq,T,D", SIZES)
+def test_all_states(B, H, Hk, Tq, T, D, dtype):
+    from nunchaku_b200.ops import cross_attention
+
+    q, k, v = _inputs(B, H, Hk, Tq, T, D, dtype, seed=Tq + T + D)
+    _check(cross_attention(q, k, v), q, k, v, _keep(B, T), D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Tq", [1, 5, 150])
+@pytest.mark.parametrize("H,Hk,T,D", [(2, 2, 300, 112), (4, 2, 128, 64), (3, 3, 700, 128), (2, 1, 40, 32)])
+def test_lengths_with_nan_behind_them(Tq, H, Hk, T, D, dtype):
+    from nunchaku_b200.ops import cross_attention
+
+    lens = torch.tensor([0, 1, T, T - 3, min(T, 64), min(T, 129), 17, T + 50, -4], dtype=torch.int32)   # the last two are clamped
+    B = len(lens)
+    q, k, v = _inputs(B, H, Hk, Tq, T, D, dtype, seed=T + Tq)
+    keep = _keep(B, T, kv_lens=lens)
+    ck, cv = k.clone(), v.clone()
+    hidden = ~keep.cuda()[:, None, :, None]
+    k.masked_fill_(hidden, float("nan"))
+    v.masked_fill_(hidden, float("inf"))
+    got = cross_attention(q, k, v, kv_lens=lens.cuda())
+    _check(got, q, ck, cv, keep, D ** -0.5)
+    v.masked_fill_(hidden, float("nan"))
+    k.masked_fill_(hidden, torch.finfo(dtype).min)
+    assert torch.equal(cross_attention(q, k, v, kv_lens=lens.cuda()), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Tq", [1, 3, 140])
+@pytest.mark.parametrize("H,Hk,T,D", [(2, 2, 77, 64), (2, 1, 520, 112), (1, 1, 1, 128), (4, 4, 300, 32)])
+def test_masks(Tq, H, Hk, T, D, dtype):
+    from nunchaku_b200.ops import cross_attention
+
+    g = torch.Generator().manual_seed(T)
+    mask = torch.rand(7, T, generator=g) < 0.6
+    mask[0] = True
+    mask[1] = False                                  # no states
+    mask[2] = False
+    mask[2, T - 1] = True                            # only the last: the blocks before it are skipped
+    mask[3] = False
+    mask[3, 0] = True
+    mask[4, 64 if T > 64 else 0:] = False            # leading states only
+    if T > 400:
+        mask[5, 100:400] = False                     # empty blocks between others
+    B = len(mask)
+    q, k, v = _inputs(B, H, Hk, Tq, T, D, dtype, seed=T + Tq)
+    ck, cv = k.clone(), v.clone()
+    hidden = ~mask.cuda()[:, None, :, None]
+    k.masked_fill_(hidden, float("inf"))
+    v.masked_fill_(hidden, float("nan"))
+    wide = torch.ones(B, T + 5, dtype=torch.bool, device="cuda")
+    wide[:, :T] = mask.cuda()
+    _check(cross_attention(q, k, v, mask=wide[:, :T]), q, ck, cv, mask, D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Tq", [1, 6, 200])
+@pytest.mark.parametrize("H,Hk,D", [(2, 2, 112), (4, 2, 64), (3, 1, 128)])
+def test_packed(Tq, H, Hk, D, dtype):
+    from nunchaku_b200.ops import cross_attention
+
+    lens = [300, 0, 5, 128, 1, 64, 0, 213]
+    B, T = len(lens), max(lens)
+    off = torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32)
+    q, kp, vp = _inputs(B, H, Hk, Tq, T, D, dtype, seed=Tq + D)
+    keep = _keep(B, T, kv_lens=torch.tensor(lens))
+    total = sum(lens)
+    packed = torch.full((total + 9, 2, Hk, D), float("nan"), dtype=dtype, device="cuda")   # rows behind the last sample: NaN
+    for b, n in enumerate(lens):
+        packed[off[b]:off[b] + n, 0] = kp[b, :, :n].transpose(0, 1)
+        packed[off[b]:off[b] + n, 1] = vp[b, :, :n].transpose(0, 1)
+    got = cross_attention(q, packed[:, 0], packed[:, 1], kv_offsets=off.cuda())
+    _check(got, q, kp, vp, keep, D ** -0.5)
+    packed[off[3]:off[4]] = float("nan")             # one sample's states: nobody else's business
+    again = cross_attention(q, packed[:, 0], packed[:, 1], kv_offsets=off.cuda())
+    others = [b for b in range(B) if b != 3]
+    assert torch.equal(again[others], got[others]) and again[3].isnan().all()
+    # offsets that point outside are clamped to the rows there are
+    bad = off.clone()
+    bad[-1] = total + 1000
+    full = cross_attention(q, packed[:total, 0], packed[:total, 1], kv_offsets=bad.cuda())
+    assert torch.equal(full[others], got[others])
+    bad = torch.tensor([-5, -1, 4, 2, 10 ** 9, 2 ** 31 - 1, -2 ** 31, 0, 3], dtype=torch.int32)
+    assert torch.isfinite(cross_attention(q, packed[:total, 0], packed[:total, 1], kv_offsets=bad.cuda())[[0, 2]]).all()
+    assert _lib.device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("Tq", [2, 130])
+def test_layouts(Tq):
+    """head-major, token-major, broadcast over batch or heads, an output inside a wider buffer"""
+    from nunchaku_b200.ops import cross_attention
+
+    B, H, T, D = 2, 4, 150, 64
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(B, H, Tq, D, generator=g).bfloat16().cuda()
+    k1, v1 = (torch.randn(1, H, T, D, generator=g).bfloat16().cuda() for _ in range(2))
+    keep, s = _keep(B, T), D ** -0.5
+    k, v = k1.expand(B, H, T, D), v1.expand(B, H, T, D)
+    _check(cross_attention(q, k, v), q, k, v, keep, s)
+    k, v = k1[:, :1].expand(B, H, T, D), v1[:, :1].expand(B, H, T, D)
+    ref = cross_attention(q, k, v)
+    _check(ref, q, k, v, keep, s)
+    assert torch.equal(cross_attention(q, k[:, :1], v[:, :1]), ref)          # one stored head for all
+    buf = torch.full((B, Tq + 7, H * D + 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = buf[:, 3:3 + Tq, 32:32 + H * D]
+    assert cross_attention(q, k, v, out=out) is out
+    assert torch.equal(out, ref) and (buf[:, :3] == 7).all() and (buf[:, 3 + Tq:] == 7).all() and (buf[:, :, :32] == 7).all() and (buf[:, :, 32 + H * D:] == 7).all()
+    hm = torch.empty(B, H, Tq, D, dtype=torch.bfloat16, device="cuda")
+    cross_attention(q, k, v, out=hm)
+    assert torch.equal(hm.transpose(1, 2).reshape(B, Tq, H * D), ref)
+
+
+@pytest.mark.parametrize("Tq", [1, 150])
+def test_growing_scores_and_large_scale(Tq):
+    """the maximum rises from block to block by far more than the rescaling step; nearly one-hot weights"""
+    from nunchaku_b200.ops import cross_attention
+
+    B, H, T, D = 2, 2, 900, 128
+    g = torch.Generator().manual_seed(8)
+    q = torch.randn(B, H, Tq, D, generator=g).abs().bfloat16().cuda()
+    k = (torch.randn(B, H, T, D, generator=g).abs() * torch.linspace(0.05, 3, T)[:, None]).bfloat16().cuda()
+    v = torch.randn(B, H, T, D, generator=g).bfloat16().cuda()
+    for s in (D ** -0.5, 0.5):
+        _check(cross_attention(q, k, v, scale=s), q, k, v, _keep(B, T), s)
+    k = k.flip(2)                                    # and falls
+    _check(cross_attention(q, k, v, scale=0.5), q, k, v, _keep(B, T), 0.5)
+
+
+def test_long_state_lists():
+    from nunchaku_b200.ops import cross_attention
+
+    for Tq, T in ((1, 40000), (200, 5000)):
+        q, k, v = _inputs(1, 2, 1, Tq, T, 64, torch.bfloat16, seed=T)
+        _check(cross_attention(q, k, v), q, k, v, _keep(1, T), 0.125)
+
+
+def test_states_beyond_32_bit_offsets():
+    """a batch whose last sample starts more than 2^31 elements into the buffer"""
+    from nunchaku_b200.ops import cross_attention
+
+    T, Hk, D, B = 4096, 8, 128, 2
+    stride = 2 ** 31 + 2 ** 20
+    buf = torch.zeros(stride + T * Hk * D, dtype=torch.bfloat16, device="cuda")
+    k = buf.as_strided((B, Hk, T, D), (stride, D, Hk * D, 1))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k.copy_(torch.randn(B, Hk, T, D, generator=g, device="cuda"))
+    for Tq in (1, 20):
+        q = torch.randn(B, Hk, Tq, D, generator=g, device="cuda").bfloat16()
+        got = cross_attention(q[:, :2], k[:, :2], k[:, :2])
+        _check(got, q[:, :2], k[:, :2].contiguous(), k[:, :2].contiguous(), _keep(B, T), D ** -0.5)
+
+
+@pytest.mark.parametrize("Tq", [1, 200])
+def test_stream_and_graph(Tq):
+    from nunchaku_b200.ops import cross_attention
+
+    q, k, v = _inputs(2, 4, 4, Tq, 300, 112, torch.float16, seed=2)
+    lens = torch.tensor([300, 123], dtype=torch.int32, device="cuda")
+    ref = cross_attention(q, k, v, kv_lens=lens).clone()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = cross_attention(q, k, v, kv_lens=lens)
+    torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(got, ref)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = cross_attention(q, k, v, kv_lens=lens)
+    lens.copy_(torch.tensor([7, 0], dtype=torch.int32))     # read on the device at replay
+    g.replay()
+    assert torch.equal(out, cross_attention(q, k, v, kv_lens=lens)) and (out[1] == 0).all() and not torch.equal(out, ref)
+
+
+def test_python_layer_refuses():
+    from nunchaku_b200.ops import cross_attention
+
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device="cuda")
+    q, k = z(2, 4, 8, 64), z(2, 2, 10, 64)
+    lens, off, mask = z(2, dtype=torch.int32), z(3, dtype=torch.int32), z(2, 10, dtype=torch.bool)
+    assert (cross_attention(q, k, k) == 0).all()
+    for a, kw in [((q.float(), k, k), {}), ((q, k.half(), k), {}), ((q, k, k[:, :, :5]), {}), ((q, z(1, 2, 10, 64), z(1, 2, 10, 64)), {}),
+                  ((q, z(2, 3, 10, 64), z(2, 3, 10, 64)), {}), ((q, z(2, 2, 10, 32), z(2, 2, 10, 32)), {}), ((z(2, 4, 8, 136), z(2, 2, 10, 136), z(2, 2, 10, 136)), {}),
+                  ((z(2, 4, 8, 12), z(2, 2, 10, 12), z(2, 2, 10, 12)), {}), ((q[..., ::2], k[..., ::2], k[..., ::2]), {}), ((q, k[:, :, :0], k[:, :, :0]), {}),
+                  ((q, k, k), dict(scale=0.0)), ((q, k, k), dict(scale=-1.0)), ((q, k, k), dict(kv_lens=lens.long())), ((q, k, k), dict(kv_lens=lens[:1])),
+                  ((q, k, k), dict(kv_lens=lens.cpu())), ((q, k, k), dict(mask=mask[:, :9])), ((q, k, k), dict(mask=mask.int())),
+                  ((q, k, k), dict(mask=mask, kv_lens=lens)), ((q, k, k), dict(kv_offsets=off)), ((q, k[0].transpose(0, 1), k[0].transpose(0, 1)), dict(kv_offsets=off[:2])),
+                  ((q, k, k), dict(out=z(2, 8, 128))), ((q, k, k), dict(out=z(2, 8, 256, dtype=torch.float16))), ((q, k, k), dict(out=z(1, 8, 256).expand(2, 8, 256)))]:
+        with pytest.raises(ValueError):
+            cross_attention(*a, **kw)
+    with pytest.raises(NotImplementedError):
+        cross_attention(q, z(2, 2, 65537, 64), z(2, 2, 65537, 64), mask=z(2, 65537, dtype=torch.bool))
+    assert _lib.device_status() == (0, 0)
