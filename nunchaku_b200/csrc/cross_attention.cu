@@ -53,126 +53,177 @@ __device__ __forceinline__ void cross_range(const CrossStates& s, int b, int& st
 }
 
 // ---------------------------------------------------------------------------------------------------------------- many queries
-constexpr int CT_BM = 128, CT_BN = 128;
-constexpr int CT_HALF_BYTES = 128 * 128;            // 128 rows x 64 channels
-constexpr int CT_TILE_BYTES = 2 * CT_HALF_BYTES;
+constexpr int CT_BM = 128, CT_BN = 64;
+constexpr int CT_Q_HALF = CT_BM * 128;              // 128 rows x 64 channels
+constexpr int CT_KV_HALF = CT_BN * 128;
+constexpr int CT_Q_BYTES = 2 * CT_Q_HALF, CT_KV_BYTES = 2 * CT_KV_HALF;
+constexpr int CT_SLOTS = 2;                         // of K and of V each
 constexpr int CT_THREADS = 256;
 constexpr int CT_PRODUCER_WARP = 4, CT_MMA_WARP = 5, CT_ZERO_WARP = 6;
 // registers move inside the pool the CTA was launched with (256 threads x 128)
-constexpr int CT_REGS_SOFTMAX = 208, CT_REGS_OTHER = 48;
+constexpr int CT_REGS_SOFTMAX = 184, CT_REGS_OTHER = 72;
 static_assert(4 * CT_REGS_SOFTMAX + 4 * CT_REGS_OTHER <= 8 * 128, "register budget");
 constexpr int CT_MASK_STATES = 65536;               // longest state list a mask may cover (its bits are kept in shared memory)
-constexpr int CT_BAR_BYTES = 128;
-constexpr int CT_SMEM = 1024 + 3 * CT_TILE_BYTES + CT_BAR_BYTES;   // 98 KB: two CTAs per SM
-constexpr int CT_TMEM_COLS = 256;
+constexpr int CT_BAR_BYTES = 256;
+constexpr int CT_SMEM = 1024 + CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + CT_BAR_BYTES;   // 97 KB: two CTAs per SM
+constexpr int CT_TABLE_BYTES = 12 * 1024;           // the samples' ranges or mask bits
+constexpr int CT_RANGES = CT_TABLE_BYTES / 8;       // most samples whose ranges are kept there
+constexpr int CT_TMEM_COLS = 256;                   // S: 2 x 64, O: 128
 constexpr long long CT_WAIT_CYCLES = 600000000ll;   // ~0.3 s
 constexpr float CT_RESCALE_STEP = 8.f;
-static_assert(2 * (CT_SMEM + CT_MASK_STATES / 8 + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(2 * (CT_SMEM + CT_TABLE_BYTES + 1024) <= 228 * 1024 && CT_TABLE_BYTES >= CT_MASK_STATES / 8, "two CTAs per SM");
 
 struct CrossTileShared {
-    uint64_t q_full, k_full, k_empty, s_full, p_half[2], pv_done;
+    uint64_t q_full, q_empty, k_full[CT_SLOTS], k_empty[CT_SLOTS], s_full[2], p_full[2], pv_done[2], o_free;
     // A block of V whose rows are all to be seen lands on v_full, which the issuer waits for; one with rows to be zeroed lands on
     // vh_full, which warp 6 waits for, and the issuer waits for v_zeroed: so every barrier has one sequence of phases that
     // its waiter follows without gaps.
-    uint64_t v_full, vh_full, v_zeroed, v_empty;
+    uint64_t v_full[CT_SLOTS], vh_full[CT_SLOTS], v_zeroed[CT_SLOTS], v_empty[CT_SLOTS];
     uint32_t tmem_base;
 };
 static_assert(sizeof(CrossTileShared) <= CT_BAR_BYTES, "barrier block");
 
 struct CrossTileParams {
     CrossStates st;
-    int q_len, dim, group;
+    uint8_t* out;
+    long long os[3];                                      // batch, head, token strides in bytes
+    int q_len, dim, group, heads, q_tiles, items, batch;  // item = (batch * heads + head) * q_tiles + tile
+    int table;                                            // ranges (or mask bits) of all samples are in shared memory
+    int mask_words;                                       // 32-bit words of mask bits per sample
     int q_bmul, q_hmul, k_bmul, k_hmul, v_bmul, v_hmul;   // 0 where that dimension is broadcast (stride 0): its coordinate is then 0
     float scale_log2;
     int* status;
 };
 
-__device__ __forceinline__ void tma_store_4d(const void* tmap, const void* src, int x, int y, int z, int w) {
-    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
-                 ::"l"(tmap), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
-                 : "memory");
-}
+// The blocks of states that a CTA works through, item after item, as each of its roles sees them.
+template <bool MASK>
+struct CrossWalk {
+    const CrossTileParams& p;
+    const int2* ranges;
+    const uint32_t* words;
+    int item, j, valid;      // current block: its leading `valid` states are looked at
+    int start, count, batch;
+    const uint32_t* w;       // MASK: the sample's bits
+
+    __device__ __forceinline__ CrossWalk(const CrossTileParams& p_, const int2* r, const uint32_t* w_)
+        : p(p_), ranges(r), words(w_), item(blockIdx.x), j(-1), valid(0), start(0), count(0), batch(0), w(w_) {
+        if (item < p.items) open();
+    }
+    __device__ __forceinline__ void open() {
+        batch = item / (p.heads * p.q_tiles);
+        if (MASK) {
+            start = 0;
+            count = p.st.kv_len;
+            w = words + (p.table ? batch * p.mask_words : 0);
+        } else if (p.table) {
+            const int2 r = ranges[batch];
+            start = r.x;
+            count = r.y;
+        } else {
+            cross_range(p.st, batch, start, count);
+        }
+        j = -1;
+    }
+    __device__ __forceinline__ int head() const { return item / p.q_tiles % p.heads; }
+    __device__ __forceinline__ int q0() const { return item % p.q_tiles * CT_BM; }
+    __device__ __forceinline__ int look(int i) const {
+        if constexpr (MASK) {
+            const uint32_t a = w[2 * i], b = w[2 * i + 1];
+            return b ? 64 - __clz(b) : a ? 32 - __clz(a) : 0;
+        }
+        return min(count - i * CT_BN, CT_BN);
+    }
+    // next block of this item that has states
+    __device__ __forceinline__ bool next_in_item() {
+        while (++j * CT_BN < count) {
+            valid = look(j);
+            if (valid) return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ bool next_item() {
+        item += gridDim.x;
+        if (item >= p.items) return false;
+        open();
+        return true;
+    }
+    // next block that has states, of this item or a later one
+    __device__ __forceinline__ bool next() {
+        if (item >= p.items) return false;
+        while (!next_in_item())
+            if (!next_item()) return false;
+        return true;
+    }
+    // some of the rows of V that P V reads (valid rounded up to 16) must not be seen and are not zeros already
+    __device__ __forceinline__ bool holes() const {
+        const int up = (valid + 15) & ~15;
+        if constexpr (MASK) {
+            const uint32_t wa = up >= 32 ? 0xffffffffu : (1u << up) - 1u, wb = up >= 64 ? 0xffffffffu : up > 32 ? (1u << (up - 32)) - 1u : 0u;
+            return (w[2 * j] & wa) != wa || (w[2 * j + 1] & wb) != wb;
+        }
+        return up != valid && (p.st.kv_lens || p.st.kv_offsets);   // without them the rows past the end are filled with zeros by the copy
+    }
+};
 
 template <bool F16, bool MASK>
 __global__ void __launch_bounds__(CT_THREADS, 2)
 cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const __grid_constant__ CUtensorMap tm_o, const CrossTileParams p) {
+                  const __grid_constant__ CrossTileParams p) {
     extern __shared__ __align__(1024) uint8_t ct_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ct_smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_s = smem;
-    uint8_t* k_s = q_s + CT_TILE_BYTES;
-    uint8_t* v_s = k_s + CT_TILE_BYTES;
-    CrossTileShared* sh = reinterpret_cast<CrossTileShared*>(v_s + CT_TILE_BYTES);
-    uint32_t* words = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(sh) + CT_BAR_BYTES);   // MASK: one bit per state
+    uint8_t* k_s = q_s + CT_Q_BYTES;
+    uint8_t* v_s = k_s + CT_SLOTS * CT_KV_BYTES;
+    CrossTileShared* sh = reinterpret_cast<CrossTileShared*>(v_s + CT_SLOTS * CT_KV_BYTES);
+    uint8_t* table = reinterpret_cast<uint8_t*>(sh) + CT_BAR_BYTES;
+    int2* ranges = reinterpret_cast<int2*>(table);
+    uint32_t* words = reinterpret_cast<uint32_t*>(table);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int q0 = blockIdx.x * CT_BM, head = blockIdx.y, batch = blockIdx.z;
-    const int kv_head = head / p.group;
-    int kv_start, kv_count;
-    cross_range(p.st, batch, kv_start, kv_count);
-    const int nblocks = (kv_count + CT_BN - 1) / CT_BN;
     const int halves = p.dim > 64 ? 2 : 1;
 
     if (tid == 0) {
         mbar_init(&sh->q_full, 1);
-        mbar_init(&sh->k_full, 1);
-        mbar_init(&sh->k_empty, 1);
-        mbar_init(&sh->v_full, 1);
-        mbar_init(&sh->vh_full, 1);
-        mbar_init(&sh->v_empty, 1);
-        mbar_init(&sh->v_zeroed, 1);
-        mbar_init(&sh->s_full, 1);
-        mbar_init(&sh->p_half[0], 4);
-        mbar_init(&sh->p_half[1], 4);
-        mbar_init(&sh->pv_done, 1);
+        mbar_init(&sh->q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->k_full[i], 1);
+            mbar_init(&sh->k_empty[i], 1);
+            mbar_init(&sh->v_full[i], 1);
+            mbar_init(&sh->vh_full[i], 1);
+            mbar_init(&sh->v_zeroed[i], 1);
+            mbar_init(&sh->v_empty[i], 1);
+            mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->p_full[i], 4);
+            mbar_init(&sh->pv_done[i], 1);
+        }
+        mbar_init(&sh->o_free, 4);
         fence_mbar_init();
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
-        prefetch_tmap(&tm_o);
     }
     if (warp == CT_MMA_WARP) {
         tmem_alloc(&sh->tmem_base, CT_TMEM_COLS);
         tmem_relinquish();
     }
     if constexpr (MASK) {
-        const uint8_t* m = p.st.mask + batch * p.st.mask_stride;
-        for (int w = warp; w < nblocks * 4; w += CT_THREADS / 32) {
-            const int i = w * 32 + lane;
-            const uint32_t bits = __ballot_sync(0xffffffffu, i < kv_count && m[i] != 0);
+        const int first = p.table ? 0 : blockIdx.x / (p.heads * p.q_tiles), count = p.table ? p.batch : 1;
+        for (int w = warp; w < count * p.mask_words; w += CT_THREADS / 32) {
+            const int b = w / p.mask_words, i = (w - b * p.mask_words) * 32 + lane;
+            const uint32_t bits = __ballot_sync(0xffffffffu, i < p.st.kv_len && p.st.mask[(first + b) * p.st.mask_stride + i] != 0);
             if (lane == 0) words[w] = bits;
+        }
+    } else if (p.table) {
+        for (int b = tid; b < p.batch; b += CT_THREADS) {
+            int2 r;
+            cross_range(p.st, b, r.x, r.y);
+            ranges[b] = r;
         }
     }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = sh->tmem_base;
-
-    // States of block j that are looked at: its leading `valid` ones (0: the block is skipped).  `holes`: some of the rows of V
-    // that P V reads (valid rounded up to 16) must not be seen and are not zeros already.
-    auto block_valid = [&](int j) {
-        if constexpr (MASK) {
-#pragma unroll
-            for (int i = 3; i >= 0; --i)
-                if (words[4 * j + i]) return 32 * i + 32 - __clz(words[4 * j + i]);
-            return 0;
-        }
-        return min(kv_count - j * CT_BN, CT_BN);
-    };
-    auto block_holes = [&](int j, int valid) {
-        const int up = (valid + 15) & ~15;
-        if constexpr (MASK) {
-            bool any = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int bits = min(max(up - 32 * i, 0), 32);
-                const uint32_t want = bits == 32 ? 0xffffffffu : (1u << bits) - 1u;
-                any |= (words[4 * j + i] & want) != want;
-            }
-            return any;
-        }
-        return up != valid && (p.st.kv_lens || p.st.kv_offsets);   // without them the rows past the end are filled with zeros by the copy
-    };
     auto timeout = [&](int code) {
         atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
         atomicExch(&p.status[1], code);
@@ -182,42 +233,58 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         reg_dealloc<CT_REGS_OTHER>();
         // ------------------------------------------------------------------ producer
         if (lane == 0) {
-            int n = 0;
+            CrossWalk<MASK> it(p, ranges, words);
+            uint32_t n = 0, q_uses = 0, v_uses[2] = {0, 0};   // v_uses: bit = number of uses of v_full / vh_full of a slot, mod 2, and (bit + 2) whether any
+            int last_item = -1;
             bool ok = true;
-            uint32_t uses[3] = {0, 0, 0};   // of k_full, v_full, vh_full
-            for (int j = 0; j < nblocks && ok; ++j) {
-                const int valid = block_valid(j);
-                if (valid == 0) continue;
-                if (n == 0) {
-                    mbar_arrive_expect_tx(&sh->q_full, halves * CT_HALF_BYTES);
-                    for (int h = 0; h < halves; ++h)
-                        tma_load_4d(q_s + h * CT_HALF_BYTES, &tm_q, &sh->q_full, h * 64, q0, head * p.q_hmul, batch * p.q_bmul);
-                }
-                const int boxes = valid > 64 ? 2 : 1;   // of 64 rows
-                const int row = kv_start + j * CT_BN;
-                for (int kv = 0; kv < 2 && ok; ++kv) {
-                    const int which = kv == 0 ? 0 : block_holes(j, valid) ? 2 : 1;
-                    uint64_t* full = which == 0 ? &sh->k_full : which == 1 ? &sh->v_full : &sh->vh_full;
-                    if (!mbar_wait(kv ? &sh->v_empty : &sh->k_empty, (n & 1) ^ 1, CT_WAIT_CYCLES)) {
-                        timeout(900 + kv);
-                        ok = false;
+            while (ok && it.next()) {
+                const int head = it.head(), kv_head = head / p.group, slot = n & 1;
+                if (it.item != last_item) {
+                    last_item = it.item;
+                    ok = mbar_wait(&sh->q_empty, (q_uses & 1) ^ 1, CT_WAIT_CYCLES);
+                    if (!ok) {
+                        timeout(900);
                         break;
                     }
-                    mbar_arrive_expect_tx(full, halves * boxes * (CT_HALF_BYTES / 2));
-                    ++uses[which];
-                    const int z = kv_head * (kv ? p.v_hmul : p.k_hmul), w = p.st.kv_offsets ? 0 : batch * (kv ? p.v_bmul : p.k_bmul);
+                    ++q_uses;
+                    mbar_arrive_expect_tx(&sh->q_full, halves * CT_Q_HALF);
                     for (int h = 0; h < halves; ++h)
-                        for (int b = 0; b < boxes; ++b)
-                            tma_load_4d((kv ? v_s : k_s) + h * CT_HALF_BYTES + b * (CT_HALF_BYTES / 2), kv ? &tm_v : &tm_k, full, h * 64,
-                                        row + b * 64, z, w);
+                        tma_load_4d(q_s + h * CT_Q_HALF, &tm_q, &sh->q_full, h * 64, it.q0(), head * p.q_hmul, it.batch * p.q_bmul);
                 }
+                const int row = it.start + it.j * CT_BN;
+                const uint32_t empty_parity = ((n >> 1) & 1) ^ 1;
+                if (!mbar_wait(&sh->k_empty[slot], empty_parity, CT_WAIT_CYCLES)) {
+                    timeout(901);
+                    ok = false;
+                    break;
+                }
+                mbar_arrive_expect_tx(&sh->k_full[slot], halves * CT_KV_HALF);
+                for (int h = 0; h < halves; ++h)
+                    tma_load_4d(k_s + slot * CT_KV_BYTES + h * CT_KV_HALF, &tm_k, &sh->k_full[slot], h * 64, row, kv_head * p.k_hmul,
+                                p.st.kv_offsets ? 0 : it.batch * p.k_bmul);
+                if (!mbar_wait(&sh->v_empty[slot], empty_parity, CT_WAIT_CYCLES)) {
+                    timeout(902);
+                    ++n;
+                    ok = false;
+                    break;
+                }
+                const bool holes = it.holes();
+                uint64_t* full = holes ? &sh->vh_full[slot] : &sh->v_full[slot];
+                v_uses[holes] = (v_uses[holes] ^ (1u << slot)) | (4u << slot);
+                mbar_arrive_expect_tx(full, halves * CT_KV_HALF);
+                for (int h = 0; h < halves; ++h)
+                    tma_load_4d(v_s + slot * CT_KV_BYTES + h * CT_KV_HALF, &tm_v, full, h * 64, row, kv_head * p.v_hmul,
+                                p.st.kv_offsets ? 0 : it.batch * p.v_bmul);
                 ++n;
             }
             if (!ok) {   // leave with no copy of this CTA in flight
-                mbar_wait(&sh->q_full, 0, CT_WAIT_CYCLES);
-                if (uses[0]) mbar_wait(&sh->k_full, (uses[0] - 1) & 1, CT_WAIT_CYCLES);
-                if (uses[1]) mbar_wait(&sh->v_full, (uses[1] - 1) & 1, CT_WAIT_CYCLES);
-                if (uses[2]) mbar_wait(&sh->vh_full, (uses[2] - 1) & 1, CT_WAIT_CYCLES);
+                if (q_uses) mbar_wait(&sh->q_full, (q_uses - 1) & 1, CT_WAIT_CYCLES);
+                for (int s = 0; s < 2; ++s) {
+                    const uint32_t uses = (n + 1 - s) >> 1;   // of K slot s
+                    if (uses) mbar_wait(&sh->k_full[s], (uses - 1) & 1, CT_WAIT_CYCLES);
+                    if (v_uses[0] & (4u << s)) mbar_wait(&sh->v_full[s], ((v_uses[0] >> s) & 1) ^ 1, CT_WAIT_CYCLES);
+                    if (v_uses[1] & (4u << s)) mbar_wait(&sh->vh_full[s], ((v_uses[1] >> s) & 1) ^ 1, CT_WAIT_CYCLES);
+                }
             }
         }
     } else if (warp == CT_MMA_WARP) {
@@ -226,7 +293,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int ksteps = (p.dim + 15) >> 4;                    // of 16 channels; channels past the head read as zeros
         const uint32_t idesc_pv = idesc_h16(CT_BM, 0, F16, true) | (static_cast<uint32_t>(ksteps * 2) << 17);
         const uint64_t qd = smem_desc_sw128(smem_u32(q_s)), kd = smem_desc_sw128(smem_u32(k_s));
-        const uint64_t vd = smem_desc_sw128_mn(smem_u32(v_s), CT_HALF_BYTES, 1024);
+        const uint64_t vd = smem_desc_sw128_mn(smem_u32(v_s), CT_KV_HALF, 1024);
         const uint32_t hi_k = static_cast<uint32_t>(qd >> 32), hi_v = static_cast<uint32_t>(vd >> 32);
         const uint32_t q_lo = static_cast<uint32_t>(qd), k_lo = static_cast<uint32_t>(kd), v_lo = static_cast<uint32_t>(vd);
         bool ok = true;
@@ -237,110 +304,121 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             return ok;
         };
-        auto next_block = [&](int j) {
-            while (j < nblocks && block_valid(j) == 0) ++j;
-            return j;
-        };
-        // S = Q K_j^T over the block's states, rounded up to 16
-        auto issue_qk = [&](int valid) {
-            const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((valid + 15) >> 4) << 18);
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-                if (kk < ksteps) {
-                    const uint32_t off = (kk >> 2) * (CT_HALF_BYTES >> 4) + (kk & 3) * 2;
-                    tc_mma_f16_lo(tmem, q_lo + off, k_lo + off, hi_k, idesc, kk > 0);
-                }
-            tc_commit(&sh->s_full);
-            tc_commit(&sh->k_empty);
-        };
-        int j = next_block(0), n = 0, plain = 0, zeroed = 0, second = 0;   // blocks; of those: V as it lies, V with zeroed rows, more than 64 states
-        if (j < nblocks && wait(&sh->q_full, 0, 910) && wait(&sh->k_full, 0, 911)) {
+        CrossWalk<MASK> cur(p, ranges, words);
+        uint32_t n = 0, opened = 0, plain = 0, zeroed = 0;   // n: block of `cur`; opened: items whose Q was waited for; plain / zeroed: phase bit per V slot
+        // S = Q K_j^T of block `w` (number m) over its states, rounded up to 16; `last`: of its item
+        auto issue_qk = [&](int valid, uint32_t m, bool first, bool last) {
+            if (first && !wait(&sh->q_full, opened++ & 1, 910)) return;
+            if (!wait(&sh->k_full[m & 1], (m >> 1) & 1, 911)) return;
             tc_fence_after_sync();
-            if (elect_one()) issue_qk(block_valid(j));
-            __syncwarp();
-        }
-        while (ok && j < nblocks) {
-            const int valid = block_valid(j), steps = (valid + 15) >> 4;
-            const int jn = next_block(j + 1);
-            if (block_holes(j, valid)) {
-                if (!wait(&sh->v_zeroed, zeroed++ & 1, 921)) break;
-            } else {
-                if (!wait(&sh->v_full, plain++ & 1, 920)) break;
-            }
-            for (int hf = 0; hf < (valid > 64 ? 2 : 1); ++hf) {
-                if (!wait(&sh->p_half[hf], hf ? second++ & 1 : n & 1, 930 + hf)) break;
-                tc_fence_after_sync();
-                if (elect_one()) {
-#pragma unroll
-                    for (int k4 = 0; k4 < 4; ++k4)
-                        if (hf * 4 + k4 < steps)
-                            tc_mma_f16_ts_lo(tmem + CT_BN, tmem + hf * 64 + k4 * 8, v_lo + (hf * 4 + k4) * 128, hi_v, idesc_pv, (n | hf | k4) ? 1u : 0u);
-                }
-                __syncwarp();
-            }
-            if (!ok) break;
+            const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((valid + 15) >> 4) << 18);
             if (elect_one()) {
-                tc_commit(&sh->pv_done);
-                tc_commit(&sh->v_empty);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    if (kk < ksteps)
+                        tc_mma_f16_lo(tmem + (m & 1) * CT_BN, q_lo + (kk >> 2) * (CT_Q_HALF >> 4) + (kk & 3) * 2,
+                                      k_lo + (m & 1) * (CT_KV_BYTES >> 4) + (kk >> 2) * (CT_KV_HALF >> 4) + (kk & 3) * 2, hi_k, idesc, kk > 0);
+                tc_commit(&sh->s_full[m & 1]);
+                tc_commit(&sh->k_empty[m & 1]);
+                if (last) tc_commit(&sh->q_empty);
             }
             __syncwarp();
-            ++n;
-            j = jn;
-            if (j < nblocks) {
-                if (!wait(&sh->k_full, n & 1, 940)) break;
-                tc_fence_after_sync();
-                if (elect_one()) issue_qk(block_valid(j));   // overwrites P: behind P V in the tensor pipe's order
-                __syncwarp();
+        };
+        bool more = cur.next(), first = true;
+        uint32_t items_done = 0;
+        bool started = false;
+        while (more && ok) {
+            CrossWalk<MASK> nxt = cur;
+            const bool next_there = nxt.next();
+            const bool same = next_there && nxt.item == cur.item;
+            if (!started) {
+                started = true;
+                issue_qk(cur.valid, n, true, !same);
+                if (!ok) break;
             }
+            if (same) {   // the scores of the item's next block while this one's exponentials run
+                CrossWalk<MASK> after = nxt;
+                const bool nlast = !after.next_in_item();
+                issue_qk(nxt.valid, n + 1, false, nlast);
+                if (!ok) break;
+            }
+            const uint32_t slot = n & 1;
+            if (first && items_done > 0 && !wait(&sh->o_free, (items_done - 1) & 1, 915)) break;   // the previous item's O has been read
+            if (cur.holes()) {
+                if (!wait(&sh->v_zeroed[slot], (zeroed >> slot) & 1, 921)) break;
+                zeroed ^= 1u << slot;
+            } else {
+                if (!wait(&sh->v_full[slot], (plain >> slot) & 1, 920)) break;
+                plain ^= 1u << slot;
+            }
+            if (!wait(&sh->p_full[slot], (n >> 1) & 1, 930)) break;
+            tc_fence_after_sync();
+            if (elect_one()) {
+                const int steps = (cur.valid + 15) >> 4;
+#pragma unroll
+                for (int k4 = 0; k4 < 4; ++k4)
+                    if (k4 < steps)
+                        tc_mma_f16_ts_lo(tmem + 2 * CT_BN, tmem + slot * CT_BN + k4 * 8, v_lo + slot * (CT_KV_BYTES >> 4) + k4 * 128, hi_v, idesc_pv,
+                                         (!first || k4 > 0) ? 1u : 0u);
+                tc_commit(&sh->pv_done[slot]);
+                tc_commit(&sh->v_empty[slot]);
+            }
+            __syncwarp();
+            first = !same;
+            if (!same) {
+                ++items_done;
+                if (next_there) {
+                    CrossWalk<MASK> after = nxt;
+                    const bool nlast = !after.next_in_item();
+                    issue_qk(nxt.valid, n + 1, true, nlast);
+                }
+            }
+            ++n;
+            more = next_there;
+            cur.item = nxt.item; cur.j = nxt.j; cur.valid = nxt.valid; cur.start = nxt.start; cur.count = nxt.count; cur.batch = nxt.batch; cur.w = nxt.w;
         }
     } else if (warp >= CT_ZERO_WARP) {
         reg_dealloc<CT_REGS_OTHER>();
         // ------------------------------------------------------------------ rows of V that must not be seen -> zeros
         if (warp == CT_ZERO_WARP) {
-            int n = 0;   // blocks with such rows
-            for (int j = 0; j < nblocks; ++j) {
-                const int valid = block_valid(j);
-                if (valid == 0) continue;
-                if (block_holes(j, valid)) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(&sh->vh_full, n & 1, CT_WAIT_CYCLES))) {
-                        if (lane == 0) timeout(950);
-                        break;
-                    }
-                    const int up = (valid + 15) & ~15;
-                    // four rows a turn, eight lanes per row (and half)
-                    for (int r0 = MASK ? 0 : valid & ~3; r0 < up; r0 += 4) {
-                        const int r = r0 + (lane >> 3);
-                        bool zero = r >= valid;
-                        if constexpr (MASK) zero = !((words[4 * j + (r >> 5)] >> (r & 31)) & 1u);
-                        if (zero && r < up)
-                            for (int h = 0; h < halves; ++h)
-                                *reinterpret_cast<uint4*>(v_s + h * CT_HALF_BYTES + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh->v_zeroed);
-                    ++n;
+            CrossWalk<MASK> it(p, ranges, words);
+            uint32_t n = 0, phase = 0;
+            while (it.next()) {
+                const uint32_t slot = n++ & 1;
+                if (!it.holes()) continue;
+                if (!__all_sync(0xffffffffu, mbar_wait(&sh->vh_full[slot], (phase >> slot) & 1, CT_WAIT_CYCLES))) {
+                    if (lane == 0) timeout(950);
+                    break;
                 }
+                phase ^= 1u << slot;
+                const int up = (it.valid + 15) & ~15;
+                // four rows a turn, eight lanes per row (and half)
+                for (int r0 = MASK ? 0 : it.valid & ~3; r0 < up; r0 += 4) {
+                    const int r = r0 + (lane >> 3);
+                    bool zero = r >= it.valid;
+                    if constexpr (MASK) zero = !((it.w[2 * it.j + (r >> 5)] >> (r & 31)) & 1u);
+                    if (zero && r < up)
+                        for (int h = 0; h < halves; ++h)
+                            *reinterpret_cast<uint4*>(v_s + slot * CT_KV_BYTES + h * CT_KV_HALF + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->v_zeroed[slot]);
             }
         }
     } else {
         reg_alloc<CT_REGS_SOFTMAX>();
         // ------------------------------------------------------------------ softmax: thread = one query row
         const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
-        const uint32_t s_tmem = tmem + lane_addr, o_tmem = s_tmem + CT_BN;
-        float m_used = 0.f, l = 0.f;
-        bool ok = true;
+        const uint32_t s_tmem = tmem + lane_addr, o_tmem = s_tmem + 2 * CT_BN;
         const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-        // 64 states (two 32-column chunks of S) -> 32 columns of packed 16-bit pairs, and their sum
-        auto exp_half = [&](const uint32_t (&a)[32], const uint32_t (&b)[32], float m, uint32_t (&w)[32]) {
+        // 32 states -> 16 columns of packed 16-bit pairs, and their sum
+        auto exp32 = [&](const uint32_t (&a)[32], float m, uint32_t (&w)[16]) {
             const float2 nm2 = make_float2(-m, -m);
             float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int e = (i & 15) * 2;
-                const float2 v = i < 16 ? make_float2(__uint_as_float(a[e]), __uint_as_float(a[e + 1]))
-                                        : make_float2(__uint_as_float(b[e]), __uint_as_float(b[e + 1]));
-                const float2 x = __ffma2_rn(v, sc2, nm2);
+            for (int i = 0; i < 16; ++i) {
+                const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), sc2, nm2);
                 float2 r;
                 if ((i & 3) == 3) {   // a quarter on the FMA pipe, as in attention.cu
                     r = exp2_fma2(x);
@@ -353,73 +431,61 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             return (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
         };
-        auto max_half = [&](const uint32_t (&a)[32], const uint32_t (&b)[32]) {
-            float m0 = __uint_as_float(a[0]), m1 = __uint_as_float(b[0]);
+        auto max32 = [&](const uint32_t (&a)[32]) {
+            float m0 = __uint_as_float(a[0]), m1 = __uint_as_float(a[1]);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
+            for (int i = 2; i < 32; i += 4) {
                 m0 = max3(m0, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
-                m1 = max3(m1, __uint_as_float(b[i]), __uint_as_float(b[i + 1]));
+                if (i + 2 < 32) m1 = max3(m1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
             }
             return fmaxf(m0, m1);
         };
+        CrossWalk<MASK> it(p, ranges, words);
         // scores that do not count -> -inf (selected, not added: they may be anything)
-        auto hide = [&](uint32_t (&a)[32], int j, int chunk, int valid) {
+        auto hide = [&](uint32_t (&a)[32], int chunk) {
             if constexpr (MASK) {
-                const uint32_t bits = words[4 * j + chunk];
+                const uint32_t bits = it.w[2 * it.j + chunk];
                 if (bits != 0xffffffffu) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (!((bits >> i) & 1u)) a[i] = 0xff800000u;
                 }
-            } else if (valid < (chunk + 1) * 32) {
+            } else if (it.valid < (chunk + 1) * 32) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    if (chunk * 32 + i >= valid) a[i] = 0xff800000u;
+                    if (chunk * 32 + i >= it.valid) a[i] = 0xff800000u;
             }
         };
-        auto publish = [&](int hf, const uint32_t (&w)[32]) {
-            tc_st_32x32b_x32(s_tmem + hf * 64, w);   // over this thread's own S values, which are all in registers by now
-            tc_wait_st();
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->p_half[hf]);
-        };
-        int n = 0;
-        for (int j = 0; j < nblocks; ++j) {
-            const int valid = block_valid(j);
-            if (valid == 0) continue;
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh->s_full, n & 1, CT_WAIT_CYCLES))) {
-                if (lane == 0) timeout(960);
-                ok = false;
-                break;
-            }
-            tc_fence_after_sync();
-            const bool two = valid > 64;
-            uint32_t s0[32], s1[32], s2[32], s3[32], w[32];
-            tc_ld_32x32b_x32(s_tmem, s0);
-            tc_ld_32x32b_x32(s_tmem + 32, s1);
-            tc_wait_ld();
-            if (two) {
-                tc_ld_32x32b_x32(s_tmem + 64, s2);
-                tc_ld_32x32b_x32(s_tmem + 96, s3);
-            }
-            hide(s0, j, 0, valid);
-            hide(s1, j, 1, valid);
-            float mx = max_half(s0, s1);
-            float sum_a = 0.f;
-            if (n > 0) sum_a = exp_half(s0, s1, m_used, w);   // with the maximum in use while the second half is on its way
-            if (two) {
+        uint32_t n = 0;
+        bool ok = true;
+        if (it.item < p.items) do {
+            float m_used = 0.f, l = 0.f;
+            bool first = true;
+            while (it.next_in_item()) {
+                const uint32_t slot = n & 1;
+                if (!__all_sync(0xffffffffu, mbar_wait(&sh->s_full[slot], (n >> 1) & 1, CT_WAIT_CYCLES))) {
+                    if (lane == 0) timeout(960);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+                const bool two = it.valid > 32;
+                const uint32_t st = s_tmem + slot * CT_BN;
+                uint32_t s0[32], s1[32], w[16];
+                tc_ld_32x32b_x32(st, s0);
+                if (two) tc_ld_32x32b_x32(st + 32, s1);
                 tc_wait_ld();
-                hide(s2, j, 2, valid);
-                hide(s3, j, 3, valid);
-                mx = fmaxf(mx, max_half(s2, s3));
-            }
-            const float ms = mx * p.scale_log2;
-            const bool grow = n == 0 || ms > m_used + CT_RESCALE_STEP;
-            if (__any_sync(0xffffffffu, grow)) {
-                if (n > 0) {
+                hide(s0, 0);
+                float mx = max32(s0);
+                if (two) {
+                    hide(s1, 1);
+                    mx = fmaxf(mx, max32(s1));
+                }
+                const float ms = mx * p.scale_log2;
+                const bool grow = first || ms > m_used + CT_RESCALE_STEP;
+                if (!first && __any_sync(0xffffffffu, grow)) {
                     // O is written by the previous P V product until it has completed
-                    if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done, (n - 1) & 1, CT_WAIT_CYCLES))) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, CT_WAIT_CYCLES))) {
                         if (lane == 0) timeout(970);
                         ok = false;
                         break;
@@ -427,73 +493,74 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     tc_fence_after_sync();
                     const float alpha = grow ? ex2(m_used - ms) : 1.f;
                     l *= alpha;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c * 32 >= p.dim) break;
-                        uint32_t o[32];
-                        tc_ld_32x32b_x32(o_tmem + c * 32, o);
+#pragma unroll 1
+                    for (int c = 0; c < p.dim; c += 16) {
+                        uint32_t o[16];
+                        tc_ld_32x32b_x16(o_tmem + c, o);
                         tc_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tc_st_32x32b_x32(o_tmem + c * 32, o);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tc_st_32x32b_x16(o_tmem + c, o);
                     }
                     tc_wait_st();
                 }
-                if (grow) {
-                    m_used = ms;
-                    sum_a = exp_half(s0, s1, m_used, w);
+                if (grow) m_used = ms;
+                // P over this thread's own S values, which are all in registers by now
+                l += exp32(s0, m_used, w);
+                tc_st_32x32b_x16(st, w);
+                if (two) {
+                    l += exp32(s1, m_used, w);
+                    tc_st_32x32b_x16(st + 16, w);
                 }
+                tc_wait_st();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->p_full[slot]);
+                first = false;
+                ++n;
             }
-            publish(0, w);
-            if (two) {
-                sum_a += exp_half(s2, s3, m_used, w);
-                publish(1, w);
+            if (!ok) break;
+            // ---- O / l -> global
+            const int qrow = it.q0() + warp * 32 + lane;
+            uint8_t* dst = p.out + it.batch * p.os[0] + it.head() * p.os[1] + qrow * p.os[2];
+            if (first) {   // no states: zeros
+                if (qrow < p.q_len)
+                    for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(dst + 2 * c) = make_uint4(0, 0, 0, 0);
+                continue;
             }
-            l += sum_a;
-            ++n;
-        }
-        // ---- O / l through shared memory (over Q, which every product has read) to global memory
-        if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh->pv_done, (n - 1) & 1, CT_WAIT_CYCLES))) {
-            if (lane == 0) timeout(980);
-            ok = false;
-        }
-        if (ok) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, CT_WAIT_CYCLES))) {
+                if (lane == 0) timeout(980);
+                ok = false;
+                break;
+            }
             tc_fence_after_sync();
-            const float inv = n > 0 ? 1.f / l : 0.f;
-            const int row = warp * 32 + lane;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (c * 32 >= p.dim) break;
-                uint32_t o[32];
-                if (n > 0) {
-                    tc_ld_32x32b_x32(o_tmem + c * 32, o);
-                    tc_wait_ld();
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0u;   // no states: zeros
+            const float inv = 1.f / l;
+#pragma unroll 1
+            for (int c = 0; c < p.dim; c += 64) {
+                uint32_t a[32], b[32];
+                tc_ld_32x32b_x32(o_tmem + c, a);
+                if (c + 32 < p.dim) tc_ld_32x32b_x32(o_tmem + c + 32, b);
+                tc_wait_ld();
+                if (c + 64 >= p.dim) {   // all of O is in registers: the next item's P V may overwrite it
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->o_free);
                 }
+                if (qrow < p.q_len) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    uint32_t w4[4];
+                    for (int u = 0; u < 8; ++u) {
+                        if (c + u * 8 < p.dim) {
+                            const uint32_t(&o)[32] = u < 4 ? a : b;
+                            uint32_t w4[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w4[e] = pack_h16<F16>(__uint_as_float(o[u * 8 + 2 * e]) * inv, __uint_as_float(o[u * 8 + 2 * e + 1]) * inv);
-                    // 16-byte piece (c & 1) * 4 + u of the row's 128 bytes, where the 128-byte swizzle puts it
-                    *reinterpret_cast<uint4*>(q_s + (c >> 1) * CT_HALF_BYTES + row * 128 + ((((c & 1) * 4 + u) ^ (row & 7)) << 4)) =
-                        make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                            for (int e = 0; e < 4; ++e)
+                                w4[e] = pack_h16<F16>(__uint_as_float(o[(u & 3) * 8 + 2 * e]) * inv, __uint_as_float(o[(u & 3) * 8 + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4*>(dst + 2 * (c + u * 8)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                        }
+                    }
                 }
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                if (q0 + warp * 32 < p.q_len)
-                    for (int h = 0; h < halves; ++h)
-                        tma_store_4d(&tm_o, q_s + h * CT_HALF_BYTES + warp * 32 * 128, h * 64, q0 + warp * 32, head, batch);
-                bulk_commit_group();
-                bulk_wait_group_read<0>();
-            }
-            __syncwarp();
-        }
+        } while (it.next_item());
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -504,7 +571,8 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 }
 
 // ---------------------------------------------------------------------------------------------------------------- few query rows
-constexpr int CR_THREADS = 128, CR_KEYS = 64, CR_STAGES = 3, CR_ROWS = 16, CR_MAX_SPLIT = 8;
+constexpr int CR_WARPS = 4, CR_THREADS = 32 * CR_WARPS, CR_KEYS = 16, CR_STAGES = 2, CR_ROWS = 16, CR_MAX_SPLIT = 8;
+constexpr int CR_TILE = CR_WARPS * CR_KEYS;          // states that the CTA's warps take in one turn
 
 struct CrossRowsParams {
     CrossStates st;
@@ -520,10 +588,13 @@ struct CrossRowsSizes {
     static constexpr int ROW = (2 * NK + 1) * 16;           // bytes of a state's row: an odd number of 16-byte pieces, so that ldmatrix has no conflicts
     static constexpr int TILE = CR_KEYS * ROW;
     static constexpr int STAGE = 2 * TILE;
-    static constexpr int SMEM = CR_STAGES * STAGE;
+    static constexpr int RING = CR_WARPS * CR_STAGES * STAGE;   // each warp has a ring of its own
     static constexpr int COLS = NK * 16;
-    // afterwards: four warps' partial sums [4][16][COLS], the CTA's [16][COLS], maxima and sums [5][16] each
-    static_assert(SMEM >= 5 * CR_ROWS * COLS * 4 + 2 * 5 * CR_ROWS * 4, "the partial sums lie over the ring");
+    // afterwards over the ring: the warps' partial sums [4][16][COLS], maxima and sums [4][16] each
+    static_assert(RING >= CR_WARPS * CR_ROWS * (COLS + 2) * 4, "the partial sums lie over the ring");
+    // behind the ring, written by the CTAs of the cluster: each one's sums of the elements that this CTA finishes, and their maxima and sums
+    static constexpr int mail_floats(int rows, int split) { return split * ((rows * COLS / 2 + split - 1) / split) * 2; }
+    static constexpr int smem(int rows, int split) { return RING + (mail_floats(rows, split) + 2 * split * rows) * 4; }
 };
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {   // writes zeros where not valid (src is not read)
@@ -544,7 +615,9 @@ __device__ __forceinline__ void mma_16816_t(float (&c)[4], const uint32_t (&a)[4
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t addr) { return __int_as_float(ld_shared_cluster_s32(addr)); }
+__device__ __forceinline__ void st_shared_cluster_f32x2(uint32_t cluster_addr, float2 v) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y) : "memory");
+}
 
 // grid (batch * kv_heads * split, row tiles), cluster (split, 1, 1)
 template <bool F16, int NK>
@@ -555,21 +628,24 @@ cross_rows_kernel(const CrossRowsParams p, const int split) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
     const int pairix = blockIdx.x / split, batch = pairix / p.kv_heads, kv_head = pairix % p.kv_heads;
-    const int r0 = blockIdx.y * CR_ROWS;
+    const int r0 = blockIdx.y * CR_ROWS, rows = min(CR_ROWS, p.q_rows - r0);
     int start, count;
     cross_range(p.st, batch, start, count);
-    const int tiles = (count + CR_KEYS - 1) / CR_KEYS;
+    const int tiles = (count + CR_TILE - 1) / CR_TILE;
     const int t0 = static_cast<int>(static_cast<long long>(tiles) * rank / split), t1 = static_cast<int>(static_cast<long long>(tiles) * (rank + 1) / split);
     const uint8_t* kbase = p.k + kv_head * p.ks[1] + (p.st.kv_offsets ? start * p.ks[2] : batch * p.ks[0]);
     const uint8_t* vbase = p.v + kv_head * p.vs[1] + (p.st.kv_offsets ? start * p.vs[2] : batch * p.vs[0]);
     const uint8_t* mask = p.st.mask ? p.st.mask + batch * p.st.mask_stride : nullptr;
+    uint8_t* ring = cr_smem + warp * CR_STAGES * S::STAGE;
 
-    auto load_tile = [&](int tile, int slot) {
-        uint8_t* ks = cr_smem + slot * S::STAGE;
+    // this warp's 16 states of a turn; rows of states that are not to be seen, and channels past the head, become zeros
+    auto load = [&](int tile, int slot) {
+        uint8_t* ks = ring + slot * S::STAGE;
+        const int key0 = tile * CR_TILE + warp * CR_KEYS;
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-            const int idx = tid + i * CR_THREADS, r = idx / (2 * NK), c = idx % (2 * NK);
-            const int key = tile * CR_KEYS + r;
+            const int idx = lane + i * 32, r = idx / (2 * NK), c = idx % (2 * NK);
+            const int key = key0 + r;
             bool valid = key < count && c * 8 < p.dim;
             if (mask && valid) valid = mask[key] != 0;
             const uint8_t* ksrc = valid ? kbase + key * p.ks[2] + c * 16 : p.k;
@@ -580,7 +656,7 @@ cross_rows_kernel(const CrossRowsParams p, const int split) {
     };
 #pragma unroll
     for (int s = 0; s < CR_STAGES - 1; ++s) {
-        if (t0 + s < t1) load_tile(t0 + s, s);
+        if (t0 + s < t1) load(t0 + s, s);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
     // query fragments: rows g and g + 8
@@ -608,14 +684,17 @@ cross_rows_kernel(const CrossRowsParams p, const int split) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int slot = 0;
     for (int tile = t0; tile < t1; ++tile) {
+        // the copies of this turn have landed for every lane, and every lane has left the slot that is filled next
         asm volatile("cp.async.wait_group %0;" ::"n"(CR_STAGES - 2) : "memory");
-        __syncthreads();   // the tile has landed for every thread, and every warp has left the slot that is filled next
-        if (tile + CR_STAGES - 1 < t1) load_tile(tile + CR_STAGES - 1, (tile - t0 + CR_STAGES - 1) % CR_STAGES);
+        __syncwarp();
+        if (tile + CR_STAGES - 1 < t1) load(tile + CR_STAGES - 1, (slot + CR_STAGES - 1) % CR_STAGES);
         asm volatile("cp.async.commit_group;" ::: "memory");
-        const uint8_t* ks = cr_smem + ((tile - t0) % CR_STAGES) * S::STAGE + warp * 16 * S::ROW;
+        const uint8_t* ks = ring + slot * S::STAGE;
         const uint8_t* vs = ks + S::TILE;
-        const int key0 = tile * CR_KEYS + warp * 16;
+        slot = (slot + 1) % CR_STAGES;
+        const int key0 = tile * CR_TILE + warp * CR_KEYS;
         if (key0 >= count) continue;
         float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -674,79 +753,86 @@ cross_rows_kernel(const CrossRowsParams p, const int split) {
             mma_16816_t<F16>(o[2 * kk + 1], pf, b[2], b[3]);
         }
     }
+    // Every CTA of the cluster has started (its shared memory may be written from here on); the wait is at the joining below.
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    // ---- join the four warps, then the CTAs of the cluster
-    const int rows = min(CR_ROWS, p.q_rows - r0);
+    // ---- the warps' sums into shared memory (over the ring), rows that exist only
     float* part = reinterpret_cast<float*>(cr_smem);               // [4][16][COLS]
-    float* mine = part + 4 * CR_ROWS * S::COLS;                    // [16][COLS]
-    float* pm = mine + CR_ROWS * S::COLS;                          // [5][16]: the warps' maxima, then the CTA's
-    float* pl = pm + 5 * CR_ROWS;
+    float* pm = part + CR_WARPS * CR_ROWS * S::COLS;               // [4][16]
+    float* pl = pm + CR_WARPS * CR_ROWS;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+        const int r = g + 8 * i;
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (t == 0) {
-            pm[warp * CR_ROWS + g + 8 * i] = m[i];
-            pl[warp * CR_ROWS + g + 8 * i] = l[i];
-        }
-    }
+        if (r < rows) {
+            if (t == 0) {
+                pm[warp * CR_ROWS + r] = m[i];
+                pl[warp * CR_ROWS + r] = l[i];
+            }
 #pragma unroll
-    for (int i = 0; i < 2 * NK; ++i) {
-        *reinterpret_cast<float2*>(part + (warp * CR_ROWS + g) * S::COLS + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
-        *reinterpret_cast<float2*>(part + (warp * CR_ROWS + g + 8) * S::COLS + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
+            for (int c = 0; c < 2 * NK; ++c)
+                *reinterpret_cast<float2*>(part + (warp * CR_ROWS + r) * S::COLS + c * 8 + 2 * t) = make_float2(o[c][2 * i], o[c][2 * i + 1]);
+        }
     }
     __syncthreads();
-    for (int idx = tid; idx < rows * S::COLS; idx += CR_THREADS) {
-        const int r = idx / S::COLS, c = idx % S::COLS;
-        float mm = -INFINITY;
+    // ---- joined over the warps and sent to the CTA of the cluster that finishes the element: element e (a pair of channels) belongs
+    // to CTA e % split, which keeps [source CTA][e / split] pairs and every source's maximum and sum per row
+    const int half = p.dim >> 1, elems = rows * half, per = (rows * S::COLS / 2 + split - 1) / split;
+    float2* mail = reinterpret_cast<float2*>(cr_smem + S::RING);   // [split][per]
+    float2* stat = mail + split * per;                             // [split][rows]: maximum, sum
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int e = tid; e < elems; e += CR_THREADS) {
+        const int r = e / half, c = (e - r * half) * 2;
+        float mm = pm[r];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, pm[w * CR_ROWS + r]);
+        for (int w = 1; w < CR_WARPS; ++w) mm = fmaxf(mm, pm[w * CR_ROWS + r]);
         const float b = mm == -INFINITY ? 0.f : mm;
-        float sum = 0.f, ls = 0.f;
+        float2 sum = make_float2(0.f, 0.f);
+        float ls = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < CR_WARPS; ++w) {
             const float f = ex2(pm[w * CR_ROWS + r] - b);
-            sum = fmaf(f, part[(w * CR_ROWS + r) * S::COLS + c], sum);
+            const float2 v = *reinterpret_cast<const float2*>(part + (w * CR_ROWS + r) * S::COLS + c);
+            sum.x = fmaf(f, v.x, sum.x);
+            sum.y = fmaf(f, v.y, sum.y);
             ls = fmaf(f, pl[w * CR_ROWS + r], ls);
         }
-        mine[idx] = sum;
-        if (c == 0) {
-            pm[4 * CR_ROWS + r] = mm;
-            pl[4 * CR_ROWS + r] = ls;
+        if (split == 1) {
+            mail[e] = sum;
+            if (c == 0) stat[r] = make_float2(mm, ls);
+        } else {
+            st_shared_cluster_f32x2(mapa_shared(smem_u32(mail + rank * per + e / split), e % split), sum);
+            if (c == 0)
+                for (int q = 0; q < split; ++q) st_shared_cluster_f32x2(mapa_shared(smem_u32(stat + rank * rows + r), q), make_float2(mm, ls));
         }
     }
-    if (split > 1) cluster_sync_all();
+    if (split > 1) cluster_sync_all();   // nothing is read from or written to another CTA behind this
     else __syncthreads();
-    const int half = p.dim >> 1;
-    for (int idx = rank * CR_THREADS + tid; idx < rows * half; idx += split * CR_THREADS) {
-        const int r = idx / half, c = (idx % half) * 2;
+    for (int e = rank + split * tid; e < elems; e += split * CR_THREADS) {
+        const int r = e / half, c = (e - r * half) * 2;
         float mm = -INFINITY;
-        for (int q = 0; q < split; ++q) {
-            const float v = split > 1 ? ld_shared_cluster_f32(mapa_shared(smem_u32(pm + 4 * CR_ROWS + r), q)) : pm[4 * CR_ROWS + r];
-            mm = fmaxf(mm, v);
-        }
+#pragma unroll
+        for (int q = 0; q < CR_MAX_SPLIT; ++q)
+            if (q < split) mm = fmaxf(mm, stat[q * rows + r].x);
         const float b = mm == -INFINITY ? 0.f : mm;
-        float x = 0.f, y = 0.f, ls = 0.f;
-        for (int q = 0; q < split; ++q) {
-            if (split > 1) {
-                const float f = ex2(ld_shared_cluster_f32(mapa_shared(smem_u32(pm + 4 * CR_ROWS + r), q)) - b);
-                const uint32_t a = mapa_shared(smem_u32(mine + r * S::COLS + c), q);
-                x = fmaf(f, ld_shared_cluster_f32(a), x);
-                y = fmaf(f, ld_shared_cluster_f32(a + 4), y);
-                ls = fmaf(f, ld_shared_cluster_f32(mapa_shared(smem_u32(pl + 4 * CR_ROWS + r), q)), ls);
-            } else {
-                x = mine[r * S::COLS + c];
-                y = mine[r * S::COLS + c + 1];
-                ls = pl[4 * CR_ROWS + r];
+        float2 sum = make_float2(0.f, 0.f);
+        float ls = 0.f;
+#pragma unroll
+        for (int q = 0; q < CR_MAX_SPLIT; ++q)
+            if (q < split) {
+                const float2 ml = stat[q * rows + r], v = mail[q * per + e / split];
+                const float f = ex2(ml.x - b);
+                sum.x = fmaf(f, v.x, sum.x);
+                sum.y = fmaf(f, v.y, sum.y);
+                ls = fmaf(f, ml.y, ls);
             }
-        }
-        const float inv = mm == -INFINITY && ls == 0.f ? 0.f : 1.f / ls;   // nothing seen: zeros
+        const float inv = ls == 0.f ? 0.f : 1.f / ls;   // nothing seen: zeros (a sum over anything is at least 1)
         const int row = r0 + r;
         uint8_t* dst = p.out + batch * p.os[0] + (kv_head * p.group + row % p.group) * p.os[1] + (row / p.group) * p.os[2] + 2 * c;
-        *reinterpret_cast<uint32_t*>(dst) = pack_h16<F16>(x * inv, y * inv);
+        *reinterpret_cast<uint32_t*>(dst) = pack_h16<F16>(sum.x * inv, sum.y * inv);
     }
-    if (split > 1) cluster_sync_all();   // peers may still read this CTA's sums
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -772,13 +858,12 @@ static int cross_tmap(CUtensorMap* map, const CrossTensor& t, int dim, int dtype
 }
 
 template <bool F16, bool MASK>
-static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const CrossTileParams& p,
-                             dim3 grid, cudaStream_t stream) {
+static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CrossTileParams& p, int grid, int table_bytes,
+                             cudaStream_t stream) {
     auto kern = cross_tile_kernel<F16, MASK>;
     static std::atomic<uint64_t> attr_done{0};
-    if (int rc = ensure_dynamic_smem(kern, CT_SMEM + (MASK ? CT_MASK_STATES / 8 : 0), attr_done)) return rc;
-    const int smem = CT_SMEM + (MASK ? (p.st.kv_len + CT_BN - 1) / CT_BN * (CT_BN / 8) : 0);
-    kern<<<grid, CT_THREADS, smem, stream>>>(tq, tk, tv, to, p);
+    if (int rc = ensure_dynamic_smem(kern, CT_SMEM + CT_TABLE_BYTES, attr_done)) return rc;
+    kern<<<grid, CT_THREADS, CT_SMEM + table_bytes, stream>>>(tq, tk, tv, p);
     SVDQ_CUDA(cudaGetLastError());
     return SVDQ_OK;
 }
@@ -787,11 +872,11 @@ template <bool F16, int NK>
 static int launch_cross_rows(const CrossRowsParams& p, int pairs, int split, cudaStream_t stream) {
     auto kern = cross_rows_kernel<F16, NK>;
     static std::atomic<uint64_t> attr_done{0};
-    if (int rc = ensure_dynamic_smem(kern, CrossRowsSizes<NK>::SMEM, attr_done)) return rc;
+    if (int rc = ensure_dynamic_smem(kern, CrossRowsSizes<NK>::smem(CR_ROWS, CR_MAX_SPLIT), attr_done)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(pairs * split, (p.q_rows + CR_ROWS - 1) / CR_ROWS, 1);
     cfg.blockDim = dim3(CR_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = CrossRowsSizes<NK>::SMEM;
+    cfg.dynamicSmemBytes = CrossRowsSizes<NK>::smem(p.q_rows < CR_ROWS ? p.q_rows : CR_ROWS, split);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -880,7 +965,7 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         p.scale_log2 = scale_log2;
         // states per sample as far as the host knows
         const long long len = a->kv_offsets ? (a->kv_len + a->batch - 1) / a->batch : a->kv_len;
-        const long long tiles = (len + CR_KEYS - 1) / CR_KEYS, ctas = kv_pairs * ((q_rows + CR_ROWS - 1) / CR_ROWS);
+        const long long tiles = (len + CR_TILE - 1) / CR_TILE, ctas = kv_pairs * ((q_rows + CR_ROWS - 1) / CR_ROWS);
         int split = 1;
         while (split < CR_MAX_SPLIT && ctas * split < 2ll * sms && 2 * split <= tiles) split *= 2;
         return f16 ? launch_cross_rows_dim<true>(p, static_cast<int>(kv_pairs), split, st) : launch_cross_rows_dim<false>(p, static_cast<int>(kv_pairs), split, st);
@@ -892,13 +977,28 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
     p.group = group;
     p.scale_log2 = scale_log2;
     if (int rc = status_words(&p.status)) return rc;
-    CUtensorMap mq, mk, mv, mo;
-    int obm, ohm;
+    const int q_tiles = (a->q_len + CT_BM - 1) / CT_BM;
+    const long long items = static_cast<long long>(a->batch) * a->heads * q_tiles;
+    SVDQ_CHECK_ARG(items < (1ll << 30), "cross_attention: too many query tiles");
+    p.out = static_cast<uint8_t*>(a->out);
+    for (int i = 0; i < 3; ++i) p.os[i] = 2 * a->o_stride[i];
+    p.heads = a->heads;
+    p.q_tiles = q_tiles;
+    p.items = static_cast<int>(items);
+    p.batch = a->batch;
+    CUtensorMap mq, mk, mv;
     if (int rc = cross_tmap(&mq, tq, a->head_dim, a->dtype, CT_BM, &p.q_bmul, &p.q_hmul)) return rc;
-    if (int rc = cross_tmap(&mk, tk, a->head_dim, a->dtype, CT_BN / 2, &p.k_bmul, &p.k_hmul)) return rc;
-    if (int rc = cross_tmap(&mv, tv, a->head_dim, a->dtype, CT_BN / 2, &p.v_bmul, &p.v_hmul)) return rc;
-    if (int rc = cross_tmap(&mo, to, a->head_dim, a->dtype, 32, &obm, &ohm)) return rc;
-    const dim3 grid((a->q_len + CT_BM - 1) / CT_BM, a->heads, a->batch);
-    if (a->mask) return f16 ? launch_cross_tile<true, true>(mq, mk, mv, mo, p, grid, st) : launch_cross_tile<false, true>(mq, mk, mv, mo, p, grid, st);
-    return f16 ? launch_cross_tile<true, false>(mq, mk, mv, mo, p, grid, st) : launch_cross_tile<false, false>(mq, mk, mv, mo, p, grid, st);
+    if (int rc = cross_tmap(&mk, tk, a->head_dim, a->dtype, CT_BN, &p.k_bmul, &p.k_hmul)) return rc;
+    if (int rc = cross_tmap(&mv, tv, a->head_dim, a->dtype, CT_BN, &p.v_bmul, &p.v_hmul)) return rc;
+    // two CTAs per SM that work through the items; without room for every sample's mask bits, one CTA per item with its sample's
+    const int resident = p.items < 2 * sms ? p.items : 2 * sms;
+    if (a->mask) {
+        p.mask_words = (a->kv_len + CT_BN - 1) / CT_BN * (CT_BN / 32);
+        p.table = static_cast<long long>(p.mask_words) * a->batch * 4 <= CT_TABLE_BYTES;
+        const int bytes = p.mask_words * 4 * (p.table ? a->batch : 1), grid = p.table ? resident : p.items;
+        return f16 ? launch_cross_tile<true, true>(mq, mk, mv, p, grid, bytes, st) : launch_cross_tile<false, true>(mq, mk, mv, p, grid, bytes, st);
+    }
+    p.table = a->batch <= CT_RANGES;
+    const int bytes = p.table ? a->batch * 8 : 0;
+    return f16 ? launch_cross_tile<true, false>(mq, mk, mv, p, resident, bytes, st) : launch_cross_tile<false, false>(mq, mk, mv, p, resident, bytes, st);
 }
