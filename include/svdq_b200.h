@@ -403,7 +403,7 @@ typedef struct svdq_cross_attention_args {
                                  which then have no batch dimension (clamped to 0..kv_len, the number of rows)                  */
     const void* mask;         /* NULL, or bytes [batch, kv_len] on the device: states whose byte is not 0 exist              */
     int64_t mask_stride;      /* bytes between the mask's rows                                   */
-    int32_t batch, heads, kv_heads, q_len, kv_len, head_dim;      /* at most one of kv_lens, kv_offsets, mask; kv_len <= 65536
+    int32_t batch, heads, kv_heads, q_len, kv_len, head_dim;      /* at most one of kv_lens, kv_offsets, mask; kv_len <= 32768
                                                                      with a mask                 */
     float scale;              /* positive                                                        */
     int32_t dtype;            /* SVDQ_DTYPE_* of q, k, v and out                                 */

@@ -63,10 +63,11 @@ constexpr int CT_PRODUCER_WARP = 4, CT_MMA_WARP = 5, CT_ZERO_WARP = 6;
 // registers move inside the pool the CTA was launched with (256 threads x 128)
 constexpr int CT_REGS_SOFTMAX = 184, CT_REGS_OTHER = 72;
 static_assert(4 * CT_REGS_SOFTMAX + 4 * CT_REGS_OTHER <= 8 * 128, "register budget");
-constexpr int CT_MASK_STATES = 65536;               // longest state list a mask may cover (its bits are kept in shared memory)
+constexpr int CT_MASK_STATES = 32768;               // longest state list a mask may cover (its bits are kept in shared memory)
+constexpr int CT_STAGE_BYTES = 4 * 32 * 64;         // output: 32 rows x 32 channels per softmax warp on their way to memory
 constexpr int CT_BAR_BYTES = 256;
-constexpr int CT_SMEM = 1024 + CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + CT_BAR_BYTES;   // 97 KB: two CTAs per SM
-constexpr int CT_TABLE_BYTES = 12 * 1024;           // the samples' ranges or mask bits
+constexpr int CT_SMEM = 1024 + CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + CT_STAGE_BYTES + CT_BAR_BYTES;   // 105 KB: two CTAs per SM
+constexpr int CT_TABLE_BYTES = 6 * 1024;           // the samples' ranges or mask bits
 constexpr int CT_RANGES = CT_TABLE_BYTES / 8;       // most samples whose ranges are kept there
 constexpr int CT_TMEM_COLS = 256;                   // S: 2 x 64, O: 128
 constexpr long long CT_WAIT_CYCLES = 600000000ll;   // ~0.3 s
@@ -88,6 +89,7 @@ struct CrossTileParams {
     uint8_t* out;
     long long os[3];                                      // batch, head, token strides in bytes
     int q_len, dim, group, heads, q_tiles, items, batch;  // item = (batch * heads + head) * q_tiles + tile
+    int per_batch, step_batch, step_rem;                  // heads * q_tiles; gridDim.x / per_batch and gridDim.x % per_batch
     int table;                                            // ranges (or mask bits) of all samples are in shared memory
     int mask_words;                                       // 32-bit words of mask bits per sample
     int q_bmul, q_hmul, k_bmul, k_hmul, v_bmul, v_hmul;   // 0 where that dimension is broadcast (stride 0): its coordinate is then 0
@@ -102,15 +104,15 @@ struct CrossWalk {
     const int2* ranges;
     const uint32_t* words;
     int item, j, valid;      // current block: its leading `valid` states are looked at
-    int start, count, batch;
+    int start, count, batch, rem;   // rem: item within its sample
     const uint32_t* w;       // MASK: the sample's bits
 
     __device__ __forceinline__ CrossWalk(const CrossTileParams& p_, const int2* r, const uint32_t* w_)
-        : p(p_), ranges(r), words(w_), item(blockIdx.x), j(-1), valid(0), start(0), count(0), batch(0), w(w_) {
+        : p(p_), ranges(r), words(w_), item(blockIdx.x), j(-1), valid(0), start(0), count(0), batch(blockIdx.x / p_.per_batch),
+          rem(blockIdx.x % p_.per_batch), w(w_) {
         if (item < p.items) open();
     }
     __device__ __forceinline__ void open() {
-        batch = item / (p.heads * p.q_tiles);
         if (MASK) {
             start = 0;
             count = p.st.kv_len;
@@ -124,8 +126,8 @@ struct CrossWalk {
         }
         j = -1;
     }
-    __device__ __forceinline__ int head() const { return item / p.q_tiles % p.heads; }
-    __device__ __forceinline__ int q0() const { return item % p.q_tiles * CT_BM; }
+    __device__ __forceinline__ int head() const { return rem / p.q_tiles; }
+    __device__ __forceinline__ int q0() const { return rem % p.q_tiles * CT_BM; }
     __device__ __forceinline__ int look(int i) const {
         if constexpr (MASK) {
             const uint32_t a = w[2 * i], b = w[2 * i + 1];
@@ -144,6 +146,12 @@ struct CrossWalk {
     __device__ __forceinline__ bool next_item() {
         item += gridDim.x;
         if (item >= p.items) return false;
+        batch += p.step_batch;
+        rem += p.step_rem;
+        if (rem >= p.per_batch) {
+            rem -= p.per_batch;
+            ++batch;
+        }
         open();
         return true;
     }
@@ -174,7 +182,8 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     uint8_t* q_s = smem;
     uint8_t* k_s = q_s + CT_Q_BYTES;
     uint8_t* v_s = k_s + CT_SLOTS * CT_KV_BYTES;
-    CrossTileShared* sh = reinterpret_cast<CrossTileShared*>(v_s + CT_SLOTS * CT_KV_BYTES);
+    uint8_t* stage = v_s + CT_SLOTS * CT_KV_BYTES;
+    CrossTileShared* sh = reinterpret_cast<CrossTileShared*>(stage + CT_STAGE_BYTES);
     uint8_t* table = reinterpret_cast<uint8_t*>(sh) + CT_BAR_BYTES;
     int2* ranges = reinterpret_cast<int2*>(table);
     uint32_t* words = reinterpret_cast<uint32_t*>(table);
@@ -207,7 +216,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tmem_relinquish();
     }
     if constexpr (MASK) {
-        const int first = p.table ? 0 : blockIdx.x / (p.heads * p.q_tiles), count = p.table ? p.batch : 1;
+        const int first = p.table ? 0 : blockIdx.x / p.per_batch, count = p.table ? p.batch : 1;
         for (int w = warp; w < count * p.mask_words; w += CT_THREADS / 32) {
             const int b = w / p.mask_words, i = (w - b * p.mask_words) * 32 + lane;
             const uint32_t bits = __ballot_sync(0xffffffffu, i < p.st.kv_len && p.st.mask[(first + b) * p.st.mask_stride + i] != 0);
@@ -375,7 +384,8 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             ++n;
             more = next_there;
-            cur.item = nxt.item; cur.j = nxt.j; cur.valid = nxt.valid; cur.start = nxt.start; cur.count = nxt.count; cur.batch = nxt.batch; cur.w = nxt.w;
+            cur.item = nxt.item; cur.j = nxt.j; cur.valid = nxt.valid; cur.start = nxt.start; cur.count = nxt.count; cur.batch = nxt.batch; cur.rem = nxt.rem;
+            cur.w = nxt.w;
         }
     } else if (warp >= CT_ZERO_WARP) {
         reg_dealloc<CT_REGS_OTHER>();
@@ -456,111 +466,133 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     if (chunk * 32 + i >= it.valid) a[i] = 0xff800000u;
             }
         };
-        uint32_t n = 0;
-        bool ok = true;
-        if (it.item < p.items) do {
-            float m_used = 0.f, l = 0.f;
-            bool first = true;
-            while (it.next_in_item()) {
-                const uint32_t slot = n & 1;
-                if (!__all_sync(0xffffffffu, mbar_wait(&sh->s_full[slot], (n >> 1) & 1, CT_WAIT_CYCLES))) {
-                    if (lane == 0) timeout(960);
-                    ok = false;
-                    break;
-                }
-                tc_fence_after_sync();
-                const bool two = it.valid > 32;
-                const uint32_t st = s_tmem + slot * CT_BN;
-                uint32_t s0[32], s1[32], w[16];
-                tc_ld_32x32b_x32(st, s0);
-                if (two) tc_ld_32x32b_x32(st + 32, s1);
-                tc_wait_ld();
-                hide(s0, 0);
-                float mx = max32(s0);
-                if (two) {
-                    hide(s1, 1);
-                    mx = fmaxf(mx, max32(s1));
-                }
-                const float ms = mx * p.scale_log2;
-                const bool grow = first || ms > m_used + CT_RESCALE_STEP;
-                if (!first && __any_sync(0xffffffffu, grow)) {
-                    // O is written by the previous P V product until it has completed
-                    if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, CT_WAIT_CYCLES))) {
-                        if (lane == 0) timeout(970);
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after_sync();
-                    const float alpha = grow ? ex2(m_used - ms) : 1.f;
-                    l *= alpha;
-#pragma unroll 1
-                    for (int c = 0; c < p.dim; c += 16) {
-                        uint32_t o[16];
-                        tc_ld_32x32b_x16(o_tmem + c, o);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tc_st_32x32b_x16(o_tmem + c, o);
-                    }
-                    tc_wait_st();
-                }
-                if (grow) m_used = ms;
-                // P over this thread's own S values, which are all in registers by now
-                l += exp32(s0, m_used, w);
-                tc_st_32x32b_x16(st, w);
-                if (two) {
-                    l += exp32(s1, m_used, w);
-                    tc_st_32x32b_x16(st + 16, w);
-                }
-                tc_wait_st();
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->p_full[slot]);
-                first = false;
-                ++n;
-            }
-            if (!ok) break;
-            // ---- O / l -> global
-            const int qrow = it.q0() + warp * 32 + lane;
-            uint8_t* dst = p.out + it.batch * p.os[0] + it.head() * p.os[1] + qrow * p.os[2];
-            if (first) {   // no states: zeros
+        // samples without states: zeros
+        {
+            CrossWalk<MASK> e(p, ranges, words);
+            if (e.item < p.items) do {
+                if (e.next_in_item()) continue;
+                const int qrow = e.q0() + warp * 32 + lane;
+                uint8_t* dst = p.out + e.batch * p.os[0] + e.head() * p.os[1] + qrow * p.os[2];
                 if (qrow < p.q_len)
                     for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(dst + 2 * c) = make_uint4(0, 0, 0, 0);
-                continue;
-            }
+            } while (e.next_item());
+        }
+        uint32_t n = 0;
+        bool ok = true;
+        float m_used = 0.f, l = 0.f;
+        int item = -1, q0 = 0;                 // item in work
+        uint8_t* out = nullptr;                // its rows
+        // O / l of the item in work -> global memory; its last block is number n - 1
+        auto finish = [&]() {
             if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, CT_WAIT_CYCLES))) {
                 if (lane == 0) timeout(980);
-                ok = false;
-                break;
+                return false;
             }
             tc_fence_after_sync();
             const float inv = 1.f / l;
+            uint8_t* box = stage + warp * (CT_STAGE_BYTES / 4);   // [32 rows][64 bytes], 16-byte pieces swizzled by row / 2
 #pragma unroll 1
-            for (int c = 0; c < p.dim; c += 64) {
-                uint32_t a[32], b[32];
-                tc_ld_32x32b_x32(o_tmem + c, a);
-                if (c + 32 < p.dim) tc_ld_32x32b_x32(o_tmem + c + 32, b);
+            for (int c = 0; c < p.dim; c += 32) {
+                uint32_t o[32];
+                tc_ld_32x32b_x32(o_tmem + c, o);
                 tc_wait_ld();
-                if (c + 64 >= p.dim) {   // all of O is in registers: the next item's P V may overwrite it
+                if (c + 32 >= p.dim) {   // all of O has been read: the next item's P V may overwrite it
                     tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh->o_free);
                 }
-                if (qrow < p.q_len) {
+                // through shared memory, so that a store instruction covers eight rows' 64 bytes and not 32 rows' 16 (one line of L1 a cycle:
+                // 3900 cycles per item the other way, a quarter of its time)
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        if (c + u * 8 < p.dim) {
-                            const uint32_t(&o)[32] = u < 4 ? a : b;
-                            uint32_t w4[4];
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t w4[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                w4[e] = pack_h16<F16>(__uint_as_float(o[(u & 3) * 8 + 2 * e]) * inv, __uint_as_float(o[(u & 3) * 8 + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4*>(dst + 2 * (c + u * 8)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        w4[e] = pack_h16<F16>(__uint_as_float(o[u * 8 + 2 * e]) * inv, __uint_as_float(o[u * 8 + 2 * e + 1]) * inv);
+                    *reinterpret_cast<uint4*>(box + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
                 }
+                __syncwarp();
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int r = u * 8 + (lane >> 2), piece = lane & 3;
+                    const uint4 v = *reinterpret_cast<const uint4*>(box + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+                    const int qrow = q0 + warp * 32 + r;
+                    if (qrow < p.q_len && c + piece * 8 < p.dim) *reinterpret_cast<uint4*>(out + qrow * p.os[2] + 2 * (c + piece * 8)) = v;
+                }
+                __syncwarp();
             }
-        } while (it.next_item());
+            return true;
+        };
+        while (it.next()) {
+            const uint32_t slot = n & 1;
+            const bool first = it.item != item;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh->s_full[slot], (n >> 1) & 1, CT_WAIT_CYCLES))) {
+                if (lane == 0) timeout(960);
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            const bool two = it.valid > 32;
+            const uint32_t st = s_tmem + slot * CT_BN;
+            uint32_t s0[32], s1[32], w0[16], w1[16];
+            tc_ld_32x32b_x32(st, s0);
+            if (two) tc_ld_32x32b_x32(st + 32, s1);
+            tc_wait_ld();
+            hide(s0, 0);
+            float mx = max32(s0);
+            if (two) {
+                hide(s1, 1);
+                mx = fmaxf(mx, max32(s1));
+            }
+            const float ms = mx * p.scale_log2;
+            const bool grow = first || ms > m_used + CT_RESCALE_STEP;
+            if (!first && __any_sync(0xffffffffu, grow)) {
+                // O is written by the previous P V product until it has completed
+                if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, CT_WAIT_CYCLES))) {
+                    if (lane == 0) timeout(970);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+                const float alpha = grow ? ex2(m_used - ms) : 1.f;
+                l *= alpha;
+#pragma unroll 1
+                for (int c = 0; c < p.dim; c += 16) {
+                    uint32_t o[16];
+                    tc_ld_32x32b_x16(o_tmem + c, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tc_st_32x32b_x16(o_tmem + c, o);
+                }
+                tc_wait_st();
+            }
+            const float m = grow ? ms : m_used;
+            float sum = exp32(s0, m, w0);
+            if (two) sum += exp32(s1, m, w1);
+            if (first) {
+                // the previous item's O, behind this item's first exponentials: its last P V runs under them
+                if (item >= 0 && !finish()) {
+                    ok = false;
+                    break;
+                }
+                item = it.item;
+                q0 = it.q0();
+                out = p.out + it.batch * p.os[0] + it.head() * p.os[1];
+                l = 0.f;
+            }
+            m_used = m;
+            l += sum;
+            // P over this thread's own S values, which are all in registers by now
+            tc_st_32x32b_x16(st, w0);
+            if (two) tc_st_32x32b_x16(st + 16, w1);
+            tc_wait_st();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->p_full[slot]);
+            ++n;
+        }
+        if (ok && item >= 0) finish();
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -986,6 +1018,7 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
     p.q_tiles = q_tiles;
     p.items = static_cast<int>(items);
     p.batch = a->batch;
+    p.per_batch = a->heads * q_tiles;
     CUtensorMap mq, mk, mv;
     if (int rc = cross_tmap(&mq, tq, a->head_dim, a->dtype, CT_BM, &p.q_bmul, &p.q_hmul)) return rc;
     if (int rc = cross_tmap(&mk, tk, a->head_dim, a->dtype, CT_BN, &p.k_bmul, &p.k_hmul)) return rc;
@@ -996,9 +1029,13 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         p.mask_words = (a->kv_len + CT_BN - 1) / CT_BN * (CT_BN / 32);
         p.table = static_cast<long long>(p.mask_words) * a->batch * 4 <= CT_TABLE_BYTES;
         const int bytes = p.mask_words * 4 * (p.table ? a->batch : 1), grid = p.table ? resident : p.items;
+        p.step_batch = grid / p.per_batch;
+        p.step_rem = grid % p.per_batch;
         return f16 ? launch_cross_tile<true, true>(mq, mk, mv, p, grid, bytes, st) : launch_cross_tile<false, true>(mq, mk, mv, p, grid, bytes, st);
     }
     p.table = a->batch <= CT_RANGES;
+    p.step_batch = resident / p.per_batch;
+    p.step_rem = resident % p.per_batch;
     const int bytes = p.table ? a->batch * 8 : 0;
     return f16 ? launch_cross_tile<true, false>(mq, mk, mv, p, resident, bytes, st) : launch_cross_tile<false, false>(mq, mk, mv, p, resident, bytes, st);
 }

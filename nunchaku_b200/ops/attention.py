@@ -73,7 +73,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
     q: [B, H, Tq, D]; k, v: [B, Hk, T, D] views with any (batch, head, token) strides (multiples of 8 elements; batch and head may be
     expanded), bf16 or fp16, D a multiple of 8 up to 128, H a multiple of Hk (query head h reads stored head h // (H // Hk)).
     Which states exist, at most one of: ``kv_lens`` int32 [B] (the first so many of each sample), ``mask`` bool [B, T] (those that are
-    True; T up to 65536), ``kv_offsets`` int32 [B + 1] (k and v are then packed [total, Hk, D], sample b owning rows
+    True; T up to 32768), ``kv_offsets`` int32 [B + 1] (k and v are then packed [total, Hk, D], sample b owning rows
     ``kv_offsets[b]:kv_offsets[b + 1]``); all on q's device, read there (lengths outside 0..T are clamped).  None: all T.  A sample without
     states gets zeros; states that do not exist may hold anything, NaN included.
     out: [B, Tq, H*D] (default: a new tensor) or a [B, H, Tq, D] view of one.  scale defaults to D ** -0.5 and must be positive."""

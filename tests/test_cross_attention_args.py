@@ -58,7 +58,7 @@ def test_refuses(lib, bad):
 
 def test_refuses_null_and_a_mask_that_is_too_long(lib):
     assert lib.load().svdq_cross_attention(None, None) == lib.SVDQ_ERR_INVALID_ARGUMENT
-    assert _call(lib, mask=64, mask_stride=70000, kv_len=65537) == lib.SVDQ_ERR_UNSUPPORTED
+    assert _call(lib, mask=64, mask_stride=70000, kv_len=32769) == lib.SVDQ_ERR_UNSUPPORTED
 
 
 def test_python_layer_refuses_cpu_tensors():

@@ -262,5 +262,5 @@ def test_python_layer_refuses():
         with pytest.raises(ValueError):
             cross_attention(*a, **kw)
     with pytest.raises(NotImplementedError):
-        cross_attention(q, z(2, 2, 65537, 64), z(2, 2, 65537, 64), mask=z(2, 65537, dtype=torch.bool))
+        cross_attention(q, z(2, 2, 32769, 64), z(2, 2, 32769, 64), mask=z(2, 32769, dtype=torch.bool))
     assert _lib.device_status() == (0, 0)
