@@ -29,6 +29,7 @@
 #include "attention_common.cuh"
 #include "host_common.h"
 
+
 namespace svdq {
 
 struct CrossStates {
@@ -58,29 +59,27 @@ constexpr int CT_Q_HALF = CT_BM * 128;              // 128 rows x 64 channels
 constexpr int CT_KV_HALF = CT_BN * 128;
 constexpr int CT_Q_BYTES = 2 * CT_Q_HALF, CT_KV_BYTES = 2 * CT_KV_HALF;
 constexpr int CT_SLOTS = 2;                         // of K and of V each
-constexpr int CT_THREADS = 256;
-constexpr int CT_PRODUCER_WARP = 4, CT_MMA_WARP = 5, CT_ZERO_WARP = 6;
-// registers move inside the pool the CTA was launched with (256 threads x 128)
-constexpr int CT_REGS_SOFTMAX = 184, CT_REGS_OTHER = 72;
-static_assert(4 * CT_REGS_SOFTMAX + 4 * CT_REGS_OTHER <= 8 * 128, "register budget");
+constexpr int CT_THREADS = 12 * 32;
+constexpr int CT_MMA_WARP = 8, CT_QK_WARP = 9, CT_V_WARP = 10;   // 0-3 softmax, 4-7 output, 11 nothing
 constexpr int CT_MASK_STATES = 32768;               // longest state list a mask may cover (its bits are kept in shared memory)
-constexpr int CT_STAGE_BYTES = 4 * 32 * 64;         // output: 32 rows x 32 channels per softmax warp on their way to memory
+constexpr int CT_STAGE_BYTES = 4 * 32 * 64;         // output: 32 rows x 32 channels per output warp on their way to memory
 constexpr int CT_BAR_BYTES = 256;
-constexpr int CT_SMEM = 1024 + CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + CT_STAGE_BYTES + CT_BAR_BYTES;   // 105 KB: two CTAs per SM
-constexpr int CT_TABLE_BYTES = 6 * 1024;           // the samples' ranges or mask bits
-constexpr int CT_RANGES = CT_TABLE_BYTES / 8;       // most samples whose ranges are kept there
+constexpr int CT_SUM_BYTES = 2 * CT_BM * 4;         // row sums of two items
+constexpr int CT_SMEM = 1024 + CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + CT_STAGE_BYTES + CT_SUM_BYTES + CT_BAR_BYTES;   // 106 KB: two CTAs per SM
+constexpr int CT_TABLE_BYTES = 6 * 1024;            // the samples' ranges or mask bits
 constexpr int CT_TMEM_COLS = 256;                   // S: 2 x 64, O: 128
-constexpr long long CT_WAIT_CYCLES = 600000000ll;   // ~0.3 s
+constexpr int CT_WAIT_LOOKS = 1 << 20;              // each of up to a microsecond
 constexpr float CT_RESCALE_STEP = 8.f;
-static_assert(2 * (CT_SMEM + CT_TABLE_BYTES + 1024) <= 228 * 1024 && CT_TABLE_BYTES >= CT_MASK_STATES / 8, "two CTAs per SM");
+static_assert(2 * (CT_SMEM + CT_TABLE_BYTES + 1024) <= 228 * 1024 && CT_TABLE_BYTES >= CT_MASK_STATES / 8 + 8, "two CTAs per SM");
 
 struct CrossTileShared {
-    uint64_t q_full, q_empty, k_full[CT_SLOTS], k_empty[CT_SLOTS], s_full[2], p_full[2], pv_done[2], o_free;
-    // A block of V whose rows are all to be seen lands on v_full, which the issuer waits for; one with rows to be zeroed lands on
-    // vh_full, which warp 6 waits for, and the issuer waits for v_zeroed: so every barrier has one sequence of phases that
-    // its waiter follows without gaps.
-    uint64_t v_full[CT_SLOTS], vh_full[CT_SLOTS], v_zeroed[CT_SLOTS], v_empty[CT_SLOTS];
+    // A slot of K is free when its Q K^T is done (s_full), one of V when its P V is (pv_done), Q when the item's last Q K^T is: the
+    // producers wait for those.  A block of V whose rows are all to be seen lands on v_full, which the issuer waits for; one with rows
+    // to be zeroed lands on vh_full, which the softmax warps wait for before they hand over P: so every barrier has one sequence of
+    // phases that its waiters follow without gaps.
+    uint64_t q_full, k_full[CT_SLOTS], v_full[CT_SLOTS], vh_full[CT_SLOTS], s_full[2], p_full[2], pv_done[2], l_full[2], o_free;
     uint32_t tmem_base;
+    int failed;            // the code of a wait that ran out
 };
 static_assert(sizeof(CrossTileShared) <= CT_BAR_BYTES, "barrier block");
 
@@ -89,89 +88,76 @@ struct CrossTileParams {
     uint8_t* out;
     long long os[3];                                      // batch, head, token strides in bytes
     int q_len, dim, group, heads, q_tiles, items, batch;  // item = (batch * heads + head) * q_tiles + tile
-    int per_batch, step_batch, step_rem;                  // heads * q_tiles; gridDim.x / per_batch and gridDim.x % per_batch
-    int table;                                            // ranges (or mask bits) of all samples are in shared memory
     int mask_words;                                       // 32-bit words of mask bits per sample
     int q_bmul, q_hmul, k_bmul, k_hmul, v_bmul, v_hmul;   // 0 where that dimension is broadcast (stride 0): its coordinate is then 0
     float scale_log2;
     int* status;
 };
 
-// The blocks of states that a CTA works through, item after item, as each of its roles sees them.
+// Bounded wait of a whole warp that lets the hardware suspend it between looks (polling takes issue slots from the softmax warps).
+// False, on every lane, when it runs out; the code is reported at the kernel's end.
+__device__ __forceinline__ bool ct_wait(uint64_t* bar, uint32_t parity, CrossTileShared* sh, int code) {
+    uint32_t ok = 0;
+#pragma unroll 1
+    for (int i = 0; i < CT_WAIT_LOOKS && !ok; ++i)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(1000u)
+            : "memory");
+    if (__all_sync(0xffffffffu, ok != 0)) return true;
+    sh->failed = code;
+    return false;
+}
+
+// The items that a CTA works through, as each of its roles sees them: states [start, start + count) of the item's sample (with a mask:
+// up to the last one that is to be seen) in blocks of 64.  Starts in front of the first.
 template <bool MASK>
-struct CrossWalk {
+struct CrossItems {
     const CrossTileParams& p;
     const int2* ranges;
     const uint32_t* words;
-    int item, j, valid;      // current block: its leading `valid` states are looked at
-    int start, count, batch, rem;   // rem: item within its sample
-    const uint32_t* w;       // MASK: the sample's bits
+    int item, end, batch, head, tile, start, count, blocks;   // end: behind this CTA's last item
 
-    __device__ __forceinline__ CrossWalk(const CrossTileParams& p_, const int2* r, const uint32_t* w_)
-        : p(p_), ranges(r), words(w_), item(blockIdx.x), j(-1), valid(0), start(0), count(0), batch(blockIdx.x / p_.per_batch),
-          rem(blockIdx.x % p_.per_batch), w(w_) {
-        if (item < p.items) open();
-    }
-    __device__ __forceinline__ void open() {
-        if (MASK) {
-            start = 0;
-            count = p.st.kv_len;
-            w = words + (p.table ? batch * p.mask_words : 0);
-        } else if (p.table) {
+    __device__ __forceinline__ CrossItems(const CrossTileParams& p_, const int2* r, const uint32_t* w, int first, int end_, int batch_, int head_, int tile_)
+        : p(p_), ranges(r), words(w), item(first - 1), end(end_), batch(batch_), head(head_), tile(tile_ - 1), start(0), count(0), blocks(0) {}
+    // to the next item (EMPTY: even if it has no states); false behind the last
+    template <bool EMPTY = false>
+    __device__ __forceinline__ bool advance() {
+#pragma unroll 1
+        do {
+            if (++item >= end) return false;
+            if (++tile == p.q_tiles) {
+                tile = 0;
+                if (++head == p.heads) {
+                    head = 0;
+                    ++batch;
+                }
+            }
             const int2 r = ranges[batch];
             start = r.x;
             count = r.y;
-        } else {
-            cross_range(p.st, batch, start, count);
-        }
-        j = -1;
-    }
-    __device__ __forceinline__ int head() const { return rem / p.q_tiles; }
-    __device__ __forceinline__ int q0() const { return rem % p.q_tiles * CT_BM; }
-    __device__ __forceinline__ int look(int i) const {
-        if constexpr (MASK) {
-            const uint32_t a = w[2 * i], b = w[2 * i + 1];
-            return b ? 64 - __clz(b) : a ? 32 - __clz(a) : 0;
-        }
-        return min(count - i * CT_BN, CT_BN);
-    }
-    // next block of this item that has states
-    __device__ __forceinline__ bool next_in_item() {
-        while (++j * CT_BN < count) {
-            valid = look(j);
-            if (valid) return true;
-        }
-        return false;
-    }
-    __device__ __forceinline__ bool next_item() {
-        item += gridDim.x;
-        if (item >= p.items) return false;
-        batch += p.step_batch;
-        rem += p.step_rem;
-        if (rem >= p.per_batch) {
-            rem -= p.per_batch;
-            ++batch;
-        }
-        open();
+            blocks = (count + CT_BN - 1) / CT_BN;
+        } while (!EMPTY && blocks == 0);
         return true;
     }
-    // next block that has states, of this item or a later one
-    __device__ __forceinline__ bool next() {
-        if (item >= p.items) return false;
-        while (!next_in_item())
-            if (!next_item()) return false;
-        return true;
-    }
+    __device__ __forceinline__ int valid(int j) const { return min(count - j * CT_BN, CT_BN); }
+    __device__ __forceinline__ const uint32_t* bits(int j) const { return words + batch * p.mask_words + 2 * j; }
     // some of the rows of V that P V reads (valid rounded up to 16) must not be seen and are not zeros already
-    __device__ __forceinline__ bool holes() const {
-        const int up = (valid + 15) & ~15;
+    __device__ __forceinline__ bool holes(int j) const {
         if constexpr (MASK) {
+            const int up = (valid(j) + 15) & ~15;
             const uint32_t wa = up >= 32 ? 0xffffffffu : (1u << up) - 1u, wb = up >= 64 ? 0xffffffffu : up > 32 ? (1u << (up - 32)) - 1u : 0u;
-            return (w[2 * j] & wa) != wa || (w[2 * j + 1] & wb) != wb;
+            return (bits(j)[0] & wa) != wa || (bits(j)[1] & wb) != wb;
         }
-        return up != valid && (p.st.kv_lens || p.st.kv_offsets);   // without them the rows past the end are filled with zeros by the copy
+        return (count & 15) != 0 && j + 1 == blocks && (p.st.kv_lens || p.st.kv_offsets);   // without them the rows past the end are filled with zeros by the copy
     }
 };
+
+// What an item costs, in tenths of a block of 64 states: its blocks, and what it takes to change queries and hand the output over.
+__device__ __forceinline__ float cross_item_cost(int count) { return static_cast<float>(10 * ((count + CT_BN - 1) / CT_BN) + 8); }
 
 template <bool F16, bool MASK>
 __global__ void __launch_bounds__(CT_THREADS, 2)
@@ -183,29 +169,28 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     uint8_t* k_s = q_s + CT_Q_BYTES;
     uint8_t* v_s = k_s + CT_SLOTS * CT_KV_BYTES;
     uint8_t* stage = v_s + CT_SLOTS * CT_KV_BYTES;
-    CrossTileShared* sh = reinterpret_cast<CrossTileShared*>(stage + CT_STAGE_BYTES);
+    float* sums = reinterpret_cast<float*>(stage + CT_STAGE_BYTES);
+    CrossTileShared* sh = reinterpret_cast<CrossTileShared*>(stage + CT_STAGE_BYTES + CT_SUM_BYTES);
     uint8_t* table = reinterpret_cast<uint8_t*>(sh) + CT_BAR_BYTES;
     int2* ranges = reinterpret_cast<int2*>(table);
-    uint32_t* words = reinterpret_cast<uint32_t*>(table);
+    uint32_t* words = reinterpret_cast<uint32_t*>(table + p.batch * 8);   // MASK: behind the ranges
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int halves = p.dim > 64 ? 2 : 1;
 
     if (tid == 0) {
         mbar_init(&sh->q_full, 1);
-        mbar_init(&sh->q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh->k_full[i], 1);
-            mbar_init(&sh->k_empty[i], 1);
             mbar_init(&sh->v_full[i], 1);
             mbar_init(&sh->vh_full[i], 1);
-            mbar_init(&sh->v_zeroed[i], 1);
-            mbar_init(&sh->v_empty[i], 1);
+            mbar_init(&sh->l_full[i], 4);
             mbar_init(&sh->s_full[i], 1);
             mbar_init(&sh->p_full[i], 4);
             mbar_init(&sh->pv_done[i], 1);
         }
         mbar_init(&sh->o_free, 4);
+        sh->failed = 0;
         fence_mbar_init();
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_k);
@@ -215,14 +200,20 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tmem_alloc(&sh->tmem_base, CT_TMEM_COLS);
         tmem_relinquish();
     }
+    // the samples' ranges and mask bits
     if constexpr (MASK) {
-        const int first = p.table ? 0 : blockIdx.x / p.per_batch, count = p.table ? p.batch : 1;
-        for (int w = warp; w < count * p.mask_words; w += CT_THREADS / 32) {
-            const int b = w / p.mask_words, i = (w - b * p.mask_words) * 32 + lane;
-            const uint32_t bits = __ballot_sync(0xffffffffu, i < p.st.kv_len && p.st.mask[(first + b) * p.st.mask_stride + i] != 0);
-            if (lane == 0) words[w] = bits;
+        for (int b = tid; b < p.batch; b += CT_THREADS) ranges[b] = make_int2(0, 0);
+        __syncthreads();
+#pragma unroll 1
+        for (int w = warp; w < p.batch * p.mask_words; w += CT_THREADS / 32) {
+            const int b = w / p.mask_words, at = (w - b * p.mask_words) * 32, i = at + lane;
+            const uint32_t bits = __ballot_sync(0xffffffffu, i < p.st.kv_len && p.st.mask[b * p.st.mask_stride + i] != 0);
+            if (lane == 0) {
+                words[w] = bits;
+                if (bits) atomicMax(&ranges[b].y, at + 32 - __clz(bits));
+            }
         }
-    } else if (p.table) {
+    } else {
         for (int b = tid; b < p.batch; b += CT_THREADS) {
             int2 r;
             cross_range(p.st, b, r.x, r.y);
@@ -233,71 +224,50 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = sh->tmem_base;
-    auto timeout = [&](int code) {
-        atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
-        atomicExch(&p.status[1], code);
-    };
-
-    if (warp == CT_PRODUCER_WARP) {
-        reg_dealloc<CT_REGS_OTHER>();
-        // ------------------------------------------------------------------ producer
-        if (lane == 0) {
-            CrossWalk<MASK> it(p, ranges, words);
-            uint32_t n = 0, q_uses = 0, v_uses[2] = {0, 0};   // v_uses: bit = number of uses of v_full / vh_full of a slot, mod 2, and (bit + 2) whether any
-            int last_item = -1;
-            bool ok = true;
-            while (ok && it.next()) {
-                const int head = it.head(), kv_head = head / p.group, slot = n & 1;
-                if (it.item != last_item) {
-                    last_item = it.item;
-                    ok = mbar_wait(&sh->q_empty, (q_uses & 1) ^ 1, CT_WAIT_CYCLES);
-                    if (!ok) {
-                        timeout(900);
-                        break;
-                    }
-                    ++q_uses;
-                    mbar_arrive_expect_tx(&sh->q_full, halves * CT_Q_HALF);
-                    for (int h = 0; h < halves; ++h)
-                        tma_load_4d(q_s + h * CT_Q_HALF, &tm_q, &sh->q_full, h * 64, it.q0(), head * p.q_hmul, it.batch * p.q_bmul);
+    // This CTA's share: a run of items, cut so that the CTAs' costs are alike.  An item belongs to the CTA in whose span of the whole
+    // cost its own begins.  (Every warp for itself, 32 samples a turn; a CTA's end and the next one's start are the same computation.)
+    const int per_batch = p.heads * p.q_tiles;
+    int edge[2] = {static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.x) + 1};
+    if (gridDim.x < p.items) {
+        float total = 0.f;
+        for (int b = lane; b < p.batch; b += 32) total += cross_item_cost(ranges[b].y);
+#pragma unroll
+        for (int m = 16; m >= 1; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) edge[e] = p.items;
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e) {
+            const float at = total * (static_cast<float>(blockIdx.x + e) / static_cast<float>(gridDim.x));   // in costs of one item per sample
+            float before = 0.f;
+            int found = p.items;
+#pragma unroll 1
+            for (int b0 = 0; b0 < p.batch && blockIdx.x + e < gridDim.x; b0 += 32) {
+                const int b = b0 + lane;
+                const float c = b < p.batch ? cross_item_cost(ranges[b].y) : 0.f;
+                float to = c;   // cost up to and including sample b
+#pragma unroll 1
+                for (int m = 1; m < 32; m <<= 1) {
+                    const float v = __shfl_up_sync(0xffffffffu, to, m);
+                    if (lane >= m) to += v;
                 }
-                const int row = it.start + it.j * CT_BN;
-                const uint32_t empty_parity = ((n >> 1) & 1) ^ 1;
-                if (!mbar_wait(&sh->k_empty[slot], empty_parity, CT_WAIT_CYCLES)) {
-                    timeout(901);
-                    ok = false;
+                to += before;
+                const uint32_t inside = __ballot_sync(0xffffffffu, b < p.batch && at < to);
+                if (inside) {
+                    const float share = fminf(fmaxf((at - (to - c)) / fmaxf(c, 1.f), 0.f), 1.f);
+                    found = __shfl_sync(0xffffffffu, b * per_batch + static_cast<int>(ceilf(share * static_cast<float>(per_batch))), __ffs(inside) - 1);
                     break;
                 }
-                mbar_arrive_expect_tx(&sh->k_full[slot], halves * CT_KV_HALF);
-                for (int h = 0; h < halves; ++h)
-                    tma_load_4d(k_s + slot * CT_KV_BYTES + h * CT_KV_HALF, &tm_k, &sh->k_full[slot], h * 64, row, kv_head * p.k_hmul,
-                                p.st.kv_offsets ? 0 : it.batch * p.k_bmul);
-                if (!mbar_wait(&sh->v_empty[slot], empty_parity, CT_WAIT_CYCLES)) {
-                    timeout(902);
-                    ++n;
-                    ok = false;
-                    break;
-                }
-                const bool holes = it.holes();
-                uint64_t* full = holes ? &sh->vh_full[slot] : &sh->v_full[slot];
-                v_uses[holes] = (v_uses[holes] ^ (1u << slot)) | (4u << slot);
-                mbar_arrive_expect_tx(full, halves * CT_KV_HALF);
-                for (int h = 0; h < halves; ++h)
-                    tma_load_4d(v_s + slot * CT_KV_BYTES + h * CT_KV_HALF, &tm_v, full, h * 64, row, kv_head * p.v_hmul,
-                                p.st.kv_offsets ? 0 : it.batch * p.v_bmul);
-                ++n;
+                before = __shfl_sync(0xffffffffu, to, 31);
             }
-            if (!ok) {   // leave with no copy of this CTA in flight
-                if (q_uses) mbar_wait(&sh->q_full, (q_uses - 1) & 1, CT_WAIT_CYCLES);
-                for (int s = 0; s < 2; ++s) {
-                    const uint32_t uses = (n + 1 - s) >> 1;   // of K slot s
-                    if (uses) mbar_wait(&sh->k_full[s], (uses - 1) & 1, CT_WAIT_CYCLES);
-                    if (v_uses[0] & (4u << s)) mbar_wait(&sh->v_full[s], ((v_uses[0] >> s) & 1) ^ 1, CT_WAIT_CYCLES);
-                    if (v_uses[1] & (4u << s)) mbar_wait(&sh->vh_full[s], ((v_uses[1] >> s) & 1) ^ 1, CT_WAIT_CYCLES);
-                }
-            }
+            if (e == 0) edge[0] = found;
+            else edge[1] = found;
         }
-    } else if (warp == CT_MMA_WARP) {
-        reg_dealloc<CT_REGS_OTHER>();
+    }
+    const int b_first = edge[0] / per_batch, h_first = (edge[0] - b_first * per_batch) / p.q_tiles, t_first = edge[0] - (b_first * p.heads + h_first) * p.q_tiles;
+    using Items = CrossItems<MASK>;
+#define CT_ITEMS(name) Items name(p, ranges, words, edge[0], edge[1], b_first, h_first, t_first)
+
+    if (warp == CT_MMA_WARP) {
         // ------------------------------------------------------------------ MMA issuer (the whole warp walks the loop, one elected lane issues)
         const int ksteps = (p.dim + 15) >> 4;                    // of 16 channels; channels past the head read as zeros
         const uint32_t idesc_pv = idesc_h16(CT_BM, 0, F16, true) | (static_cast<uint32_t>(ksteps * 2) << 17);
@@ -305,204 +275,150 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const uint64_t vd = smem_desc_sw128_mn(smem_u32(v_s), CT_KV_HALF, 1024);
         const uint32_t hi_k = static_cast<uint32_t>(qd >> 32), hi_v = static_cast<uint32_t>(vd >> 32);
         const uint32_t q_lo = static_cast<uint32_t>(qd), k_lo = static_cast<uint32_t>(kd), v_lo = static_cast<uint32_t>(vd);
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-            if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity, CT_WAIT_CYCLES))) {
-                if (lane == 0) timeout(code);
-                ok = false;
+        // Two walks over the blocks: `s` for Q K^T, up to one block ahead inside an item, and `o` for P V.  (Each product is issued at
+        // one place: the kernel's code has to stay in the instruction caches with five roles at work.)
+        CT_ITEMS(s);
+        CT_ITEMS(o);
+        int sj = 0, oj = 0;
+        uint32_t m = 0, n = 0, s_items = 0, o_items = 0, plain = 0;   // blocks and items so far; plain: phase bit of v_full per slot
+        bool s_there = true;
+        while (true) {
+            if (sj == s.blocks && s_there) {
+                sj = 0;
+                s_there = s.advance();
             }
-            return ok;
-        };
-        CrossWalk<MASK> cur(p, ranges, words);
-        uint32_t n = 0, opened = 0, plain = 0, zeroed = 0;   // n: block of `cur`; opened: items whose Q was waited for; plain / zeroed: phase bit per V slot
-        // S = Q K_j^T of block `w` (number m) over its states, rounded up to 16; `last`: of its item
-        auto issue_qk = [&](int valid, uint32_t m, bool first, bool last) {
-            if (first && !wait(&sh->q_full, opened++ & 1, 910)) return;
-            if (!wait(&sh->k_full[m & 1], (m >> 1) & 1, 911)) return;
-            tc_fence_after_sync();
-            const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((valid + 15) >> 4) << 18);
-            if (elect_one()) {
+            if (oj == o.blocks) {
+                oj = 0;
+                if (!o.advance()) break;
+                ++o_items;
+            }
+            // S = Q K_j^T over the block's states, rounded up to 16: now if no scores are left to work on, ahead of P V if K has landed
+            if (s_there && (m == n || (m == n + 1 && s.item == o.item &&
+                                              __all_sync(0xffffffffu, mbar_test_wait(&sh->k_full[m & 1], (m >> 1) & 1))))) {
+                if (sj == 0 && !ct_wait(&sh->q_full, s_items++ & 1, sh, 910)) break;
+                if (!ct_wait(&sh->k_full[m & 1], (m >> 1) & 1, sh, 911)) break;
+                tc_fence_after_sync();
+                const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((s.valid(sj) + 15) >> 4) << 18);
+                const uint32_t d = tmem + (m & 1) * CT_BN, k0 = k_lo + (m & 1) * (CT_KV_BYTES >> 4);
+                if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk)
-                    if (kk < ksteps)
-                        tc_mma_f16_lo(tmem + (m & 1) * CT_BN, q_lo + (kk >> 2) * (CT_Q_HALF >> 4) + (kk & 3) * 2,
-                                      k_lo + (m & 1) * (CT_KV_BYTES >> 4) + (kk >> 2) * (CT_KV_HALF >> 4) + (kk & 3) * 2, hi_k, idesc, kk > 0);
-                tc_commit(&sh->s_full[m & 1]);
-                tc_commit(&sh->k_empty[m & 1]);
-                if (last) tc_commit(&sh->q_empty);
-            }
-            __syncwarp();
-        };
-        bool more = cur.next(), first = true;
-        uint32_t items_done = 0;
-        bool started = false;
-        while (more && ok) {
-            CrossWalk<MASK> nxt = cur;
-            const bool next_there = nxt.next();
-            const bool same = next_there && nxt.item == cur.item;
-            if (!started) {
-                started = true;
-                issue_qk(cur.valid, n, true, !same);
-                if (!ok) break;
-            }
-            if (same) {   // the scores of the item's next block while this one's exponentials run
-                CrossWalk<MASK> after = nxt;
-                const bool nlast = !after.next_in_item();
-                issue_qk(nxt.valid, n + 1, false, nlast);
-                if (!ok) break;
+                    for (int kk = 0; kk < 8; ++kk)
+                        if (kk < ksteps)
+                            tc_mma_f16_lo(d, q_lo + (kk >> 2) * (CT_Q_HALF >> 4) + (kk & 3) * 2, k0 + (kk >> 2) * (CT_KV_HALF >> 4) + (kk & 3) * 2, hi_k,
+                                          idesc, kk > 0);
+                    tc_commit(&sh->s_full[m & 1]);
+                }
+                __syncwarp();
+                ++m;
+                ++sj;
+                if (m == n + 1) continue;   // look for one more
             }
             const uint32_t slot = n & 1;
-            if (first && items_done > 0 && !wait(&sh->o_free, (items_done - 1) & 1, 915)) break;   // the previous item's O has been read
-            if (cur.holes()) {
-                if (!wait(&sh->v_zeroed[slot], (zeroed >> slot) & 1, 921)) break;
-                zeroed ^= 1u << slot;
-            } else {
-                if (!wait(&sh->v_full[slot], (plain >> slot) & 1, 920)) break;
+            if (oj == 0 && o_items > 1 && !ct_wait(&sh->o_free, o_items & 1, sh, 915)) break;   // the previous item's O has been read
+            if (!o.holes(oj)) {   // otherwise P is only handed over behind it
+                if (!ct_wait(&sh->v_full[slot], (plain >> slot) & 1, sh, 920)) break;
                 plain ^= 1u << slot;
             }
-            if (!wait(&sh->p_full[slot], (n >> 1) & 1, 930)) break;
+            if (!ct_wait(&sh->p_full[slot], (n >> 1) & 1, sh, 930)) break;
             tc_fence_after_sync();
+            const int steps = (o.valid(oj) + 15) >> 4;
+            const uint32_t a = tmem + slot * CT_BN, v0 = v_lo + slot * (CT_KV_BYTES >> 4);
             if (elect_one()) {
-                const int steps = (cur.valid + 15) >> 4;
 #pragma unroll
                 for (int k4 = 0; k4 < 4; ++k4)
-                    if (k4 < steps)
-                        tc_mma_f16_ts_lo(tmem + 2 * CT_BN, tmem + slot * CT_BN + k4 * 8, v_lo + slot * (CT_KV_BYTES >> 4) + k4 * 128, hi_v, idesc_pv,
-                                         (!first || k4 > 0) ? 1u : 0u);
+                    if (k4 < steps) tc_mma_f16_ts_lo(tmem + 2 * CT_BN, a + k4 * 8, v0 + k4 * 128, hi_v, idesc_pv, (oj | k4) ? 1u : 0u);
                 tc_commit(&sh->pv_done[slot]);
-                tc_commit(&sh->v_empty[slot]);
             }
             __syncwarp();
-            first = !same;
-            if (!same) {
-                ++items_done;
-                if (next_there) {
-                    CrossWalk<MASK> after = nxt;
-                    const bool nlast = !after.next_in_item();
-                    issue_qk(nxt.valid, n + 1, true, nlast);
-                }
-            }
             ++n;
-            more = next_there;
-            cur.item = nxt.item; cur.j = nxt.j; cur.valid = nxt.valid; cur.start = nxt.start; cur.count = nxt.count; cur.batch = nxt.batch; cur.rem = nxt.rem;
-            cur.w = nxt.w;
+            ++oj;
         }
-    } else if (warp >= CT_ZERO_WARP) {
-        reg_dealloc<CT_REGS_OTHER>();
-        // ------------------------------------------------------------------ rows of V that must not be seen -> zeros
-        if (warp == CT_ZERO_WARP) {
-            CrossWalk<MASK> it(p, ranges, words);
-            uint32_t n = 0, phase = 0;
-            while (it.next()) {
-                const uint32_t slot = n++ & 1;
-                if (!it.holes()) continue;
-                if (!__all_sync(0xffffffffu, mbar_wait(&sh->vh_full[slot], (phase >> slot) & 1, CT_WAIT_CYCLES))) {
-                    if (lane == 0) timeout(950);
+    } else if (warp == CT_QK_WARP || warp == CT_V_WARP) {
+        // ------------------------------------------------------------------ producers: one warp for Q and K, one for V (the copies of one issuing
+        // warp are worked off one after the other)
+        const bool v_warp = warp == CT_V_WARP;
+        const CUtensorMap* map = v_warp ? &tm_v : &tm_k;
+        uint64_t* free_bar = v_warp ? sh->pv_done : sh->s_full;
+        CT_ITEMS(it);
+        uint32_t n = 0, items = 0;
+        uint32_t used = 0, phase = 0;   // per slot and kind of V block (bit 2 * slot + holes): any copy yet, and the next one's phase bit
+        auto full_of = [&](int slot, int holes) { return (!v_warp ? sh->k_full : holes ? sh->vh_full : sh->v_full) + slot; };
+        bool ok = true;
+        while (ok && it.advance()) {
+            const int kv_head = it.head / p.group;
+            if (!v_warp) {
+                // block n - 1 was the previous item's last
+                if (n > 0 && !ct_wait(&sh->s_full[(n - 1) & 1], ((n - 1) >> 1) & 1, sh, 900)) break;
+                ++items;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sh->q_full, halves * CT_Q_HALF);
+#pragma unroll 1
+                    for (int h = 0; h < halves; ++h)
+                        tma_load_4d(q_s + h * CT_Q_HALF, &tm_q, &sh->q_full, h * 64, it.tile * CT_BM, it.head * p.q_hmul, it.batch * p.q_bmul);
+                }
+                __syncwarp();
+            }
+            const int z = kv_head * (v_warp ? p.v_hmul : p.k_hmul), w = p.st.kv_offsets ? 0 : it.batch * (v_warp ? p.v_bmul : p.k_bmul);
+            for (int j = 0; j < it.blocks; ++j, ++n) {
+                const int slot = n & 1;
+                if (n > 1 && !ct_wait(free_bar + slot, ((n - 2) >> 1) & 1, sh, 901 + v_warp)) {
+                    ok = false;
                     break;
                 }
-                phase ^= 1u << slot;
-                const int up = (it.valid + 15) & ~15;
-                // four rows a turn, eight lanes per row (and half)
-                for (int r0 = MASK ? 0 : it.valid & ~3; r0 < up; r0 += 4) {
-                    const int r = r0 + (lane >> 3);
-                    bool zero = r >= it.valid;
-                    if constexpr (MASK) zero = !((it.w[2 * it.j + (r >> 5)] >> (r & 31)) & 1u);
-                    if (zero && r < up)
-                        for (int h = 0; h < halves; ++h)
-                            *reinterpret_cast<uint4*>(v_s + slot * CT_KV_BYTES + h * CT_KV_HALF + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                const int holes = v_warp && it.holes(j);
+                used |= 1u << (2 * slot + holes);
+                phase ^= 1u << (2 * slot + holes);
+                if (lane == 0) {
+                    uint64_t* full = full_of(slot, holes);
+                    uint8_t* to = (v_warp ? v_s : k_s) + slot * CT_KV_BYTES;
+                    mbar_arrive_expect_tx(full, halves * CT_KV_HALF);
+#pragma unroll 1
+                    for (int h = 0; h < halves; ++h) tma_load_4d(to + h * CT_KV_HALF, map, full, h * 64, it.start + j * CT_BN, z, w);
                 }
-                fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->v_zeroed[slot]);
             }
         }
-    } else {
-        reg_alloc<CT_REGS_SOFTMAX>();
-        // ------------------------------------------------------------------ softmax: thread = one query row
-        const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
-        const uint32_t s_tmem = tmem + lane_addr, o_tmem = s_tmem + 2 * CT_BN;
-        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-        // 32 states -> 16 columns of packed 16-bit pairs, and their sum
-        auto exp32 = [&](const uint32_t (&a)[32], float m, uint32_t (&w)[16]) {
-            const float2 nm2 = make_float2(-m, -m);
-            float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), sc2, nm2);
-                float2 r;
-                if ((i & 3) == 3) {   // a quarter on the FMA pipe, as in attention.cu
-                    r = exp2_fma2(x);
-                } else {
-                    r.x = ex2(x.x);
-                    r.y = ex2(x.y);
-                }
-                sum2[i & 1] = __fadd2_rn(sum2[i & 1], r);
-                w[i] = pack_h16<F16>(r.x, r.y);
+        // leave with none of this warp's copies in flight (where all went well they have all been waited for)
+        if (items) ct_wait(&sh->q_full, (items & 1) ^ 1, sh, 903);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+            if ((used >> i) & 1u) ct_wait(full_of(i >> 1, i & 1), ((phase >> i) & 1u) ^ 1u, sh, 904);
+    } else if (warp >= 4 && warp < 8) {
+        // ------------------------------------------------------------------ output: O / l -> global memory, while the softmax warps are at the
+        // next item already
+        const int quad = warp & 3;
+        const uint32_t o_tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 2 * CT_BN;
+        uint8_t* box = stage + quad * (CT_STAGE_BYTES / 4);   // [32 rows][64 bytes], 16-byte pieces swizzled by row / 2
+        CT_ITEMS(it);
+        uint32_t n = 0, done = 0;   // blocks and items with states so far
+        while (it.template advance<true>()) {
+            n += it.blocks;
+            const int row0 = it.tile * CT_BM + quad * 32;
+            uint8_t* out = p.out + it.batch * p.os[0] + it.head * p.os[1] + row0 * p.os[2];
+            float inv = 0.f;
+            if (it.blocks) {
+                const uint32_t last = n - 1;
+                if (!ct_wait(&sh->l_full[done & 1], (done >> 1) & 1, sh, 980) || !ct_wait(&sh->pv_done[last & 1], (last >> 1) & 1, sh, 981)) break;
+                inv = 1.f / sums[(done & 1) * CT_BM + quad * 32 + lane];
+                ++done;
+                tc_fence_after_sync();
             }
-            return (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-        };
-        auto max32 = [&](const uint32_t (&a)[32]) {
-            float m0 = __uint_as_float(a[0]), m1 = __uint_as_float(a[1]);
-#pragma unroll
-            for (int i = 2; i < 32; i += 4) {
-                m0 = max3(m0, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
-                if (i + 2 < 32) m1 = max3(m1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
-            }
-            return fmaxf(m0, m1);
-        };
-        CrossWalk<MASK> it(p, ranges, words);
-        // scores that do not count -> -inf (selected, not added: they may be anything)
-        auto hide = [&](uint32_t (&a)[32], int chunk) {
-            if constexpr (MASK) {
-                const uint32_t bits = it.w[2 * it.j + chunk];
-                if (bits != 0xffffffffu) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (!((bits >> i) & 1u)) a[i] = 0xff800000u;
-                }
-            } else if (it.valid < (chunk + 1) * 32) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (chunk * 32 + i >= it.valid) a[i] = 0xff800000u;
-            }
-        };
-        // samples without states: zeros
-        {
-            CrossWalk<MASK> e(p, ranges, words);
-            if (e.item < p.items) do {
-                if (e.next_in_item()) continue;
-                const int qrow = e.q0() + warp * 32 + lane;
-                uint8_t* dst = p.out + e.batch * p.os[0] + e.head() * p.os[1] + qrow * p.os[2];
-                if (qrow < p.q_len)
-                    for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(dst + 2 * c) = make_uint4(0, 0, 0, 0);
-            } while (e.next_item());
-        }
-        uint32_t n = 0;
-        bool ok = true;
-        float m_used = 0.f, l = 0.f;
-        int item = -1, q0 = 0;                 // item in work
-        uint8_t* out = nullptr;                // its rows
-        // O / l of the item in work -> global memory; its last block is number n - 1
-        auto finish = [&]() {
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, CT_WAIT_CYCLES))) {
-                if (lane == 0) timeout(980);
-                return false;
-            }
-            tc_fence_after_sync();
-            const float inv = 1.f / l;
-            uint8_t* box = stage + warp * (CT_STAGE_BYTES / 4);   // [32 rows][64 bytes], 16-byte pieces swizzled by row / 2
 #pragma unroll 1
             for (int c = 0; c < p.dim; c += 32) {
                 uint32_t o[32];
-                tc_ld_32x32b_x32(o_tmem + c, o);
-                tc_wait_ld();
-                if (c + 32 >= p.dim) {   // all of O has been read: the next item's P V may overwrite it
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh->o_free);
+                if (it.blocks) {
+                    tc_ld_32x32b_x32(o_tmem + c, o);   // columns past the head hold anything and are not stored
+                    tc_wait_ld();
+                    if (c + 32 >= p.dim) {   // all of O has been read: the next item's P V may overwrite it
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh->o_free);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0u;   // no states: zeros
                 }
-                // through shared memory, so that a store instruction covers eight rows' 64 bytes and not 32 rows' 16 (one line of L1 a cycle:
-                // 3900 cycles per item the other way, a quarter of its time)
+                // through shared memory, so that a store instruction covers eight rows' 64 bytes and not 32 rows' 16 (L1 takes one line a cycle)
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     uint32_t w4[4];
@@ -516,86 +432,129 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 for (int u = 0; u < 4; ++u) {
                     const int r = u * 8 + (lane >> 2), piece = lane & 3;
                     const uint4 v = *reinterpret_cast<const uint4*>(box + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-                    const int qrow = q0 + warp * 32 + r;
-                    if (qrow < p.q_len && c + piece * 8 < p.dim) *reinterpret_cast<uint4*>(out + qrow * p.os[2] + 2 * (c + piece * 8)) = v;
+                    if (row0 + r < p.q_len && c + piece * 8 < p.dim) *reinterpret_cast<uint4*>(out + r * p.os[2] + 2 * (c + piece * 8)) = v;
                 }
                 __syncwarp();
             }
-            return true;
-        };
-        while (it.next()) {
-            const uint32_t slot = n & 1;
-            const bool first = it.item != item;
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh->s_full[slot], (n >> 1) & 1, CT_WAIT_CYCLES))) {
-                if (lane == 0) timeout(960);
-                ok = false;
-                break;
-            }
-            tc_fence_after_sync();
-            const bool two = it.valid > 32;
-            const uint32_t st = s_tmem + slot * CT_BN;
-            uint32_t s0[32], s1[32], w0[16], w1[16];
-            tc_ld_32x32b_x32(st, s0);
-            if (two) tc_ld_32x32b_x32(st + 32, s1);
-            tc_wait_ld();
-            hide(s0, 0);
-            float mx = max32(s0);
-            if (two) {
-                hide(s1, 1);
-                mx = fmaxf(mx, max32(s1));
-            }
-            const float ms = mx * p.scale_log2;
-            const bool grow = first || ms > m_used + CT_RESCALE_STEP;
-            if (!first && __any_sync(0xffffffffu, grow)) {
-                // O is written by the previous P V product until it has completed
-                if (!__all_sync(0xffffffffu, mbar_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, CT_WAIT_CYCLES))) {
-                    if (lane == 0) timeout(970);
-                    ok = false;
-                    break;
-                }
-                tc_fence_after_sync();
-                const float alpha = grow ? ex2(m_used - ms) : 1.f;
-                l *= alpha;
+        }
+    } else if (warp < 4) {
+        // ------------------------------------------------------------------ softmax: thread = one query row
+        const uint32_t s_tmem = tmem + (static_cast<uint32_t>(warp * 32) << 16), o_tmem = s_tmem + 2 * CT_BN;
+        CT_ITEMS(it);
+        uint32_t n = 0, done = 0, hole_phase = 0;   // blocks, items with states; hole_phase: phase bit of vh_full per slot
+        bool ok = true;
+        while (ok && it.advance()) {
+            float m_used = 0.f, l = 0.f;
 #pragma unroll 1
-                for (int c = 0; c < p.dim; c += 16) {
-                    uint32_t o[16];
-                    tc_ld_32x32b_x16(o_tmem + c, o);
+            for (int j = 0; j < it.blocks; ++j, ++n) {
+                const uint32_t slot = n & 1, st = s_tmem + slot * CT_BN;
+                const int valid = it.valid(j);
+                if (!(ok = ct_wait(&sh->s_full[slot], (n >> 1) & 1, sh, 960))) break;
+                tc_fence_after_sync();
+                // Two passes over the scores in tensor memory, 32 at a time: the maximum, then the exponentials.  Scores that do not count are
+                // replaced by -inf (selected, not added: they may be anything).
+                float mx = __int_as_float(0xff800000);
+#pragma unroll 1
+                for (int c = 0; c < valid; c += 32) {
+                    uint32_t a[32];
+                    tc_ld_32x32b_x32(st + c, a);
+                    const uint32_t bits = MASK ? it.bits(j)[c >> 5] : valid - c >= 32 ? 0xffffffffu : (1u << (valid - c)) - 1u;
+                    tc_wait_ld();
+                    if (bits != 0xffffffffu) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!((bits >> i) & 1u)) a[i] = 0xff800000u;
+                        tc_st_32x32b_x32(st + c, a);
+                        tc_wait_st();
+                    }
+                    float m1 = __uint_as_float(a[0]);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        mx = max3(mx, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
+                        m1 = max3(m1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
+                    }
+                    mx = fmaxf(mx, m1);
+                }
+                // (a block of which nothing is to be seen, ahead of others: its exponentials are of -inf whatever the finite maximum is)
+                const float ms = MASK ? fmaxf(mx * p.scale_log2, -1e30f) : mx * p.scale_log2;
+                const bool grow = j == 0 || ms > m_used + CT_RESCALE_STEP;
+                if (j > 0 && __any_sync(0xffffffffu, grow)) {
+                    // O is written by the previous P V product until it has completed
+                    if (!(ok = ct_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, sh, 970))) break;
+                    tc_fence_after_sync();
+                    const float alpha = grow ? ex2(m_used - ms) : 1.f;
+                    l *= alpha;
+#pragma unroll 1
+                    for (int c = 0; c < p.dim; c += 16) {
+                        uint32_t o[16];
+                        tc_ld_32x32b_x16(o_tmem + c, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tc_st_32x32b_x16(o_tmem + c, o);
+                    }
+                    tc_wait_st();
+                }
+                if (grow) m_used = ms;
+                const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m_used, -m_used);
+                float2 sum2 = make_float2(0.f, 0.f);
+#pragma unroll 1
+                for (int c = 0; c < valid; c += 32) {
+                    uint32_t a[32], w[16];
+                    tc_ld_32x32b_x32(st + c, a);
                     tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                    tc_st_32x32b_x16(o_tmem + c, o);
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), sc2, nm2);
+                        float2 r;
+                        if ((i & 3) == 3) {   // a quarter on the FMA pipe, as in attention.cu
+                            r = exp2_fma2(x);
+                        } else {
+                            r.x = ex2(x.x);
+                            r.y = ex2(x.y);
+                        }
+                        sum2 = __fadd2_rn(sum2, r);
+                        w[i] = pack_h16<F16>(r.x, r.y);
+                    }
+                    // P over scores of this thread that are in registers by now
+                    tc_st_32x32b_x16(st + (c >> 1), w);
+                }
+                l += sum2.x + sum2.y;
+                if (it.holes(j)) {   // rows of V that must not be seen -> zeros: four rows per warp and turn, eight lanes per row (and half)
+                    if (!(ok = ct_wait(&sh->vh_full[slot], (hole_phase >> slot) & 1, sh, 950))) break;
+                    hole_phase ^= 1u << slot;
+                    const int up = (valid + 15) & ~15;
+#pragma unroll 1
+                    for (int r = (MASK ? 0 : valid & ~15) + warp * 4 + (lane >> 3); r < up; r += 16) {
+                        bool zero = r >= valid;
+                        if constexpr (MASK) zero = !((it.bits(j)[r >> 5] >> (r & 31)) & 1u);
+                        if (zero)
+                            for (int h = 0; h < halves; ++h)
+                                *reinterpret_cast<uint4*>(v_s + slot * CT_KV_BYTES + h * CT_KV_HALF + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
                 }
                 tc_wait_st();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->p_full[slot]);
             }
-            const float m = grow ? ms : m_used;
-            float sum = exp32(s0, m, w0);
-            if (two) sum += exp32(s1, m, w1);
-            if (first) {
-                // the previous item's O, behind this item's first exponentials: its last P V runs under them
-                if (item >= 0 && !finish()) {
-                    ok = false;
-                    break;
-                }
-                item = it.item;
-                q0 = it.q0();
-                out = p.out + it.batch * p.os[0] + it.head() * p.os[1];
-                l = 0.f;
-            }
-            m_used = m;
-            l += sum;
-            // P over this thread's own S values, which are all in registers by now
-            tc_st_32x32b_x16(st, w0);
-            if (two) tc_st_32x32b_x16(st + 16, w1);
-            tc_wait_st();
-            tc_fence_before_sync();
+            if (!ok) break;
+            // Two buffers (and barriers) in turn: an item's P V waits until the output warps have read the previous item's O and sums, and
+            // the scores of the item after it come behind that P V; so the buffer written here was read two items ago.
+            sums[(done & 1) * CT_BM + warp * 32 + lane] = l;
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->p_full[slot]);
-            ++n;
+            if (lane == 0) mbar_arrive(&sh->l_full[done & 1]);
+            ++done;
         }
-        if (ok && item >= 0) finish();
     }
+#undef CT_ITEMS
     tc_fence_before_sync();
     __syncthreads();
+    if (tid == 0 && sh->failed) {
+        atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
+        atomicExch(&p.status[1], sh->failed);
+    }
     if (warp == CT_MMA_WARP) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, CT_TMEM_COLS);
@@ -1002,40 +961,45 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         while (split < CR_MAX_SPLIT && ctas * split < 2ll * sms && 2 * split <= tiles) split *= 2;
         return f16 ? launch_cross_rows_dim<true>(p, static_cast<int>(kv_pairs), split, st) : launch_cross_rows_dim<false>(p, static_cast<int>(kv_pairs), split, st);
     }
-    CrossTileParams p = {};
-    p.st = states;
-    p.q_len = a->q_len;
-    p.dim = a->head_dim;
-    p.group = group;
-    p.scale_log2 = scale_log2;
-    if (int rc = status_words(&p.status)) return rc;
+    // The kernel keeps its samples' ranges and mask bits in shared memory: launches of as many samples as fit (hundreds, without a mask).
     const int q_tiles = (a->q_len + CT_BM - 1) / CT_BM;
-    const long long items = static_cast<long long>(a->batch) * a->heads * q_tiles;
-    SVDQ_CHECK_ARG(items < (1ll << 30), "cross_attention: too many query tiles");
-    p.out = static_cast<uint8_t*>(a->out);
-    for (int i = 0; i < 3; ++i) p.os[i] = 2 * a->o_stride[i];
-    p.heads = a->heads;
-    p.q_tiles = q_tiles;
-    p.items = static_cast<int>(items);
-    p.batch = a->batch;
-    p.per_batch = a->heads * q_tiles;
-    CUtensorMap mq, mk, mv;
-    if (int rc = cross_tmap(&mq, tq, a->head_dim, a->dtype, CT_BM, &p.q_bmul, &p.q_hmul)) return rc;
-    if (int rc = cross_tmap(&mk, tk, a->head_dim, a->dtype, CT_BN, &p.k_bmul, &p.k_hmul)) return rc;
-    if (int rc = cross_tmap(&mv, tv, a->head_dim, a->dtype, CT_BN, &p.v_bmul, &p.v_hmul)) return rc;
-    // two CTAs per SM that work through the items; without room for every sample's mask bits, one CTA per item with its sample's
-    const int resident = p.items < 2 * sms ? p.items : 2 * sms;
-    if (a->mask) {
-        p.mask_words = (a->kv_len + CT_BN - 1) / CT_BN * (CT_BN / 32);
-        p.table = static_cast<long long>(p.mask_words) * a->batch * 4 <= CT_TABLE_BYTES;
-        const int bytes = p.mask_words * 4 * (p.table ? a->batch : 1), grid = p.table ? resident : p.items;
-        p.step_batch = grid / p.per_batch;
-        p.step_rem = grid % p.per_batch;
-        return f16 ? launch_cross_tile<true, true>(mq, mk, mv, p, grid, bytes, st) : launch_cross_tile<false, true>(mq, mk, mv, p, grid, bytes, st);
+    const int mask_words = a->mask ? (a->kv_len + CT_BN - 1) / CT_BN * (CT_BN / 32) : 0;
+    const int most = CT_TABLE_BYTES / (8 + 4 * mask_words);
+    SVDQ_CHECK_ARG(static_cast<long long>(a->heads) * q_tiles * (a->batch < most ? a->batch : most) < (1ll << 30), "cross_attention: too many query tiles");
+    for (int b0 = 0; b0 < a->batch; b0 += most) {
+        const int nb = a->batch - b0 < most ? a->batch - b0 : most;
+        auto from = [&](CrossTensor t, int count) {
+            if (count) {
+                t.base = static_cast<const uint8_t*>(t.base) + 2 * b0 * t.stride[0];
+                t.batch = nb;
+            }
+            return t;
+        };
+        CrossTileParams p = {};
+        p.st = states;
+        if (p.st.kv_lens) p.st.kv_lens += b0;
+        if (p.st.kv_offsets) p.st.kv_offsets += b0;
+        if (p.st.mask) p.st.mask += b0 * p.st.mask_stride;
+        p.q_len = a->q_len;
+        p.dim = a->head_dim;
+        p.group = group;
+        p.scale_log2 = scale_log2;
+        if (int rc = status_words(&p.status)) return rc;
+        p.out = static_cast<uint8_t*>(a->out) + 2 * b0 * a->o_stride[0];
+        for (int i = 0; i < 3; ++i) p.os[i] = 2 * a->o_stride[i];
+        p.heads = a->heads;
+        p.q_tiles = q_tiles;
+        p.batch = nb;
+        p.items = nb * a->heads * q_tiles;
+        p.mask_words = mask_words;
+        CUtensorMap mq, mk, mv;
+        if (int rc = cross_tmap(&mq, from(tq, 1), a->head_dim, a->dtype, CT_BM, &p.q_bmul, &p.q_hmul)) return rc;
+        if (int rc = cross_tmap(&mk, from(tk, !a->kv_offsets), a->head_dim, a->dtype, CT_BN, &p.k_bmul, &p.k_hmul)) return rc;
+        if (int rc = cross_tmap(&mv, from(tv, !a->kv_offsets), a->head_dim, a->dtype, CT_BN, &p.v_bmul, &p.v_hmul)) return rc;
+        const int grid = p.items < 2 * sms ? p.items : 2 * sms, bytes = nb * (8 + 4 * mask_words);   // two CTAs per SM work through the items
+        const int rc = a->mask ? (f16 ? launch_cross_tile<true, true>(mq, mk, mv, p, grid, bytes, st) : launch_cross_tile<false, true>(mq, mk, mv, p, grid, bytes, st))
+                               : (f16 ? launch_cross_tile<true, false>(mq, mk, mv, p, grid, bytes, st) : launch_cross_tile<false, false>(mq, mk, mv, p, grid, bytes, st));
+        if (rc) return rc;
     }
-    p.table = a->batch <= CT_RANGES;
-    p.step_batch = resident / p.per_batch;
-    p.step_rem = resident % p.per_batch;
-    const int bytes = p.table ? a->batch * 8 : 0;
-    return f16 ? launch_cross_tile<true, false>(mq, mk, mv, p, resident, bytes, st) : launch_cross_tile<false, false>(mq, mk, mv, p, resident, bytes, st);
+    return SVDQ_OK;
 }
