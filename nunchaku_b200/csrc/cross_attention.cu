@@ -61,6 +61,9 @@ constexpr int CT_Q_BYTES = 2 * CT_Q_HALF, CT_KV_BYTES = 2 * CT_KV_HALF;
 constexpr int CT_SLOTS = 2;                         // of K and of V each
 constexpr int CT_THREADS = 12 * 32;
 constexpr int CT_MMA_WARP = 8, CT_QK_WARP = 9, CT_V_WARP = 10;   // 0-3 softmax, 4-7 output, 11 nothing
+// registers move inside the pool the CTA was launched with (384 threads x 80: two CTAs fill the file)
+constexpr int CT_REGS_SOFTMAX = 112, CT_REGS_OUTPUT = 64, CT_REGS_OTHER = 64;
+static_assert(CT_REGS_SOFTMAX + CT_REGS_OUTPUT + CT_REGS_OTHER <= 3 * 80, "register budget");
 constexpr int CT_MASK_STATES = 32768;               // longest state list a mask may cover (its bits are kept in shared memory)
 constexpr int CT_STAGE_BYTES = 4 * 32 * 64;         // output: 32 rows x 32 channels per output warp on their way to memory
 constexpr int CT_BAR_BYTES = 256;
@@ -87,7 +90,7 @@ struct CrossTileParams {
     CrossStates st;
     uint8_t* out;
     long long os[3];                                      // batch, head, token strides in bytes
-    int q_len, dim, group, heads, q_tiles, items, batch;  // item = (batch * heads + head) * q_tiles + tile
+    int q_len, dim, group, heads, q_tiles, items, batch;  // item = (batch * q_tiles + tile) * heads + head
     int mask_words;                                       // 32-bit words of mask bits per sample
     int q_bmul, q_hmul, k_bmul, k_hmul, v_bmul, v_hmul;   // 0 where that dimension is broadcast (stride 0): its coordinate is then 0
     float scale_log2;
@@ -122,17 +125,17 @@ struct CrossItems {
     int item, end, batch, head, tile, start, count, blocks;   // end: behind this CTA's last item
 
     __device__ __forceinline__ CrossItems(const CrossTileParams& p_, const int2* r, const uint32_t* w, int first, int end_, int batch_, int head_, int tile_)
-        : p(p_), ranges(r), words(w), item(first - 1), end(end_), batch(batch_), head(head_), tile(tile_ - 1), start(0), count(0), blocks(0) {}
+        : p(p_), ranges(r), words(w), item(first - 1), end(end_), batch(batch_), head(head_ - 1), tile(tile_), start(0), count(0), blocks(0) {}
     // to the next item (EMPTY: even if it has no states); false behind the last
     template <bool EMPTY = false>
     __device__ __forceinline__ bool advance() {
 #pragma unroll 1
         do {
             if (++item >= end) return false;
-            if (++tile == p.q_tiles) {
-                tile = 0;
-                if (++head == p.heads) {
-                    head = 0;
+            if (++head == p.heads) {   // heads first: their channels lie next to each other in token-major rows
+                head = 0;
+                if (++tile == p.q_tiles) {
+                    tile = 0;
                     ++batch;
                 }
             }
@@ -263,10 +266,12 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             else edge[1] = found;
         }
     }
-    const int b_first = edge[0] / per_batch, h_first = (edge[0] - b_first * per_batch) / p.q_tiles, t_first = edge[0] - (b_first * p.heads + h_first) * p.q_tiles;
+    const int b_first = edge[0] / per_batch, t_first = (edge[0] - b_first * per_batch) / p.heads, h_first = edge[0] - (b_first * p.q_tiles + t_first) * p.heads;
     using Items = CrossItems<MASK>;
 #define CT_ITEMS(name) Items name(p, ranges, words, edge[0], edge[1], b_first, h_first, t_first)
 
+    if (warp >= 8) {
+    reg_dealloc<CT_REGS_OTHER>();
     if (warp == CT_MMA_WARP) {
         // ------------------------------------------------------------------ MMA issuer (the whole warp walks the loop, one elected lane issues)
         const int ksteps = (p.dim + 15) >> 4;                    // of 16 channels; channels past the head read as zeros
@@ -383,7 +388,9 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll 1
         for (int i = 0; i < 4; ++i)
             if ((used >> i) & 1u) ct_wait(full_of(i >> 1, i & 1), ((phase >> i) & 1u) ^ 1u, sh, 904);
-    } else if (warp >= 4 && warp < 8) {
+    }
+    } else if (warp >= 4) {
+        reg_dealloc<CT_REGS_OUTPUT>();
         // ------------------------------------------------------------------ output: O / l -> global memory, while the softmax warps are at the
         // next item already
         const int quad = warp & 3;
@@ -437,9 +444,46 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 __syncwarp();
             }
         }
-    } else if (warp < 4) {
+    } else {
+        reg_alloc<CT_REGS_SOFTMAX>();
         // ------------------------------------------------------------------ softmax: thread = one query row
         const uint32_t s_tmem = tmem + (static_cast<uint32_t>(warp * 32) << 16), o_tmem = s_tmem + 2 * CT_BN;
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+        // 32 states -> 16 columns of packed 16-bit pairs, and their sum
+        auto exp32 = [&](const uint32_t (&a)[32], float m, uint32_t (&w)[16]) {
+            const float2 nm2 = make_float2(-m, -m);
+            float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), sc2, nm2);
+                float2 r;
+                if ((i & 3) == 3) {   // a quarter on the FMA pipe, as in attention.cu
+                    r = exp2_fma2(x);
+                } else {
+                    r.x = ex2(x.x);
+                    r.y = ex2(x.y);
+                }
+                sum2[i & 1] = __fadd2_rn(sum2[i & 1], r);
+                w[i] = pack_h16<F16>(r.x, r.y);
+            }
+            return (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+        };
+        auto max32 = [&](const uint32_t (&a)[32]) {
+            float m0 = __uint_as_float(a[0]), m1 = __uint_as_float(a[1]);
+#pragma unroll
+            for (int i = 2; i < 30; i += 4) {
+                m0 = max3(m0, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
+                m1 = max3(m1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
+            }
+            return max3(m0, m1, fmaxf(__uint_as_float(a[30]), __uint_as_float(a[31])));
+        };
+        auto hide = [&](uint32_t (&a)[32], uint32_t bits) {
+            if (bits != 0xffffffffu) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (!((bits >> i) & 1u)) a[i] = 0xff800000u;
+            }
+        };
         CT_ITEMS(it);
         uint32_t n = 0, done = 0, hole_phase = 0;   // blocks, items with states; hole_phase: phase bit of vh_full per slot
         bool ok = true;
@@ -451,29 +495,17 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 const int valid = it.valid(j);
                 if (!(ok = ct_wait(&sh->s_full[slot], (n >> 1) & 1, sh, 960))) break;
                 tc_fence_after_sync();
-                // Two passes over the scores in tensor memory, 32 at a time: the maximum, then the exponentials.  Scores that do not count are
-                // replaced by -inf (selected, not added: they may be anything).
-                float mx = __int_as_float(0xff800000);
-#pragma unroll 1
-                for (int c = 0; c < valid; c += 32) {
-                    uint32_t a[32];
-                    tc_ld_32x32b_x32(st + c, a);
-                    const uint32_t bits = MASK ? it.bits(j)[c >> 5] : valid - c >= 32 ? 0xffffffffu : (1u << (valid - c)) - 1u;
-                    tc_wait_ld();
-                    if (bits != 0xffffffffu) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!((bits >> i) & 1u)) a[i] = 0xff800000u;
-                        tc_st_32x32b_x32(st + c, a);
-                        tc_wait_st();
-                    }
-                    float m1 = __uint_as_float(a[0]);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        mx = max3(mx, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
-                        m1 = max3(m1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
-                    }
-                    mx = fmaxf(mx, m1);
+                // Scores that do not count are replaced by -inf (selected, not added: they may be anything).
+                uint32_t a0[32], a1[32], w[16];
+                const bool two = valid > 32;
+                tc_ld_32x32b_x32(st, a0);
+                if (two) tc_ld_32x32b_x32(st + 32, a1);
+                tc_wait_ld();
+                hide(a0, MASK ? it.bits(j)[0] : valid >= 32 ? 0xffffffffu : (1u << valid) - 1u);
+                float mx = max32(a0);
+                if (two) {
+                    hide(a1, MASK ? it.bits(j)[1] : valid >= 64 ? 0xffffffffu : (1u << (valid - 32)) - 1u);
+                    mx = fmaxf(mx, max32(a1));
                 }
                 // (a block of which nothing is to be seen, ahead of others: its exponentials are of -inf whatever the finite maximum is)
                 const float ms = MASK ? fmaxf(mx * p.scale_log2, -1e30f) : mx * p.scale_log2;
@@ -496,30 +528,13 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     tc_wait_st();
                 }
                 if (grow) m_used = ms;
-                const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m_used, -m_used);
-                float2 sum2 = make_float2(0.f, 0.f);
-#pragma unroll 1
-                for (int c = 0; c < valid; c += 32) {
-                    uint32_t a[32], w[16];
-                    tc_ld_32x32b_x32(st + c, a);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), sc2, nm2);
-                        float2 r;
-                        if ((i & 3) == 3) {   // a quarter on the FMA pipe, as in attention.cu
-                            r = exp2_fma2(x);
-                        } else {
-                            r.x = ex2(x.x);
-                            r.y = ex2(x.y);
-                        }
-                        sum2 = __fadd2_rn(sum2, r);
-                        w[i] = pack_h16<F16>(r.x, r.y);
-                    }
-                    // P over scores of this thread that are in registers by now
-                    tc_st_32x32b_x16(st + (c >> 1), w);
+                // P over scores of this thread that are in registers by now
+                l += exp32(a0, m_used, w);
+                tc_st_32x32b_x16(st, w);
+                if (two) {
+                    l += exp32(a1, m_used, w);
+                    tc_st_32x32b_x16(st + 16, w);
                 }
-                l += sum2.x + sum2.y;
                 if (it.holes(j)) {   // rows of V that must not be seen -> zeros: four rows per warp and turn, eight lanes per row (and half)
                     if (!(ok = ct_wait(&sh->vh_full[slot], (hole_phase >> slot) & 1, sh, 950))) break;
                     hole_phase ^= 1u << slot;
