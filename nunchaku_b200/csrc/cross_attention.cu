@@ -73,6 +73,9 @@ constexpr int CT_TABLE_BYTES = 6 * 1024;            // the samples' ranges or ma
 constexpr int CT_TMEM_COLS = 256;                   // S: 2 x 64, O: 128
 constexpr int CT_WAIT_LOOKS = 1 << 20;              // each of up to a microsecond
 constexpr float CT_RESCALE_STEP = 8.f;
+#ifndef CT_ITEM_COST
+#define CT_ITEM_COST 16
+#endif
 static_assert(2 * (CT_SMEM + CT_TABLE_BYTES + 1024) <= 228 * 1024 && CT_TABLE_BYTES >= CT_MASK_STATES / 8 + 8, "two CTAs per SM");
 
 struct CrossTileShared {
@@ -160,7 +163,7 @@ struct CrossItems {
 };
 
 // What an item costs, in tenths of a block of 64 states: its blocks, and what it takes to change queries and hand the output over.
-__device__ __forceinline__ float cross_item_cost(int count) { return static_cast<float>(10 * ((count + CT_BN - 1) / CT_BN) + 8); }
+__device__ __forceinline__ float cross_item_cost(int count) { return static_cast<float>(10 * ((count + CT_BN - 1) / CT_BN) + CT_ITEM_COST); }
 
 template <bool F16, bool MASK>
 __global__ void __launch_bounds__(CT_THREADS, 2)
@@ -431,7 +434,10 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     uint32_t w4[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        w4[e] = pack_h16<F16>(__uint_as_float(o[u * 8 + 2 * e]) * inv, __uint_as_float(o[u * 8 + 2 * e + 1]) * inv);
+                    {
+                        const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[u * 8 + 2 * e]), __uint_as_float(o[u * 8 + 2 * e + 1])), make_float2(inv, inv));
+                        w4[e] = pack_h16<F16>(v.x, v.y);
+                    }
                     *reinterpret_cast<uint4*>(box + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
                 }
                 __syncwarp();
@@ -509,8 +515,9 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 }
                 // (a block of which nothing is to be seen, ahead of others: its exponentials are of -inf whatever the finite maximum is)
                 const float ms = MASK ? fmaxf(mx * p.scale_log2, -1e30f) : mx * p.scale_log2;
-                const bool grow = j == 0 || ms > m_used + CT_RESCALE_STEP;
-                if (j > 0 && __any_sync(0xffffffffu, grow)) {
+                if (j == 0) {
+                    m_used = ms;
+                } else if (const bool grow = ms > m_used + CT_RESCALE_STEP; __any_sync(0xffffffffu, grow)) {
                     // O is written by the previous P V product until it has completed
                     if (!(ok = ct_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, sh, 970))) break;
                     tc_fence_after_sync();
@@ -525,9 +532,8 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
                         tc_st_32x32b_x16(o_tmem + c, o);
                     }
-                    tc_wait_st();
+                    if (grow) m_used = ms;
                 }
-                if (grow) m_used = ms;
                 // P over scores of this thread that are in registers by now
                 l += exp32(a0, m_used, w);
                 tc_st_32x32b_x16(st, w);
