@@ -242,10 +242,8 @@ class CrossAttentionArgs(Structure):
         ("k", c_void_p),
         ("v", c_void_p),
         ("out", c_void_p),
-        ("q_stride", ctypes.c_int64 * 3),
-        ("k_stride", ctypes.c_int64 * 3),
-        ("v_stride", ctypes.c_int64 * 3),
-        ("o_stride", ctypes.c_int64 * 3),
+        # q_stride[3] and so on, element by element: twelve integers cost a quarter of four ctypes arrays
+        *((f"{t}_stride{i}", ctypes.c_int64) for t in "qkvo" for i in range(3)),
         ("kv_lens", c_void_p),
         ("kv_offsets", c_void_p),
         ("mask", c_void_p),

@@ -301,10 +301,10 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 ++o_items;
             }
             // S = Q K_j^T over the block's states, rounded up to 16: now if no scores are left to work on, ahead of P V if K has landed
-            if (s_there && (m == n || (m == n + 1 && s.item == o.item &&
-                                              __all_sync(0xffffffffu, mbar_test_wait(&sh->k_full[m & 1], (m >> 1) & 1))))) {
+            const bool landed = s_there && m == n + 1 && s.item == o.item && __all_sync(0xffffffffu, mbar_test_wait(&sh->k_full[m & 1], (m >> 1) & 1));
+            if (landed || (s_there && m == n)) {
                 if (sj == 0 && !ct_wait(&sh->q_full, s_items++ & 1, sh, 910)) break;
-                if (!ct_wait(&sh->k_full[m & 1], (m >> 1) & 1, sh, 911)) break;
+                if (!landed && !ct_wait(&sh->k_full[m & 1], (m >> 1) & 1, sh, 911)) break;
                 tc_fence_after_sync();
                 const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((s.valid(sj) + 15) >> 4) << 18);
                 const uint32_t d = tmem + (m & 1) * CT_BN, k0 = k_lo + (m & 1) * (CT_KV_BYTES >> 4);

@@ -10,7 +10,7 @@ import ctypes
 import torch
 
 from .. import _lib
-from ..utils import HALF_DTYPES, dtype_code, on_device, stream_ptr
+from ..utils import HALF_DTYPES, dtype_code, launch, on_device, stream_ptr
 
 HEAD_DIM = 128
 
@@ -95,7 +95,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
         if k.dim() != 3 or k.shape[2] != D:
             raise ValueError("with kv_offsets, k and v are packed [total, kv_heads, D]")
         T, Hk = k.shape[0], k.shape[1]
-        ks, vs = (0, k.stride(1), k.stride(0)), (0, v.stride(1), v.stride(0))
+        kst, vst = k.stride(), v.stride()
+        ks, vs = (0, kst[1], kst[0]), (0, vst[1], vst[0])
         if kv_offsets.dtype != torch.int32 or kv_offsets.device != dev or kv_offsets.shape != (B + 1,) or not kv_offsets.is_contiguous():
             raise ValueError("kv_offsets must be a contiguous int32 [batch + 1] on q's device")
         off_ptr = kv_offsets.data_ptr()
@@ -103,7 +104,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
         if k.dim() != 4 or k.shape[0] != B or k.shape[3] != D:
             raise ValueError("k and v must be [batch, kv_heads, tokens, D] with q's batch and D")
         Hk, T = k.shape[1], k.shape[2]
-        ks, vs = k.stride()[:3], v.stride()[:3]
+        kst, vst = k.stride(), v.stride()
+        ks, vs = kst[:3], vst[:3]
         if kv_lens is not None:
             if kv_lens.dtype != torch.int32 or kv_lens.device != dev or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
                 raise ValueError("kv_lens must be a contiguous int32 [batch] on q's device")
@@ -112,14 +114,16 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
             if mask.dtype != torch.bool or mask.device != dev or mask.shape != (B, T) or (mask.stride(1) != 1 and T > 1):
                 raise ValueError("mask must be bool [batch, tokens] on q's device with unit token stride")
             mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0)
-    if q.stride(3) != 1 or k.stride(-1) != 1 or v.stride(-1) != 1:
+    qs = q.stride()
+    if qs[3] != 1 or kst[-1] != 1 or vst[-1] != 1:
         raise ValueError("the last dimension of q, k and v must be contiguous")
     if min(B, H, Tq, D, Hk, T) == 0:
         raise ValueError("cross_attention: empty tensors (where no sample has states, k and v still need one row, of any content)")
     ret = out
     if out is None:
-        ret = torch.empty((B, Tq, H * D), dtype=dtype, device=dev)
-        os = (Tq * H * D, D, H * D)
+        C = H * D
+        ret = torch.empty_strided((B, Tq, C), (Tq * C, C, 1), dtype=dtype, device=dev)
+        os = (Tq * C, D, C)
     else:
         if out.dtype != dtype or out.device != dev:
             raise ValueError("out must have q's dtype and device")
@@ -131,10 +135,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
             if out.shape != q.shape or out.stride(3) != 1:
                 raise ValueError("out must be [batch, tokens_q, heads*D] or [batch, heads, tokens_q, D]")
             os = out.stride()[:3]
-    i3 = ctypes.c_int64 * 3
-    args = _lib.CrossAttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), ret.data_ptr(), i3(*q.stride()[:3]), i3(*ks), i3(*vs), i3(*os),
-                                   lens_ptr, off_ptr, mask_ptr, mask_stride, B, H, Hk, Tq, T, D,
-                                   float(D ** -0.5 if scale is None else scale), dtype_code(dtype))
-    with on_device(dev):
-        _lib.check(_lib.load().svdq_cross_attention(ctypes.byref(args), stream_ptr(dev)))
+    args = _lib.CrossAttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), ret.data_ptr(), *qs[:3], *ks, *vs, *os, lens_ptr, off_ptr, mask_ptr, mask_stride,
+                                   B, H, Hk, Tq, T, D, float(D ** -0.5 if scale is None else scale), dtype_code(dtype))
+    launch(_lib.load().svdq_cross_attention, args, dev)
     return ret

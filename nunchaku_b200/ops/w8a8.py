@@ -6,12 +6,10 @@ Forward only, as the rest of the package.
 """
 from __future__ import annotations
 
-from ctypes import byref
-
 import torch
 
 from .. import _lib
-from ..utils import HALF_DTYPES, dtype_code, on_device, stream_ptr
+from ..utils import HALF_DTYPES, dtype_code, launch
 
 
 def _rows(name: str, t: torch.Tensor, cols: int) -> tuple[int, int]:
@@ -44,28 +42,38 @@ def _check_half(name: str, t: torch.Tensor, like: torch.Tensor | None = None) ->
 
 def _quantize(x, weight, residual, eps):
     _check_half("x", x)
-    cols = x.shape[-1] if x.dim() else 0
-    if x.numel() == 0 or cols % 16:
+    shape = x.shape
+    cols = shape[-1] if shape else 0
+    n = x.numel()
+    if n == 0 or cols % 16:
         raise ValueError("x must be [..., C] with at least one row and C a positive multiple of 16")
-    rows, x_stride = _rows("x", x, cols)
-    hidden, res_stride = None, 0
+    dev = x.device
+    if x.is_contiguous():
+        rows, x_stride = n // cols, cols
+        codes = torch.empty_like(x, dtype=torch.int8)
+    else:
+        rows, x_stride = _rows("x", x, cols)
+        codes = torch.empty(shape, dtype=torch.int8, device=dev)
+    scales = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=dev)
+    if len(shape) != 2:
+        scales = scales.view(shape[:-1])
+    hidden_ptr = res_ptr = weight_ptr = hidden = None
+    res_stride = 0
     if weight is not None:
         _check_half("weight", weight, x)
         if weight.shape != (cols,) or not weight.is_contiguous():
             raise ValueError("weight must be a contiguous [C]")
+        weight_ptr = weight.data_ptr()
     if residual is not None:
         _check_half("residual", residual, x)
-        if residual.shape != x.shape:
+        if residual.shape != shape:
             raise ValueError("residual must have x's shape")
-        res_stride = _rows("residual", residual, cols)[1]
-        hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    args = _lib.QuantizeW8A8Args(x.data_ptr(), None if residual is None else residual.data_ptr(), None if weight is None else weight.data_ptr(),
-                                 codes.data_ptr(), scales.data_ptr(), None if hidden is None else hidden.data_ptr(), rows, x_stride,
-                                 res_stride, cols, eps, dtype_code(x.dtype))
-    with on_device(x.device):
-        _lib.check(_lib.load().svdq_quantize_w8a8(byref(args), stream_ptr(x.device)))
+        res_stride = cols if residual.is_contiguous() else _rows("residual", residual, cols)[1]
+        hidden = torch.empty_like(x, memory_format=torch.contiguous_format)
+        res_ptr, hidden_ptr = residual.data_ptr(), hidden.data_ptr()
+    launch(_lib.load().svdq_quantize_w8a8,
+           _lib.QuantizeW8A8Args(x.data_ptr(), res_ptr, weight_ptr, codes.data_ptr(), scales.data_ptr(), hidden_ptr, rows, x_stride, res_stride,
+                                 cols, eps, dtype_code(x.dtype)), dev)
     return codes, scales, hidden
 
 
@@ -102,10 +110,10 @@ def dequantize_w8a8(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.
     cols = codes.shape[-1] if codes.dim() else 0
     if codes.numel() == 0 or cols % 16 or scales.shape != codes.shape[:-1]:
         raise ValueError("codes must be [..., C] with at least one row and C a positive multiple of 16, scales [...]")
-    out = torch.empty(codes.shape, dtype=out_dtype, device=codes.device)
-    args = _lib.DequantizeW8A8Args(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel() // cols, cols, dtype_code(out_dtype))
-    with on_device(codes.device):
-        _lib.check(_lib.load().svdq_dequantize_w8a8(byref(args), stream_ptr(codes.device)))
+    code = dtype_code(out_dtype)
+    out = torch.empty_like(codes, dtype=out_dtype)
+    launch(_lib.load().svdq_dequantize_w8a8,
+           _lib.DequantizeW8A8Args(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel() // cols, cols, code), codes.device)
     return out
 
 
@@ -117,21 +125,20 @@ def gemm_w8a8(act: torch.Tensor, wgt: torch.Tensor, ascales: torch.Tensor, wscal
     K: a multiple of 16 up to 131056; N: a multiple of 8; any number of rows from one on.  ``out`` [..., N] bf16 / fp16 may be rows of a
     wider buffer (unit column stride, one row stride that is a multiple of 8); by default a new tensor of ``out_dtype`` (bias's dtype,
     else bf16)."""
-    for name, t in (("act", act), ("wgt", wgt)):
-        if not t.is_cuda or t.dtype != torch.int8 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous CUDA int8 tensor")
-    for name, t in (("ascales", ascales), ("wscales", wscales)):
-        if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous CUDA fp32 tensor")
-    if wgt.dim() != 2 or act.dim() < 1 or act.shape[-1] != wgt.shape[1] or act.numel() == 0:
-        raise ValueError("act must be [..., K] with at least one row and wgt [N, K]")
-    N, K = wgt.shape
-    lead = act.shape[:-1]
-    if ascales.shape != lead or wscales.shape != (N,):
-        raise ValueError("ascales must be act's shape without K and wscales [N]")
     dev = act.device
+    if not act.is_cuda or act.dtype != torch.int8 or wgt.dtype != torch.int8 or not act.is_contiguous() or not wgt.is_contiguous():
+        raise ValueError("act and wgt must be contiguous CUDA int8 tensors")
+    if ascales.dtype != torch.float32 or wscales.dtype != torch.float32 or not ascales.is_contiguous() or not wscales.is_contiguous():
+        raise ValueError("ascales and wscales must be contiguous fp32 tensors")
     if wgt.device != dev or ascales.device != dev or wscales.device != dev:
         raise ValueError("all tensors must be on act's device")
+    shape = act.shape
+    if wgt.dim() != 2 or not shape or shape[-1] != wgt.shape[1] or act.numel() == 0:
+        raise ValueError("act must be [..., K] with at least one row and wgt [N, K]")
+    N, K = wgt.shape
+    lead = shape[:-1]
+    if ascales.shape != lead or wscales.shape != (N,):
+        raise ValueError("ascales must be act's shape without K and wscales [N]")
     if out is not None:
         if out.shape != (*lead, N) or out.device != dev or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError("out must be [..., N] on act's device (of out_dtype, where that is given)")
@@ -141,13 +148,15 @@ def gemm_w8a8(act: torch.Tensor, wgt: torch.Tensor, ascales: torch.Tensor, wscal
     code = dtype_code(dtype)
     if bias is not None and (bias.shape != (N,) or bias.dtype != dtype or not bias.is_contiguous() or bias.device != dev):
         raise ValueError("bias must be a contiguous [N] of the output's dtype on act's device")
+    rows = act.numel() // K
     if out is None:
-        out = torch.empty((*lead, N), dtype=dtype, device=dev)
+        out = torch.empty_strided((rows, N), (N, 1), dtype=dtype, device=dev)
+        if len(shape) != 2:
+            out = out.view(*lead, N)
         stride = N
     else:
         stride = _rows("out", out, N)[1]
-    args = _lib.GemmW8A8Args(act.data_ptr(), wgt.data_ptr(), ascales.data_ptr(), wscales.data_ptr(), None if bias is None else bias.data_ptr(),
-                             out.data_ptr(), stride, act.numel() // K, N, K, code)
-    with on_device(dev):
-        _lib.check(_lib.load().svdq_gemm_w8a8(byref(args), stream_ptr(dev)))
+    launch(_lib.load().svdq_gemm_w8a8,
+           _lib.GemmW8A8Args(act.data_ptr(), wgt.data_ptr(), ascales.data_ptr(), wscales.data_ptr(), None if bias is None else bias.data_ptr(),
+                             out.data_ptr(), stride, rows, N, K, code), dev)
     return out

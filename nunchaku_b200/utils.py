@@ -59,6 +59,18 @@ def on_device(device: torch.device):
     return torch.cuda.device(idx)
 
 
+def launch(entry, args, device: torch.device) -> None:
+    """``entry(args, stream)`` on torch's current stream of ``device``, with ``device`` current; raises what its status says."""
+    cur, idx = torch._C._cuda_getDevice(), device.index
+    if idx is None or idx == cur:
+        rc = entry(args, torch._C._cuda_getCurrentRawStream(cur))
+    else:
+        with torch.cuda.device(idx):
+            rc = entry(args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        _lib.check(rc)
+
+
 # The 16-bit floating-point types of the path (the reference's GEMMConfig_W4A4_BF16 / _FP16) and their C-ABI codes.
 HALF_DTYPES = (torch.bfloat16, torch.float16)
 

@@ -23,7 +23,8 @@ def lib():
 def test_struct_layout_matches_c(lib, tmp_path):
     cname, cls = "svdq_cross_attention_args", lib.CrossAttentionArgs
     lines = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{HEADER}"', "int main(void){", f'printf("size %zu\\n", sizeof({cname}));']
-    lines += [f'printf("{f} %zu\\n", offsetof({cname}, {f}));' for f, _ in cls._fields_]
+    member = lambda f: f"{f[:-1]}[{f[-1]}]" if "_stride" in f and f[-1].isdigit() else f   # q_stride0 stands for q_stride[0]
+    lines += [f'printf("{f} %zu\\n", offsetof({cname}, {member(f)}));' for f, _ in cls._fields_]
     c = tmp_path / "layout.c"
     c.write_text("\n".join([*lines, "return 0;}"]))
     subprocess.run(["gcc", "-std=c99", "-o", str(tmp_path / "layout"), str(c)], check=True)
@@ -33,7 +34,6 @@ def test_struct_layout_matches_c(lib, tmp_path):
         assert int(got[f]) == getattr(cls, f).offset, f
 
 
-I3 = ctypes.c_int64 * 3
 GOOD = dict(q=64, k=64, v=64, out=64, q_stride=(4096, 64, 256), k_stride=(4096, 64, 256), v_stride=(4096, 64, 256), o_stride=(4096, 64, 256),
             batch=2, heads=4, kv_heads=4, q_len=16, kv_len=16, head_dim=64, scale=0.125)
 
@@ -41,7 +41,7 @@ GOOD = dict(q=64, k=64, v=64, out=64, q_stride=(4096, 64, 256), k_stride=(4096, 
 def _call(lib, **kw):
     d = {**GOOD, **kw}
     for s in ("q_stride", "k_stride", "v_stride", "o_stride"):
-        d[s] = I3(*d[s])
+        d.update({f"{s}{i}": x for i, x in enumerate(d.pop(s))})
     return lib.load().svdq_cross_attention(ctypes.byref(lib.CrossAttentionArgs(**d)), None)
 
 
