@@ -11,13 +11,12 @@
 // w8a8_pair_kernel (many tokens): the two SMs of a CTA pair walk 256 x BN output tiles (tcgen05.mma cta_group::2 kind::i8,
 // M 256, K 32), each CTA holding its 128 token rows and half of the weight rows of a 128-deep K stage (128B-swizzled TMA
 // boxes) in a ring; two accumulators of up to 256 columns alternate in TMEM, so that the epilogue of a tile runs under the
-// next tile's products.  Warps: 0 tokens' producer, 1 weights' producer, 2 MMA issuer (leader CTA), 4-11 epilogue (two per
-// lane quadrant, alternating 32-column chunks).
+// next tile's products.  Warps: 0-3 producers, 4 MMA issuer (leader CTA), 8-15
+// epilogue (two per lane quadrant, alternating 32-column chunks).
 //
 // w8a8_skinny_kernel (few tokens, the serving form): there every weight is used for a handful of rows and the kernel streams
-// weights.  The operands change places: 128 weight rows are the M side of the product, the tokens (16 to 128) its N side,
-// so that a tile of weights is 16 KB whatever the token count, and K is split over a cluster of up to 8 CTAs to fill the
-// SMs.  The int32 partial sums are exchanged through distributed shared memory (integers: the order does not matter).
+// weights.  The operands change places: 128 weight rows are the M side of the product, up to 16 tokens its N side, and K is split
+// over a cluster of up to 8 CTAs to fill the SMs.  The int32 partial sums are exchanged through distributed shared memory (integers: the order does not matter).
 //
 // Every wait is bounded; a role whose wait runs out records SVDQ_ERR_TIMEOUT and leaves its loop.
 #include <cuda_bf16.h>
@@ -36,7 +35,8 @@ constexpr int W8_B_BYTES = (W8_BN_MAX / 2) * W8_BK;
 constexpr int W8_STAGE_BYTES = W8_A_BYTES + W8_B_BYTES;
 constexpr int W8_STAGES = 6;
 constexpr int W8_EPI_WARPS = 8;
-constexpr int W8_THREADS = (4 + W8_EPI_WARPS) * 32;
+constexpr int W8_MMA_WARP = 4, W8_EPI_WARP0 = 8;   // 0-3 producers, 5-7 nothing
+constexpr int W8_THREADS = (W8_EPI_WARP0 + W8_EPI_WARPS) * 32;
 constexpr int W8_COL_BYTES = 2 * W8_BN_MAX * 4;   // column scales and bias of one tile
 constexpr int W8_SMEM = 1024 + W8_STAGES * W8_STAGE_BYTES + W8_COL_BYTES + 256;
 constexpr int W8_MAX_K = 131071;
@@ -116,7 +116,7 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < W8_STAGES; ++s) {
-            mbar_init(&sh->full[s], 4);       // two producers in each CTA
+            mbar_init(&sh->full[s], 4);       // two copies in each CTA
             mbar_init(&sh->empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -129,39 +129,41 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         prefetch_tmap(&tm_a);
         prefetch_tmap(&tm_b);
     }
-    if (warp == 2) {
+    if (warp == W8_MMA_WARP) {
         tmem_alloc_pair(&sh->tmem_base, 512);
         tmem_relinquish_pair();
     }
     tc_fence_before_sync();
     cluster_sync_all();   // barriers of both CTAs are initialised before anything remote touches them
     tc_fence_after_sync();
+    pdl_launch_dependents();
+    pdl_wait();           // nothing above touches global memory
     const uint32_t tmem = sh->tmem_base;
 
-    if (warp < 2) {
-        // ------------------------------------------------------------------ producers: 0 = tokens, 1 = weights
-        uint32_t slot = 0, phase = 1;
+    if (warp < 4) {
+        // ------------------------------------------------------------------ producers: warps 0, 2 tokens, 1, 3 weights, of every other stage each (the
+        // copies of one issuing warp are worked off one after the other, in about the time a stage's products take)
+        const bool wgt = warp & 1;
+        const uint32_t turn = warp >> 1, bytes = wgt ? bnh * W8_BK : W8_A_BYTES;
+        uint32_t it = 0;      // W8S_STAGES so far
         bool ok = true;
-        const uint32_t bytes = warp == 0 ? W8_A_BYTES : bnh * W8_BK;
         for (int tile = pair; tile < ntiles && ok; tile += npairs) {
-            const int row = warp == 0 ? (tile % p.tiles_m) * (2 * W8_BM) + rank * W8_BM : (tile / p.tiles_m) * p.bn + rank * bnh;
-            for (int ks = 0; ks < kstages; ++ks) {
-                ok = __all_sync(0xffffffffu, w8_wait(&sh->empty[slot], phase, sh, p.status, 810 + warp));
+            const int row = wgt ? (tile / p.tiles_m) * p.bn + rank * bnh : (tile % p.tiles_m) * (2 * W8_BM) + rank * W8_BM;
+            for (int ks = 0; ks < kstages; ++ks, ++it) {
+                if ((it & 1) != turn) continue;
+                const uint32_t slot = it % W8_STAGES;
+                ok = __all_sync(0xffffffffu, w8_wait(&sh->empty[slot], ((it / W8_STAGES) & 1) ^ 1, sh, p.status, 810 + warp));
                 if (!ok) break;
-                uint8_t* dst = smem + slot * W8_STAGE_BYTES + (warp ? W8_A_BYTES : 0);
+                uint8_t* dst = smem + slot * W8_STAGE_BYTES + (wgt ? W8_A_BYTES : 0);
                 const uint32_t lfull = mapa_shared(smem_u32(&sh->full[slot]), 0);
                 if (elect_one()) {
                     mbar_arrive_expect_tx_cluster(lfull, bytes);
-                    tma_load_2d_pair(dst, warp == 0 ? &tm_a : &tm_b, lfull, ks * W8_BK, row);
+                    tma_load_2d_pair(dst, wgt ? &tm_b : &tm_a, lfull, ks * W8_BK, row);
                 }
                 __syncwarp();
-                if (++slot == W8_STAGES) {
-                    slot = 0;
-                    phase ^= 1;
-                }
             }
         }
-    } else if (warp == 2 && rank == 0) {
+    } else if (warp == W8_MMA_WARP && rank == 0) {
         // ------------------------------------------------------------------ MMA issuer
         const uint32_t idesc = idesc_i8(2 * W8_BM, p.bn, true);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
@@ -209,10 +211,10 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             }
             __syncwarp();
         }
-    } else if (warp >= 4) {
+    } else if (warp >= W8_EPI_WARP0) {
         // ------------------------------------------------------------------ epilogue
-        const int quad = warp & 3, set = (warp - 4) >> 2;
-        const int et = threadIdx.x - 128;
+        const int quad = warp & 3, set = (warp - W8_EPI_WARP0) >> 2;
+        const int et = threadIdx.x - W8_EPI_WARP0 * 32;
         int ti = 0;
         for (int tile = pair; tile < ntiles; tile += npairs, ++ti) {
             const uint32_t as = ti & 1;
@@ -265,7 +267,7 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();
-    if (warp == 2) {
+    if (warp == W8_MMA_WARP) {
         tc_fence_after_sync();
         tmem_dealloc_pair(tmem, 512);
     }
@@ -275,78 +277,74 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
 constexpr int W8S_BW = 128;                       // weight rows per CTA (the M side)
 constexpr int W8S_W_BYTES = W8S_BW * W8_BK;
 constexpr int W8S_THREADS = 6 * 32;
-constexpr int W8S_MAX_STAGES = 4;
-constexpr int W8S_MAX_TOKENS = 128;               // tokens per CTA (the N side)
+constexpr int W8S_STAGES = 4;
+constexpr int W8S_TOKENS = 16;                    // the N side; more tokens are the other kernel's
 constexpr int W8S_MAX_SPLIT = 8;
+constexpr int W8S_STAGE_BYTES = W8S_W_BYTES + W8S_TOKENS * W8_BK;
+constexpr int W8S_TMEM_COLS = 32;
+constexpr int W8S_SMEM = 1024 + W8S_STAGES * W8S_STAGE_BYTES + 256;   // 73 KB: three CTAs per SM
 
 struct W8SShared {
-    uint64_t full[W8S_MAX_STAGES], empty[W8S_MAX_STAGES], done;
+    uint64_t full[W8S_STAGES], empty[W8S_STAGES], done;
     uint32_t tmem_base;
-    int failed;
 };
+static_assert(W8S_STAGES * W8S_STAGE_BYTES >= W8S_TOKENS * W8S_BW * 4 && sizeof(W8SShared) <= 256, "the exchange buffer lies over the ring");
 
-__host__ __device__ constexpr int w8s_stages(int bt) { return bt <= 64 ? 4 : 3; }
-__host__ __device__ constexpr int w8s_smem(int bt) { return 1024 + w8s_stages(bt) * (W8S_W_BYTES + bt * W8_BK) + 256; }
-static_assert(w8s_stages(128) * (W8S_W_BYTES + 128 * W8_BK) >= 128 * W8S_BW * 4 && w8s_stages(16) * W8S_W_BYTES >= 16 * W8S_BW * 4,
-              "the exchange buffer lies over the ring");
-
-// grid (weight tiles * split, token tiles), cluster (split, 1, 1)
+// grid (weight tiles * split), cluster (split, 1, 1)
 template <bool F16>
 __global__ void __launch_bounds__(W8S_THREADS)
-w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t, const W8Params p, const int bt,
-                   const int split) {
+w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t, const W8Params p, const int split) {
     extern __shared__ __align__(1024) uint8_t w8_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(w8_smem_raw) + 1023) & ~uintptr_t(1023));
-    const int stages = w8s_stages(bt), stage_bytes = W8S_W_BYTES + bt * W8_BK;
-    W8SShared* sh = reinterpret_cast<W8SShared*>(smem + stages * stage_bytes);
+    W8SShared* sh = reinterpret_cast<W8SShared*>(smem + W8S_STAGES * W8S_STAGE_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-    const int n0 = (blockIdx.x / split) * W8S_BW, m0 = blockIdx.y * bt;
+    const int n0 = (blockIdx.x / split) * W8S_BW;
     const int kstages = (p.K + W8_BK - 1) / W8_BK;
     const int ks0 = kstages * rank / split, ks1 = kstages * (rank + 1) / split;
-    const uint32_t tcols = bt <= 32 ? 32 : bt;    // TMEM columns: a power of two from 32 on
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) {
+        for (int s = 0; s < W8S_STAGES; ++s) {
             mbar_init(&sh->full[s], 1);
             mbar_init(&sh->empty[s], 1);
         }
         mbar_init(&sh->done, 1);
-        sh->failed = 0;
         fence_mbar_init();
         prefetch_tmap(&tm_w);
         prefetch_tmap(&tm_t);
     }
     if (warp == 1) {
-        tmem_alloc(&sh->tmem_base, tcols);
+        tmem_alloc(&sh->tmem_base, W8S_TMEM_COLS);
         tmem_relinquish();
     }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
+    pdl_launch_dependents();
+    pdl_wait();           // nothing above touches global memory
     const uint32_t tmem = sh->tmem_base;
 
     if (warp == 0) {
         if (lane == 0) {
             for (int i = 0; i < ks1 - ks0; ++i) {
-                const int s = i % stages;
-                if (!mbar_wait(&sh->empty[s], ((i / stages) & 1) ^ 1, W8_WAIT_CYCLES)) {
+                const int s = i % W8S_STAGES;
+                if (!mbar_wait(&sh->empty[s], ((i / W8S_STAGES) & 1) ^ 1, W8_WAIT_CYCLES)) {
                     atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
                     atomicExch(&p.status[1], 840);
                     break;
                 }
-                uint8_t* st = smem + s * stage_bytes;
-                mbar_arrive_expect_tx(&sh->full[s], stage_bytes);
+                uint8_t* st = smem + s * W8S_STAGE_BYTES;
+                mbar_arrive_expect_tx(&sh->full[s], W8S_STAGE_BYTES);
                 tma_load_2d(st, &tm_w, &sh->full[s], (ks0 + i) * W8_BK, n0);
-                tma_load_2d(st + W8S_W_BYTES, &tm_t, &sh->full[s], (ks0 + i) * W8_BK, m0);
+                tma_load_2d(st + W8S_W_BYTES, &tm_t, &sh->full[s], (ks0 + i) * W8_BK, 0);
             }
         }
     } else if (warp == 1) {
-        const uint32_t idesc = idesc_i8(W8S_BW, bt, true);
+        constexpr uint32_t idesc = idesc_i8(W8S_BW, W8S_TOKENS, true);
         bool ok = true;
         for (int i = 0; i < ks1 - ks0; ++i) {
-            const int s = i % stages;
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh->full[s], (i / stages) & 1, W8_WAIT_CYCLES));
+            const int s = i % W8S_STAGES;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh->full[s], (i / W8S_STAGES) & 1, W8_WAIT_CYCLES));
             if (!ok) {
                 if (lane == 0) {
                     atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
@@ -356,8 +354,8 @@ w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
             }
             tc_fence_after_sync();
             if (elect_one()) {
-                const uint64_t wd = smem_desc_sw128(smem_u32(smem + s * stage_bytes));
-                const uint64_t td = smem_desc_sw128(smem_u32(smem + s * stage_bytes + W8S_W_BYTES));
+                const uint64_t wd = smem_desc_sw128(smem_u32(smem + s * W8S_STAGE_BYTES));
+                const uint64_t td = smem_desc_sw128(smem_u32(smem + s * W8S_STAGE_BYTES + W8S_W_BYTES));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) tc_mma_i8(tmem, wd + 2 * j, td + 2 * j, idesc, (i | j) ? 1u : 0u);
                 tc_commit(&sh->empty[s]);
@@ -377,13 +375,11 @@ w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     if (done && warp >= 2) {
         tc_fence_after_sync();
         const int quad = warp & 3;
-        for (int c = 0; c < bt; c += 16) {
-            uint32_t r[16];
-            tc_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + c, r);
-            tc_wait_ld();
+        uint32_t r[16];
+        tc_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16), r);
+        tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) red[(c + i) * W8S_BW + quad * 32 + lane] = static_cast<int>(r[i]);
-        }
+        for (int i = 0; i < W8S_TOKENS; ++i) red[i * W8S_BW + quad * 32 + lane] = static_cast<int>(r[i]);
     }
     tc_fence_before_sync();
     if (split > 1) cluster_sync_all();
@@ -392,18 +388,27 @@ w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
         const int row = (warp & 3) * 32 + lane, n = n0 + row;
         const float sw = n < p.N ? p.wscales[n] : 0.f;
         const float bias = p.bias && n < p.N ? w8_load16<F16>(p.bias, n) : 0.f;
-        for (int t = rank; t < bt && m0 + t < p.M; t += split) {
-            int sum = 0;
-            if (split > 1) {
-#pragma unroll 1
-                for (int q = 0; q < split; ++q) sum += ld_shared_cluster_s32(mapa_shared(smem_u32(red + t * W8S_BW + row), q));
-            } else {
-                sum = red[t * W8S_BW + row];
-            }
-            if (n < p.N) {
-                const float v = fmaf(static_cast<float>(sum) * p.ascales[m0 + t], sw, bias);
-                const uint32_t w = w8_pack<F16>(v, 0.f);
-                static_cast<uint16_t*>(p.out)[static_cast<long long>(m0 + t) * p.out_stride + n] = static_cast<uint16_t>(w);
+        uint32_t peer[W8S_MAX_SPLIT];
+#pragma unroll
+        for (int q = 0; q < W8S_MAX_SPLIT; ++q) peer[q] = q < split ? mapa_shared(smem_u32(red + row), q) : 0;
+        const int tokens = min(W8S_TOKENS, p.M);
+        // this CTA's tokens, four at a time with every peer's value asked for before the first is used
+        for (int t = rank; t < tokens; t += 4 * split) {
+            int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int q = 0; q < W8S_MAX_SPLIT; ++q)
+                if (q < split) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (t + u * split < tokens) sum[u] += ld_shared_cluster_s32(peer[q] + (t + u * split) * (W8S_BW * 4));
+                }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int m = t + u * split;
+                if (m < tokens && n < p.N) {
+                    const uint32_t w = w8_pack<F16>(fmaf(static_cast<float>(sum[u]) * p.ascales[m], sw, bias), 0.f);
+                    static_cast<uint16_t*>(p.out)[static_cast<long long>(m) * p.out_stride + n] = static_cast<uint16_t>(w);
+                }
             }
         }
     }
@@ -411,7 +416,7 @@ w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     else __syncthreads();
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem, tcols);
+        tmem_dealloc(tmem, W8S_TMEM_COLS);
     }
 }
 
@@ -421,44 +426,37 @@ static int w8_tmap(CUtensorMap* map, const void* base, int rows, int K, int box_
                         static_cast<uint64_t>(K), W8_BK, static_cast<uint32_t>(box_rows), true);
 }
 
+// `cluster` CTAs of a cluster along x; launched so that the prologue may run under the predecessor's tail (both kernels wait for it
+// before they touch global memory)
+template <typename Kernel, typename... Args>
+static int launch_w8(Kernel kernel, int grid, int threads, int smem, int cluster, std::atomic<uint64_t>& attr_done, cudaStream_t stream, Args... args) {
+    if (int rc = ensure_dynamic_smem(kernel, smem, attr_done)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return SVDQ_OK;
+}
 template <bool F16>
 static int launch_w8_pair(const CUtensorMap& ta, const CUtensorMap& tb, const W8Params& p, int pairs, cudaStream_t stream) {
     static std::atomic<uint64_t> attr_done{0};
-    if (int rc = ensure_dynamic_smem(w8a8_pair_kernel<F16>, W8_SMEM, attr_done)) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * pairs, 1, 1);
-    cfg.blockDim = dim3(W8_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = W8_SMEM;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, w8a8_pair_kernel<F16>, ta, tb, p));
-    return SVDQ_OK;
+    return launch_w8(w8a8_pair_kernel<F16>, 2 * pairs, W8_THREADS, W8_SMEM, 2, attr_done, stream, ta, tb, p);
 }
-
 template <bool F16>
-static int launch_w8_skinny(const CUtensorMap& tw, const CUtensorMap& tt, const W8Params& p, int bt, int split, cudaStream_t stream) {
+static int launch_w8_skinny(const CUtensorMap& tw, const CUtensorMap& tt, const W8Params& p, int split, cudaStream_t stream) {
     static std::atomic<uint64_t> attr_done{0};
-    if (int rc = ensure_dynamic_smem(w8a8_skinny_kernel<F16>, w8s_smem(W8S_MAX_TOKENS), attr_done)) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((p.N + W8S_BW - 1) / W8S_BW * split, (p.M + bt - 1) / bt, 1);
-    cfg.blockDim = dim3(W8S_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = w8s_smem(bt);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, w8a8_skinny_kernel<F16>, tw, tt, p, bt, split));
-    return SVDQ_OK;
+    return launch_w8(w8a8_skinny_kernel<F16>, (p.N + W8S_BW - 1) / W8S_BW * split, W8S_THREADS, W8S_SMEM, split, attr_done, stream, tw, tt, p, split);
 }
 
 }  // namespace svdq
@@ -490,14 +488,14 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args* a, void* stream) {
     const bool f16 = a->dtype == SVDQ_DTYPE_FP16;
     const int kstages = (a->K + W8_BK - 1) / W8_BK;
     CUtensorMap ta, tb;
-    if (a->M <= W8S_MAX_TOKENS) {
-        const int bt = a->M <= 16 ? 16 : a->M <= 32 ? 32 : a->M <= 64 ? 64 : 128;
+    if (a->M <= W8S_TOKENS) {
+        // K over as many CTAs as give every SM one (more cost more in joining than they bring)
         const int tiles = (a->N + W8S_BW - 1) / W8S_BW;
         int split = 1;
-        while (split < W8S_MAX_SPLIT && tiles * split < 2 * sms && 2 * split <= kstages) split *= 2;
+        while (split < W8S_MAX_SPLIT && tiles * split < sms && 2 * split <= kstages) split *= 2;
         if (int rc = w8_tmap(&ta, a->wgt, a->N, a->K, W8S_BW)) return rc;
-        if (int rc = w8_tmap(&tb, a->act, a->M, a->K, bt)) return rc;
-        return f16 ? launch_w8_skinny<true>(ta, tb, p, bt, split, st) : launch_w8_skinny<false>(ta, tb, p, bt, split, st);
+        if (int rc = w8_tmap(&tb, a->act, a->M, a->K, W8S_TOKENS)) return rc;
+        return f16 ? launch_w8_skinny<true>(ta, tb, p, split, st) : launch_w8_skinny<false>(ta, tb, p, split, st);
     }
     const int max_pairs = sms / 2;
     p.tiles_m = (a->M + 2 * W8_BM - 1) / (2 * W8_BM);
