@@ -40,10 +40,15 @@ struct Quant8Params {
     float eps;
 };
 
-// maximum that keeps a NaN (fmaxf drops it)
-__device__ __forceinline__ float max_nan(float a, float b) {
+// largest magnitude of three; a NaN stays one (fmaxf drops it)
+__device__ __forceinline__ float absmax3_nan(float a, float b, float c) {
     float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {   // of magnitudes
+    float d;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
     return d;
 }
 
@@ -104,18 +109,18 @@ quantize_w8a8_kernel(const Quant8Params p) {
                 }
                 z[j][2 * i] = h.x;
                 z[j][2 * i + 1] = h.y;
-                top = max_nan(top, max_nan(fabsf(h.x), fabsf(h.y)));
+                top = absmax3_nan(top, h.x, h.y);
             }
             if constexpr (RES) {
                 if (tid + j * threads < nvec)
                     reinterpret_cast<uint4*>(p.hidden + row * p.cols)[tid + j * threads] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
             }
         }
+        if constexpr (NORM) {
 #pragma unroll
-        for (int m = 16; m >= 1; m >>= 1) {
-            if constexpr (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
+            for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
         }
+        top = warp_max_nan(top);
         if (W > 1) {
             // two buffers in turn: a warp that writes row r + 2 has passed row r + 1's barrier, which every reader of row r's
             // values reaches behind its reads
@@ -123,33 +128,40 @@ quantize_w8a8_kernel(const Quant8Params p) {
             __syncthreads();
             const float2 o = lane < W ? part[buf][lane] : make_float2(0.f, 0.f);
             ss = o.x;
-            top = o.y;
+            if constexpr (NORM) {
 #pragma unroll
-            for (int m = 16; m >= 1; m >>= 1) {
-                if constexpr (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-                top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
+                for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);   // at most 16 warps
+                ss = __shfl_sync(0xffffffffu, ss, 0);
             }
+            top = warp_max_nan(o.y);
         }
-        const float rstd = NORM ? 1.0f / sqrtf(ss / static_cast<float>(p.cols) + p.eps) : 1.0f;
+        // Per-row scalars, which every thread computes: kept to a few instructions (with four full divisions and a root the kernel was
+        // bound by them).
         const bool finite = top < __int_as_float(0x7f800000) && ss < __int_as_float(0x7f800000);   // false for NaN
-        float inv = top > 0.f ? 127.0f / top : 0.f;
-        if (top > 0.f && top < 1e-30f) {   // 127 / top would leave fp32: both sides times 2^100 (exact)
-            constexpr float UP = 1.2676506002282294e30f;
-            inv = 127.0f / (top * UP);
+        const float up = top < 1e-30f ? 1.2676506002282294e30f : 1.0f;   // 2^100 (exact) for a row whose 127 / top would leave fp32
+        const float inv = top > 0.f ? 127.0f * __frcp_rn(top * up) : 0.f;
+        // 127 / top to twice the precision: a value of half the row's largest, common among 16-bit inputs, stands exactly on the tie 63.5,
+        // and is to be told from its neighbours by the quotient, not by the rounding of the reciprocal
+        const float inv_lo = NORM ? 0.f : fmaf(-(top * up), inv, 127.0f) * (inv * (1.0f / 127.0f));
+        if (up != 1.0f) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) z[j][i] *= UP;
+                for (int i = 0; i < 8; ++i) z[j][i] *= up;
         }
+        auto code = [&](float v) { return NORM ? v * inv : fmaf(v, inv, v * inv_lo); };
         uint2* cp = reinterpret_cast<uint2*>(p.codes + row * p.cols);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             if (tid + j * threads >= nvec) continue;
-            const uint2 c = make_uint2(pack_codes4(z[j][0] * inv, z[j][1] * inv, z[j][2] * inv, z[j][3] * inv),
-                                       pack_codes4(z[j][4] * inv, z[j][5] * inv, z[j][6] * inv, z[j][7] * inv));
+            const uint2 c = make_uint2(pack_codes4(code(z[j][0]), code(z[j][1]), code(z[j][2]), code(z[j][3])),
+                                       pack_codes4(code(z[j][4]), code(z[j][5]), code(z[j][6]), code(z[j][7])));
             cp[tid + j * threads] = finite ? c : make_uint2(0u, 0u);
         }
-        if (tid == 0) p.scales[row] = finite ? top * rstd / 127.0f : __int_as_float(0x7fc00000);
+        if (tid == 0) {
+            const float rstd = NORM ? 1.0f / sqrtf(ss / static_cast<float>(p.cols) + p.eps) : 1.0f;
+            p.scales[row] = finite ? top * rstd / 127.0f : __int_as_float(0x7fc00000);
+        }
     }
 }
 
