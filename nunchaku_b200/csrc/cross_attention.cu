@@ -583,40 +583,41 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 }
 
 // ---------------------------------------------------------------------------------------------------------------- few query rows
-constexpr int CR_WARPS = 4, CR_THREADS = 32 * CR_WARPS, CR_KEYS = 16, CR_STAGES = 2, CR_ROWS = 16, CR_MAX_SPLIT = 8;
-constexpr int CR_TILE = CR_WARPS * CR_KEYS;          // states that the CTA's warps take in one turn
+constexpr int CR_WARPS = 4, CR_THREADS = 32 * (CR_WARPS + 1), CR_KEYS = 16, CR_ROWS = 16, CR_MAX_SPLIT = 8;
+constexpr int CR_TILE = CR_WARPS * CR_KEYS;          // states of a tile: 16 per warp
+constexpr int CR_STAGES = 2;
+constexpr long long CR_WAIT_CYCLES = 600000000ll;   // ~0.3 s
+constexpr int CR_HALF_BYTES = CR_TILE * 128;         // 64 states x 64 channels
 
 struct CrossRowsParams {
     CrossStates st;
-    const uint8_t *q, *k, *v;
+    const uint8_t* q;
     uint8_t* out;
-    long long qs[3], ks[3], vs[3], os[3];   // batch, head, token strides in bytes
+    long long qs[3], os[3];                 // batch, head, token strides in bytes
     int kv_heads, group, q_rows, dim;       // q_rows = q_len * group: row r is query r / group, head kv_head * group + r % group
+    int k_bmul, k_hmul, v_bmul, v_hmul;     // 0 where that dimension is broadcast: its coordinate is then 0
     float scale_log2;
+    int* status;
 };
 
 template <int NK>
 struct CrossRowsSizes {
-    static constexpr int ROW = (2 * NK + 1) * 16;           // bytes of a state's row: an odd number of 16-byte pieces, so that ldmatrix has no conflicts
-    static constexpr int TILE = CR_KEYS * ROW;
-    static constexpr int STAGE = 2 * TILE;
-    static constexpr int RING = CR_WARPS * CR_STAGES * STAGE;   // each warp has a ring of its own
+    static constexpr int HALVES = NK > 4 ? 2 : 1;
+    static constexpr int STAGE = 2 * HALVES * CR_HALF_BYTES;    // K and V
+    static constexpr int RING = CR_STAGES * STAGE;
     static constexpr int COLS = NK * 16;
     // afterwards over the ring: the warps' partial sums [4][16][COLS], maxima and sums [4][16] each
     static_assert(RING >= CR_WARPS * CR_ROWS * (COLS + 2) * 4, "the partial sums lie over the ring");
     // behind the ring, written by the CTAs of the cluster: each one's sums of the elements that this CTA finishes, and their maxima and sums
     static constexpr int mail_floats(int rows, int split) { return split * ((rows * COLS / 2 + split - 1) / split) * 2; }
-    static constexpr int smem(int rows, int split) { return RING + (mail_floats(rows, split) + 2 * split * rows) * 4; }
+    static constexpr int smem(int rows, int split) { return 1024 + RING + 64 + (mail_floats(rows, split) + 2 * split * rows) * 4; }
 };
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {   // writes zeros where not valid (src is not read)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t src) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(src) : "memory");
 }
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const void* src) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(src)) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* src) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(src)) : "memory");
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t src) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(src) : "memory");
 }
 template <bool F16>
 __device__ __forceinline__ void mma_16816_t(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -631,170 +632,213 @@ __device__ __forceinline__ void st_shared_cluster_f32x2(uint32_t cluster_addr, f
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y) : "memory");
 }
 
-// grid (batch * kv_heads * split, row tiles), cluster (split, 1, 1)
+// grid (batch * kv_heads * split), cluster (split, 1, 1)
 template <bool F16, int NK>
 __global__ void __launch_bounds__(CR_THREADS)
-cross_rows_kernel(const CrossRowsParams p, const int split) {
+cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CrossRowsParams p,
+                  const int split) {
     using S = CrossRowsSizes<NK>;
-    extern __shared__ __align__(1024) uint8_t cr_smem[];
+    extern __shared__ __align__(1024) uint8_t cr_smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cr_smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::RING);
+    uint64_t* empty = full + CR_STAGES;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
     const int pairix = blockIdx.x / split, batch = pairix / p.kv_heads, kv_head = pairix % p.kv_heads;
-    const int r0 = blockIdx.y * CR_ROWS, rows = min(CR_ROWS, p.q_rows - r0);
+    const int rows = p.q_rows;
+    if (tid == 0) {
+#pragma unroll
+        for (int i = 0; i < CR_STAGES; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], CR_WARPS);
+        }
+        fence_mbar_init();
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+    }
+    pdl_launch_dependents();
+    pdl_wait();   // nothing above touches global memory
     int start, count;
     cross_range(p.st, batch, start, count);
     const int tiles = (count + CR_TILE - 1) / CR_TILE;
     const int t0 = static_cast<int>(static_cast<long long>(tiles) * rank / split), t1 = static_cast<int>(static_cast<long long>(tiles) * (rank + 1) / split);
-    const uint8_t* kbase = p.k + kv_head * p.ks[1] + (p.st.kv_offsets ? start * p.ks[2] : batch * p.ks[0]);
-    const uint8_t* vbase = p.v + kv_head * p.vs[1] + (p.st.kv_offsets ? start * p.vs[2] : batch * p.vs[0]);
-    const uint8_t* mask = p.st.mask ? p.st.mask + batch * p.st.mask_stride : nullptr;
-    uint8_t* ring = cr_smem + warp * CR_STAGES * S::STAGE;
+    __syncthreads();
 
-    // this warp's 16 states of a turn; rows of states that are not to be seen, and channels past the head, become zeros
-    auto load = [&](int tile, int slot) {
-        uint8_t* ks = ring + slot * S::STAGE;
-        const int key0 = tile * CR_TILE + warp * CR_KEYS;
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const int idx = lane + i * 32, r = idx / (2 * NK), c = idx % (2 * NK);
-            const int key = key0 + r;
-            bool valid = key < count && c * 8 < p.dim;
-            if (mask && valid) valid = mask[key] != 0;
-            const uint8_t* ksrc = valid ? kbase + key * p.ks[2] + c * 16 : p.k;
-            const uint8_t* vsrc = valid ? vbase + key * p.vs[2] + c * 16 : p.v;
-            cp_async16(ks + r * S::ROW + c * 16, ksrc, valid);
-            cp_async16(ks + S::TILE + r * S::ROW + c * 16, vsrc, valid);
-        }
-    };
-#pragma unroll
-    for (int s = 0; s < CR_STAGES - 1; ++s) {
-        if (t0 + s < t1) load(t0 + s, s);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    // query fragments: rows g and g + 8
-    uint32_t qf[NK][4];
-    {
-        const uint8_t* qrow[2];
-        bool there[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = r0 + g + 8 * i;
-            there[i] = r < p.q_rows;
-            qrow[i] = p.q + batch * p.qs[0] + (kv_head * p.group + (there[i] ? r % p.group : 0)) * p.qs[1] + (there[i] ? r / p.group : 0) * p.qs[2];
-        }
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int ch = kk * 16 + (i >> 1) * 8 + 2 * t;
-                qf[kk][i] = there[i & 1] && ch < p.dim ? *reinterpret_cast<const uint32_t*>(qrow[i & 1] + 2 * ch) : 0u;
-            }
-    }
     float o[2 * NK][4];
-#pragma unroll
-    for (int i = 0; i < 2 * NK; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int slot = 0;
-    for (int tile = t0; tile < t1; ++tile) {
-        // the copies of this turn have landed for every lane, and every lane has left the slot that is filled next
-        asm volatile("cp.async.wait_group %0;" ::"n"(CR_STAGES - 2) : "memory");
-        __syncwarp();
-        if (tile + CR_STAGES - 1 < t1) load(tile + CR_STAGES - 1, (slot + CR_STAGES - 1) % CR_STAGES);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        const uint8_t* ks = ring + slot * S::STAGE;
-        const uint8_t* vs = ks + S::TILE;
-        slot = (slot + 1) % CR_STAGES;
-        const int key0 = tile * CR_TILE + warp * CR_KEYS;
-        if (key0 >= count) continue;
-        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    bool ok = true;
+    if (warp == CR_WARPS) {
+        // ------------------------------------------------------------------ producer
+        if (lane == 0) {
+            int i = 0;
+#pragma unroll 1
+            for (int tile = t0; tile < t1; ++tile, ++i) {
+                const int s = i % CR_STAGES;
+                if (!mbar_wait(&empty[s], ((i / CR_STAGES) & 1) ^ 1, CR_WAIT_CYCLES)) {
+                    ok = false;
+                    break;
+                }
+                mbar_arrive_expect_tx(&full[s], S::STAGE);
+                uint8_t* st = smem + s * S::STAGE;
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-            uint32_t b[4];
-            ldmatrix_x4(b, ks + ((lane >> 4) * 8 + (lane & 7)) * S::ROW + (kk * 2 + ((lane >> 3) & 1)) * 16);
-            mma_16816_t<F16>(s[0], qf[kk], b[0], b[1]);
-            mma_16816_t<F16>(s[1], qf[kk], b[2], b[3]);
-        }
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int key = key0 + i * 8 + 2 * t + (e & 1);
-                const bool seen = key < count && (!mask || mask[key] != 0);
-                s[i][e] = seen ? s[i][e] * p.scale_log2 : -INFINITY;
-                top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
+                for (int h = 0; h < S::HALVES; ++h) {
+                    tma_load_4d(st + h * CR_HALF_BYTES, &tm_k, &full[s], h * 64, start + tile * CR_TILE, kv_head * p.k_hmul, p.st.kv_offsets ? 0 : batch * p.k_bmul);
+                    tma_load_4d(st + (S::HALVES + h) * CR_HALF_BYTES, &tm_v, &full[s], h * 64, start + tile * CR_TILE, kv_head * p.v_hmul,
+                                p.st.kv_offsets ? 0 : batch * p.v_bmul);
+                }
             }
-        float alpha[2], base[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-            const float mn = fmaxf(m[i], top[i]);
-            base[i] = mn == -INFINITY ? 0.f : mn;         // nothing seen yet: every exponential below is 2^-inf = 0
-            alpha[i] = ex2(m[i] - base[i]);
-            m[i] = mn;
-            l[i] *= alpha[i];
+            if (!ok)   // leave with none of the copies in flight
+                for (int k = i > CR_STAGES ? i - CR_STAGES : 0; k < i; ++k) mbar_wait(&full[k % CR_STAGES], (k / CR_STAGES) & 1, CR_WAIT_CYCLES);
         }
-        uint32_t pf[4];
+    } else {
+        // ------------------------------------------------------------------ consumers
+        const uint8_t* mask = p.st.mask ? p.st.mask + batch * p.st.mask_stride : nullptr;
+        const bool cut = p.st.kv_lens || p.st.kv_offsets;   // rows behind the sample's last are somebody's: elsewhere the copy fills in zeros
+        // query fragments: rows g and g + 8
+        uint32_t qf[NK][4];
+        {
+            const uint8_t* qrow[2];
+            bool there[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float e[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) e[q] = ex2(s[i][q] - base[q >> 1]);
-            l[0] += e[0] + e[1];
-            l[1] += e[2] + e[3];
-            pf[2 * i] = pack_h16<F16>(e[0], e[1]);
-            pf[2 * i + 1] = pack_h16<F16>(e[2], e[3]);
-        }
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-            for (int i = 0; i < 2 * NK; ++i) {
-                o[i][0] *= alpha[0];
-                o[i][1] *= alpha[0];
-                o[i][2] *= alpha[1];
-                o[i][3] *= alpha[1];
+            for (int i = 0; i < 2; ++i) {
+                const int r = g + 8 * i;
+                there[i] = r < rows;
+                qrow[i] = p.q + batch * p.qs[0] + (kv_head * p.group + (there[i] ? r % p.group : 0)) * p.qs[1] + (there[i] ? r / p.group : 0) * p.qs[2] + 4 * t;
             }
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    qf[kk][i] = there[i & 1] && kk * 16 + (i >> 1) * 8 < p.dim ? *reinterpret_cast<const uint32_t*>(qrow[i & 1] + kk * 32 + (i >> 1) * 16) : 0u;
         }
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-            uint32_t b[4];
-            ldmatrix_x4_trans(b, vs + (((lane >> 3) & 1) * 8 + (lane & 7)) * S::ROW + (kk * 2 + (lane >> 4)) * 16);
-            mma_16816_t<F16>(o[2 * kk], pf, b[0], b[1]);
-            mma_16816_t<F16>(o[2 * kk + 1], pf, b[2], b[3]);
+        for (int i = 0; i < 2 * NK; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+        // this lane's rows of the ldmatrix groups, and the 16-byte piece that stands for piece 0 / 1 of its row (128-byte swizzle)
+        const uint32_t base = smem_u32(smem) + warp * CR_KEYS * 128;
+        const uint32_t k_row = ((lane >> 4) * 8 + (lane & 7)) * 128, k_x = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
+        const uint32_t v_row = (((lane >> 3) & 1) * 8 + (lane & 7)) * 128, v_x = ((lane >> 4) ^ (lane & 7)) << 4;
+        // which of this warp's 16 states of a tile are to be seen
+        auto visible = [&](int tile) {
+            const int left = count - tile * CR_TILE - warp * CR_KEYS;
+            uint32_t bits = left >= CR_KEYS ? 0xffffu : left > 0 ? (1u << left) - 1u : 0u;
+            if (mask) bits &= __ballot_sync(0xffffffffu, lane < CR_KEYS && lane < left && mask[tile * CR_TILE + warp * CR_KEYS + lane] != 0);
+            return bits;
+        };
+        uint32_t next_bits = t0 < t1 ? visible(t0) : 0u;
+#pragma unroll 1
+        for (int tile = t0; tile < t1; ++tile) {
+            const int i = tile - t0, slot = i % CR_STAGES;
+            const uint32_t bits = next_bits;
+            if (tile + 1 < t1) next_bits = visible(tile + 1);
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (i / CR_STAGES) & 1, CR_WAIT_CYCLES)))) break;
+            if (bits) {
+                const uint32_t ks = base + slot * S::STAGE, vs = ks + S::HALVES * CR_HALF_BYTES;
+                float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int kk = 0; kk < NK; ++kk) {
+                    uint32_t b[4];
+                    ldmatrix_x4(b, ks + (kk >> 2) * CR_HALF_BYTES + k_row + (k_x ^ ((kk & 3) << 5)));
+                    mma_16816_t<F16>(s[0], qf[kk], b[0], b[1]);
+                    mma_16816_t<F16>(s[1], qf[kk], b[2], b[3]);
+                }
+                if (bits != 0xffffu && (mask || cut)) {   // rows of V that must not be seen -> zeros: two lanes per row
+                    if (!((bits >> (lane >> 1)) & 1u))
+#pragma unroll
+                        for (int c = 0; c < 4 * S::HALVES; ++c)
+                            *reinterpret_cast<uint4*>(smem + slot * S::STAGE + (S::HALVES + (c >> 2)) * CR_HALF_BYTES + (warp * CR_KEYS + (lane >> 1)) * 128 +
+                                                      ((lane & 1) * 4 + (c & 3)) * 16) = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                }
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[h][e] = (bits >> (h * 8 + 2 * t + (e & 1))) & 1u ? s[h][e] * p.scale_log2 : -INFINITY;
+                        top[e >> 1] = fmaxf(top[e >> 1], s[h][e]);
+                    }
+                float alpha[2], ref[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                    const float mn = fmaxf(m[r], top[r]);
+                    ref[r] = mn == -INFINITY ? 0.f : mn;         // nothing seen yet: every exponential below is 2^-inf = 0
+                    alpha[r] = ex2(m[r] - ref[r]);
+                    m[r] = mn;
+                    l[r] *= alpha[r];
+                }
+                uint32_t pf[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float e[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) e[q] = ex2(s[h][q] - ref[q >> 1]);
+                    l[0] += e[0] + e[1];
+                    l[1] += e[2] + e[3];
+                    pf[2 * h] = pack_h16<F16>(e[0], e[1]);
+                    pf[2 * h + 1] = pack_h16<F16>(e[2], e[3]);
+                }
+                if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+                    for (int c = 0; c < 2 * NK; ++c) {
+                        o[c][0] *= alpha[0];
+                        o[c][1] *= alpha[0];
+                        o[c][2] *= alpha[1];
+                        o[c][3] *= alpha[1];
+                    }
+                }
+#pragma unroll
+                for (int kk = 0; kk < NK; ++kk) {
+                    uint32_t b[4];
+                    ldmatrix_x4_trans(b, vs + (kk >> 2) * CR_HALF_BYTES + v_row + (v_x ^ ((kk & 3) << 5)));
+                    mma_16816_t<F16>(o[2 * kk], pf, b[0], b[1]);
+                    mma_16816_t<F16>(o[2 * kk + 1], pf, b[2], b[3]);
+                }
+                if (bits != 0xffffu && (mask || cut)) fence_proxy_async_smem();   // zeros written here, ahead of the next copy into the slot
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[slot]);
         }
+    }
+    if (!ok && lane == 0) {
+        atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
+        atomicExch(&p.status[1], 880 + warp);
     }
     // Every CTA of the cluster has started (its shared memory may be written from here on); the wait is at the joining below.
     if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    // ---- the warps' sums into shared memory (over the ring), rows that exist only
-    float* part = reinterpret_cast<float*>(cr_smem);               // [4][16][COLS]
+    // ---- the warps' sums into shared memory (over the ring: every copy has been waited for), rows that exist only
+    float* part = reinterpret_cast<float*>(smem);                  // [4][16][COLS]
     float* pm = part + CR_WARPS * CR_ROWS * S::COLS;               // [4][16]
     float* pl = pm + CR_WARPS * CR_ROWS;
+    if (warp < CR_WARPS) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = g + 8 * i;
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (r < rows) {
-            if (t == 0) {
-                pm[warp * CR_ROWS + r] = m[i];
-                pl[warp * CR_ROWS + r] = l[i];
+        for (int i = 0; i < 2; ++i) {
+            const int r = g + 8 * i;
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (r < rows) {
+                if (t == 0) {
+                    pm[warp * CR_ROWS + r] = m[i];
+                    pl[warp * CR_ROWS + r] = l[i];
+                }
+                float* dst = part + (warp * CR_ROWS + r) * S::COLS + 2 * t;
+#pragma unroll
+                for (int c = 0; c < 2 * NK; ++c) *reinterpret_cast<float2*>(dst + c * 8) = make_float2(o[c][2 * i], o[c][2 * i + 1]);
             }
-#pragma unroll
-            for (int c = 0; c < 2 * NK; ++c)
-                *reinterpret_cast<float2*>(part + (warp * CR_ROWS + r) * S::COLS + c * 8 + 2 * t) = make_float2(o[c][2 * i], o[c][2 * i + 1]);
         }
     }
     __syncthreads();
     // ---- joined over the warps and sent to the CTA of the cluster that finishes the element: element e (a pair of channels) belongs
     // to CTA e % split, which keeps [source CTA][e / split] pairs and every source's maximum and sum per row
     const int half = p.dim >> 1, elems = rows * half, per = (rows * S::COLS / 2 + split - 1) / split;
-    float2* mail = reinterpret_cast<float2*>(cr_smem + S::RING);   // [split][per]
-    float2* stat = mail + split * per;                             // [split][rows]: maximum, sum
+    float2* mail = reinterpret_cast<float2*>(smem + S::RING + 64);   // [split][per]
+    float2* stat = mail + split * per;                               // [split][rows]: maximum, sum
     if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+#pragma unroll 1
     for (int e = tid; e < elems; e += CR_THREADS) {
         const int r = e / half, c = (e - r * half) * 2;
         float mm = pm[r];
@@ -817,32 +861,31 @@ cross_rows_kernel(const CrossRowsParams p, const int split) {
         } else {
             st_shared_cluster_f32x2(mapa_shared(smem_u32(mail + rank * per + e / split), e % split), sum);
             if (c == 0)
+#pragma unroll 1
                 for (int q = 0; q < split; ++q) st_shared_cluster_f32x2(mapa_shared(smem_u32(stat + rank * rows + r), q), make_float2(mm, ls));
         }
     }
     if (split > 1) cluster_sync_all();   // nothing is read from or written to another CTA behind this
     else __syncthreads();
+#pragma unroll 1
     for (int e = rank + split * tid; e < elems; e += split * CR_THREADS) {
         const int r = e / half, c = (e - r * half) * 2;
         float mm = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < CR_MAX_SPLIT; ++q)
-            if (q < split) mm = fmaxf(mm, stat[q * rows + r].x);
+#pragma unroll 1
+        for (int q = 0; q < split; ++q) mm = fmaxf(mm, stat[q * rows + r].x);
         const float b = mm == -INFINITY ? 0.f : mm;
         float2 sum = make_float2(0.f, 0.f);
         float ls = 0.f;
-#pragma unroll
-        for (int q = 0; q < CR_MAX_SPLIT; ++q)
-            if (q < split) {
-                const float2 ml = stat[q * rows + r], v = mail[q * per + e / split];
-                const float f = ex2(ml.x - b);
-                sum.x = fmaf(f, v.x, sum.x);
-                sum.y = fmaf(f, v.y, sum.y);
-                ls = fmaf(f, ml.y, ls);
-            }
+#pragma unroll 2
+        for (int q = 0; q < split; ++q) {
+            const float2 ml = stat[q * rows + r], v = mail[q * per + e / split];
+            const float f = ex2(ml.x - b);
+            sum.x = fmaf(f, v.x, sum.x);
+            sum.y = fmaf(f, v.y, sum.y);
+            ls = fmaf(f, ml.y, ls);
+        }
         const float inv = ls == 0.f ? 0.f : 1.f / ls;   // nothing seen: zeros (a sum over anything is at least 1)
-        const int row = r0 + r;
-        uint8_t* dst = p.out + batch * p.os[0] + (kv_head * p.group + row % p.group) * p.os[1] + (row / p.group) * p.os[2] + 2 * c;
+        uint8_t* dst = p.out + batch * p.os[0] + (kv_head * p.group + r % p.group) * p.os[1] + (r / p.group) * p.os[2] + 2 * c;
         *reinterpret_cast<uint32_t*>(dst) = pack_h16<F16>(sum.x * inv, sum.y * inv);
     }
 }
@@ -881,37 +924,39 @@ static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const
 }
 
 template <bool F16, int NK>
-static int launch_cross_rows(const CrossRowsParams& p, int pairs, int split, cudaStream_t stream) {
+static int launch_cross_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CrossRowsParams& p, int pairs, int split, cudaStream_t stream) {
     auto kern = cross_rows_kernel<F16, NK>;
     static std::atomic<uint64_t> attr_done{0};
     if (int rc = ensure_dynamic_smem(kern, CrossRowsSizes<NK>::smem(CR_ROWS, CR_MAX_SPLIT), attr_done)) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(pairs * split, (p.q_rows + CR_ROWS - 1) / CR_ROWS, 1);
+    cfg.gridDim = dim3(pairs * split, 1, 1);
     cfg.blockDim = dim3(CR_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = CrossRowsSizes<NK>::smem(p.q_rows < CR_ROWS ? p.q_rows : CR_ROWS, split);
+    cfg.dynamicSmemBytes = CrossRowsSizes<NK>::smem(p.q_rows, split);
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = split;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // the prologue may run under the predecessor's tail
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, p, split));
+    cfg.numAttrs = 2;
+    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, tk, tv, p, split));
     return SVDQ_OK;
 }
 
 template <bool F16>
-static int launch_cross_rows_dim(const CrossRowsParams& p, int pairs, int split, cudaStream_t stream) {
+static int launch_cross_rows_dim(const CUtensorMap& tk, const CUtensorMap& tv, const CrossRowsParams& p, int pairs, int split, cudaStream_t stream) {
     switch ((p.dim + 15) / 16) {
-        case 1: return launch_cross_rows<F16, 1>(p, pairs, split, stream);
-        case 2: return launch_cross_rows<F16, 2>(p, pairs, split, stream);
-        case 3: return launch_cross_rows<F16, 3>(p, pairs, split, stream);
-        case 4: return launch_cross_rows<F16, 4>(p, pairs, split, stream);
-        case 5: return launch_cross_rows<F16, 5>(p, pairs, split, stream);
-        case 6: return launch_cross_rows<F16, 6>(p, pairs, split, stream);
-        case 7: return launch_cross_rows<F16, 7>(p, pairs, split, stream);
-        default: return launch_cross_rows<F16, 8>(p, pairs, split, stream);
+        case 1: return launch_cross_rows<F16, 1>(tk, tv, p, pairs, split, stream);
+        case 2: return launch_cross_rows<F16, 2>(tk, tv, p, pairs, split, stream);
+        case 3: return launch_cross_rows<F16, 3>(tk, tv, p, pairs, split, stream);
+        case 4: return launch_cross_rows<F16, 4>(tk, tv, p, pairs, split, stream);
+        case 5: return launch_cross_rows<F16, 5>(tk, tv, p, pairs, split, stream);
+        case 6: return launch_cross_rows<F16, 6>(tk, tv, p, pairs, split, stream);
+        case 7: return launch_cross_rows<F16, 7>(tk, tv, p, pairs, split, stream);
+        default: return launch_cross_rows<F16, 8>(tk, tv, p, pairs, split, stream);
     }
 }
 
@@ -961,13 +1006,9 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         CrossRowsParams p = {};
         p.st = states;
         p.q = static_cast<const uint8_t*>(a->q);
-        p.k = static_cast<const uint8_t*>(a->k);
-        p.v = static_cast<const uint8_t*>(a->v);
         p.out = static_cast<uint8_t*>(a->out);
         for (int i = 0; i < 3; ++i) {
             p.qs[i] = 2 * a->q_stride[i];
-            p.ks[i] = 2 * a->k_stride[i];
-            p.vs[i] = 2 * a->v_stride[i];
             p.os[i] = 2 * a->o_stride[i];
         }
         p.kv_heads = a->kv_heads;
@@ -975,12 +1016,20 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         p.q_rows = static_cast<int>(q_rows);
         p.dim = a->head_dim;
         p.scale_log2 = scale_log2;
-        // states per sample as far as the host knows
-        const long long len = a->kv_offsets ? (a->kv_len + a->batch - 1) / a->batch : a->kv_len;
-        const long long tiles = (len + CR_TILE - 1) / CR_TILE, ctas = kv_pairs * ((q_rows + CR_ROWS - 1) / CR_ROWS);
+        // Split while the CTAs are all resident at once (three per SM for heads above 64 channels, six below): a further wave costs more
+        // than it balances (16 samples x 8 heads x 4096 x 128: 43 us with 256 CTAs, 47 with 512, 57 with 1024).
+        const long long len = a->kv_offsets ? (a->kv_len + a->batch - 1) / a->batch : a->kv_len;   // states per sample as far as the host knows
+        const long long tiles = (len + CR_TILE - 1) / CR_TILE;
+        const int ring = CR_STAGES * 2 * (a->head_dim > 64 ? 2 : 1) * CR_HALF_BYTES;
+        const long long resident = static_cast<long long>(sms) * (228 * 1024 / (ring + 6 * 1024));
         int split = 1;
-        while (split < CR_MAX_SPLIT && ctas * split < 2ll * sms && 2 * split <= tiles) split *= 2;
-        return f16 ? launch_cross_rows_dim<true>(p, static_cast<int>(kv_pairs), split, st) : launch_cross_rows_dim<false>(p, static_cast<int>(kv_pairs), split, st);
+        while (split < CR_MAX_SPLIT && kv_pairs * split * 2 <= resident && 2 * split <= tiles) split *= 2;
+        if (int rc = status_words(&p.status)) return rc;
+        CUtensorMap mk, mv;
+        if (int rc = cross_tmap(&mk, tk, a->head_dim, a->dtype, CR_TILE, &p.k_bmul, &p.k_hmul)) return rc;
+        if (int rc = cross_tmap(&mv, tv, a->head_dim, a->dtype, CR_TILE, &p.v_bmul, &p.v_hmul)) return rc;
+        return f16 ? launch_cross_rows_dim<true>(mk, mv, p, static_cast<int>(kv_pairs), split, st)
+                   : launch_cross_rows_dim<false>(mk, mv, p, static_cast<int>(kv_pairs), split, st);
     }
     // The kernel keeps its samples' ranges and mask bits in shared memory: launches of as many samples as fit (hundreds, without a mask).
     const int q_tiles = (a->q_len + CT_BM - 1) / CT_BM;
