@@ -600,6 +600,10 @@ struct CrossRowsParams {
     int* status;
 };
 
+// CTAs per SM, by the registers that the queries and the output take (a third CTA at 128 channels spills and is slower: 34 -> 38 us on
+// [16, 24 over 8, 1 over <= 4096, 128])
+__host__ __device__ constexpr int cross_rows_per_sm(int nk) { return nk > 7 ? 2 : nk > 4 ? 3 : nk > 2 ? 4 : 6; }
+
 template <int NK>
 struct CrossRowsSizes {
     static constexpr int HALVES = NK > 4 ? 2 : 1;
@@ -632,20 +636,20 @@ __device__ __forceinline__ void st_shared_cluster_f32x2(uint32_t cluster_addr, f
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y) : "memory");
 }
 
-// grid (batch * kv_heads * split), cluster (split, 1, 1)
+// grid (batch * kv_heads * split, row tiles), cluster (split, 1, 1)
 template <bool F16, int NK>
-__global__ void __launch_bounds__(CR_THREADS)
+__global__ void __launch_bounds__(CR_THREADS, cross_rows_per_sm(NK))
 cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CrossRowsParams p,
-                  const int split) {
+                  const int log_split) {
     using S = CrossRowsSizes<NK>;
     extern __shared__ __align__(1024) uint8_t cr_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cr_smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::RING);
     uint64_t* empty = full + CR_STAGES;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-    const int pairix = blockIdx.x / split, batch = pairix / p.kv_heads, kv_head = pairix % p.kv_heads;
-    const int rows = p.q_rows;
+    const int split = 1 << log_split, rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int pairix = blockIdx.x >> log_split, batch = pairix / p.kv_heads, kv_head = pairix % p.kv_heads;
+    const int r0 = blockIdx.y * CR_ROWS, rows = min(CR_ROWS, p.q_rows - r0);
     if (tid == 0) {
 #pragma unroll
         for (int i = 0; i < CR_STAGES; ++i) {
@@ -703,7 +707,8 @@ cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             for (int i = 0; i < 2; ++i) {
                 const int r = g + 8 * i;
                 there[i] = r < rows;
-                qrow[i] = p.q + batch * p.qs[0] + (kv_head * p.group + (there[i] ? r % p.group : 0)) * p.qs[1] + (there[i] ? r / p.group : 0) * p.qs[2] + 4 * t;
+                const int row = r0 + (there[i] ? r : 0);
+                qrow[i] = p.q + batch * p.qs[0] + (kv_head * p.group + row % p.group) * p.qs[1] + (row / p.group) * p.qs[2] + 4 * t;
             }
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
@@ -812,8 +817,8 @@ cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     __syncthreads();
     // ---- the warps' sums into shared memory (over the ring: every copy has been waited for), rows that exist only
     float* part = reinterpret_cast<float*>(smem);                  // [4][16][COLS]
-    float* pm = part + CR_WARPS * CR_ROWS * S::COLS;               // [4][16]
-    float* pl = pm + CR_WARPS * CR_ROWS;
+    float* pm = part + CR_WARPS * CR_ROWS * S::COLS;               // [4][16] maxima, then the warps' factors
+    float* pl = pm + CR_WARPS * CR_ROWS;                           // [4][16] sums
     if (warp < CR_WARPS) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -832,61 +837,82 @@ cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         }
     }
     __syncthreads();
-    // ---- joined over the warps and sent to the CTA of the cluster that finishes the element: element e (a pair of channels) belongs
-    // to CTA e % split, which keeps [source CTA][e / split] pairs and every source's maximum and sum per row
-    const int half = p.dim >> 1, elems = rows * half, per = (rows * S::COLS / 2 + split - 1) / split;
+    // ---- joined over the warps and sent to the CTA of the cluster that finishes the element: pair of channels e (row e / (COLS / 2))
+    // belongs to CTA e % split, which keeps [source CTA][e / split] pairs, and every CTA every source's maximum and sum per row
+    constexpr int HALF = S::COLS / 2;
+    const int elems = rows * HALF, per = (elems + split - 1) >> log_split;
     float2* mail = reinterpret_cast<float2*>(smem + S::RING + 64);   // [split][per]
     float2* stat = mail + split * per;                               // [split][rows]: maximum, sum
     if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-#pragma unroll 1
-    for (int e = tid; e < elems; e += CR_THREADS) {
-        const int r = e / half, c = (e - r * half) * 2;
-        float mm = pm[r];
+    if (tid < rows) {
+        float mw[CR_WARPS], mm = -INFINITY, ls = 0.f;
 #pragma unroll
-        for (int w = 1; w < CR_WARPS; ++w) mm = fmaxf(mm, pm[w * CR_ROWS + r]);
+        for (int w = 0; w < CR_WARPS; ++w) mm = fmaxf(mm, mw[w] = pm[w * CR_ROWS + tid]);
         const float b = mm == -INFINITY ? 0.f : mm;
-        float2 sum = make_float2(0.f, 0.f);
-        float ls = 0.f;
 #pragma unroll
         for (int w = 0; w < CR_WARPS; ++w) {
-            const float f = ex2(pm[w * CR_ROWS + r] - b);
+            const float f = ex2(mw[w] - b);
+            pm[w * CR_ROWS + tid] = f;
+            ls = fmaf(f, pl[w * CR_ROWS + tid], ls);
+        }
+#pragma unroll 1
+        for (int q = 0; q < split; ++q) {
+            float2* dst = stat + rank * rows + tid;
+            if (split > 1) st_shared_cluster_f32x2(mapa_shared(smem_u32(dst), q), make_float2(mm, ls));
+            else *dst = make_float2(mm, ls);
+        }
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int e = tid; e < elems; e += CR_THREADS) {
+        const int r = e / HALF, c = (e % HALF) * 2;
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < CR_WARPS; ++w) {
+            const float f = pm[w * CR_ROWS + r];
             const float2 v = *reinterpret_cast<const float2*>(part + (w * CR_ROWS + r) * S::COLS + c);
             sum.x = fmaf(f, v.x, sum.x);
             sum.y = fmaf(f, v.y, sum.y);
-            ls = fmaf(f, pl[w * CR_ROWS + r], ls);
         }
-        if (split == 1) {
-            mail[e] = sum;
-            if (c == 0) stat[r] = make_float2(mm, ls);
-        } else {
-            st_shared_cluster_f32x2(mapa_shared(smem_u32(mail + rank * per + e / split), e % split), sum);
-            if (c == 0)
-#pragma unroll 1
-                for (int q = 0; q < split; ++q) st_shared_cluster_f32x2(mapa_shared(smem_u32(stat + rank * rows + r), q), make_float2(mm, ls));
-        }
+        float2* dst = mail + rank * per + (e >> log_split);
+        if (split > 1) st_shared_cluster_f32x2(mapa_shared(smem_u32(dst), e & (split - 1)), sum);
+        else *dst = sum;
     }
     if (split > 1) cluster_sync_all();   // nothing is read from or written to another CTA behind this
     else __syncthreads();
+    // ---- joined over the CTAs: factors of the sources first (over the warps' sums, which have been read)
+    float* factor = part;                // [split][rows], the quotient by the whole sum included
+    if (tid < rows) {
+        float mm = -INFINITY, ls = 0.f;
 #pragma unroll 1
-    for (int e = rank + split * tid; e < elems; e += split * CR_THREADS) {
-        const int r = e / half, c = (e - r * half) * 2;
-        float mm = -INFINITY;
-#pragma unroll 1
-        for (int q = 0; q < split; ++q) mm = fmaxf(mm, stat[q * rows + r].x);
+        for (int q = 0; q < split; ++q) mm = fmaxf(mm, stat[q * rows + tid].x);
         const float b = mm == -INFINITY ? 0.f : mm;
-        float2 sum = make_float2(0.f, 0.f);
-        float ls = 0.f;
-#pragma unroll 2
+#pragma unroll 1
         for (int q = 0; q < split; ++q) {
-            const float2 ml = stat[q * rows + r], v = mail[q * per + e / split];
+            const float2 ml = stat[q * rows + tid];
             const float f = ex2(ml.x - b);
-            sum.x = fmaf(f, v.x, sum.x);
-            sum.y = fmaf(f, v.y, sum.y);
+            factor[q * rows + tid] = f;
             ls = fmaf(f, ml.y, ls);
         }
         const float inv = ls == 0.f ? 0.f : 1.f / ls;   // nothing seen: zeros (a sum over anything is at least 1)
-        uint8_t* dst = p.out + batch * p.os[0] + (kv_head * p.group + r % p.group) * p.os[1] + (r / p.group) * p.os[2] + 2 * c;
-        *reinterpret_cast<uint32_t*>(dst) = pack_h16<F16>(sum.x * inv, sum.y * inv);
+#pragma unroll 1
+        for (int q = 0; q < split; ++q) factor[q * rows + tid] *= inv;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int e = rank + split * tid; e < elems; e += split * CR_THREADS) {
+        const int r = e / HALF, c = (e % HALF) * 2, row = r0 + r;
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 2
+        for (int q = 0; q < split; ++q) {
+            const float f = factor[q * rows + r];
+            const float2 v = mail[q * per + (e >> log_split)];
+            sum.x = fmaf(f, v.x, sum.x);
+            sum.y = fmaf(f, v.y, sum.y);
+        }
+        if (c < p.dim)
+            *reinterpret_cast<uint32_t*>(p.out + batch * p.os[0] + (kv_head * p.group + row % p.group) * p.os[1] + (row / p.group) * p.os[2] + 2 * c) =
+                pack_h16<F16>(sum.x, sum.y);
     }
 }
 
@@ -929,9 +955,9 @@ static int launch_cross_rows(const CUtensorMap& tk, const CUtensorMap& tv, const
     static std::atomic<uint64_t> attr_done{0};
     if (int rc = ensure_dynamic_smem(kern, CrossRowsSizes<NK>::smem(CR_ROWS, CR_MAX_SPLIT), attr_done)) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(pairs * split, 1, 1);
+    cfg.gridDim = dim3(pairs * split, (p.q_rows + CR_ROWS - 1) / CR_ROWS, 1);
     cfg.blockDim = dim3(CR_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = CrossRowsSizes<NK>::smem(p.q_rows, split);
+    cfg.dynamicSmemBytes = CrossRowsSizes<NK>::smem(p.q_rows < CR_ROWS ? p.q_rows : CR_ROWS, split);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -942,7 +968,7 @@ static int launch_cross_rows(const CUtensorMap& tk, const CUtensorMap& tv, const
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, tk, tv, p, split));
+    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, tk, tv, p, __builtin_ctz(split)));   // a power of two
     return SVDQ_OK;
 }
 
@@ -1002,7 +1028,23 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
     const CrossStates states = {a->kv_lens, a->kv_offsets, static_cast<const uint8_t*>(a->mask), a->mask_stride, a->kv_len};
     const float scale_log2 = a->scale * 1.4426950408889634f;
     const long long kv_pairs = static_cast<long long>(a->batch) * a->kv_heads;
-    if (q_rows <= CR_ROWS && kv_pairs * CR_MAX_SPLIT < (1ll << 31)) {
+    // Which kernel: up to 16 rows per stored head the row kernel; beyond, the one that both kernels' times, fitted in microseconds to
+    // 17 to 512 rows, 77 to 4096 states and 8 to 256 pairs of sample and stored head, say is faster.  The row kernel reads K and V again for every
+    // 16 rows but splits the states; the tile kernel takes 128 rows of one query head at a time, a CTA per 128 x head, and walks all states.
+    // (1 sample, 20 heads of 112, 32 queries over 4096 states: 16 us against 57; 16 x 16 x 64, 128 queries: 233 against 70.)
+    const long long len = a->kv_offsets ? (a->kv_len + a->batch - 1) / a->batch : a->kv_len;   // states per sample as far as the host knows
+    const long long tiles = (len + CR_TILE - 1) / CR_TILE, ctas = kv_pairs * ((q_rows + CR_ROWS - 1) / CR_ROWS);
+    // Split while the CTAs are all resident at once: a further wave costs more than it balances (16 samples x 8 heads x 4096 x 128:
+    // 43 us with 256 CTAs, 47 with 512, 57 with 1024).
+    const long long resident = static_cast<long long>(sms) * cross_rows_per_sm((a->head_dim + 15) / 16);
+    int split = 1;
+    while (split < CR_MAX_SPLIT && ctas * split * 2 <= resident && 2 * split <= tiles) split *= 2;
+    const long long q_items = static_cast<long long>(a->batch) * a->heads * ((a->q_len + CT_BM - 1) / CT_BM);
+    const double rows_alone = 0.65 * static_cast<double>((tiles + split - 1) / split),
+                 rows_shared = (a->head_dim > 64 ? 0.53 : 0.26) * static_cast<double>(ctas) * static_cast<double>(tiles) / sms;
+    const double rows_us = 6.5 + (rows_alone > rows_shared ? rows_alone : rows_shared);
+    const double tile_us = 5.0 + (q_items <= sms ? 0.8 : 1.0 * static_cast<double>((q_items + 2 * sms - 1) / (2 * sms))) * static_cast<double>(tiles);
+    if ((q_rows <= CR_ROWS || rows_us < tile_us) && kv_pairs * CR_MAX_SPLIT < (1ll << 31) && q_rows <= CR_ROWS * 65535ll) {
         CrossRowsParams p = {};
         p.st = states;
         p.q = static_cast<const uint8_t*>(a->q);
@@ -1016,14 +1058,6 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         p.q_rows = static_cast<int>(q_rows);
         p.dim = a->head_dim;
         p.scale_log2 = scale_log2;
-        // Split while the CTAs are all resident at once (three per SM for heads above 64 channels, six below): a further wave costs more
-        // than it balances (16 samples x 8 heads x 4096 x 128: 43 us with 256 CTAs, 47 with 512, 57 with 1024).
-        const long long len = a->kv_offsets ? (a->kv_len + a->batch - 1) / a->batch : a->kv_len;   // states per sample as far as the host knows
-        const long long tiles = (len + CR_TILE - 1) / CR_TILE;
-        const int ring = CR_STAGES * 2 * (a->head_dim > 64 ? 2 : 1) * CR_HALF_BYTES;
-        const long long resident = static_cast<long long>(sms) * (228 * 1024 / (ring + 6 * 1024));
-        int split = 1;
-        while (split < CR_MAX_SPLIT && kv_pairs * split * 2 <= resident && 2 * split <= tiles) split *= 2;
         if (int rc = status_words(&p.status)) return rc;
         CUtensorMap mk, mv;
         if (int rc = cross_tmap(&mk, tk, a->head_dim, a->dtype, CR_TILE, &p.k_bmul, &p.k_hmul)) return rc;

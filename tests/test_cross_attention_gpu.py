@@ -66,7 +66,10 @@ def _inputs(B, H, Hk, Tq, T, D, dtype, seed):
 # few query rows, one tile, ragged tiles; one state, ragged blocks, exact blocks, many blocks; head widths of every step count
 SIZES = [(1, 1, 1, 1, 1, 8), (1, 20, 20, 1, 300, 112), (3, 4, 2, 1, 65, 128), (2, 6, 2, 5, 129, 40), (2, 2, 2, 16, 64, 64), (1, 3, 1, 2, 1000, 72),
          (1, 2, 2, 17, 1, 16), (2, 3, 3, 128, 128, 64), (1, 4, 2, 129, 300, 112), (2, 2, 1, 33, 77, 8), (1, 2, 2, 300, 16, 128), (2, 2, 2, 200, 257, 96),
-         (1, 2, 1, 64, 190, 24), (1, 1, 1, 100, 1153, 80), (3, 1, 1, 40, 64, 48), (1, 2, 2, 70, 192, 104)]
+         (1, 2, 1, 64, 190, 24), (1, 1, 1, 100, 1153, 80), (3, 1, 1, 40, 64, 48), (1, 2, 2, 70, 192, 104),
+         # row tiles of 16 over long lists, split; many heads: 128-row tiles over several blocks (which of the two runs goes by their times)
+         (1, 4, 2, 40, 1000, 72), (2, 6, 2, 30, 700, 128), (1, 1, 1, 500, 900, 32), (1, 16, 16, 140, 300, 112), (1, 16, 4, 150, 257, 128),
+         (2, 32, 32, 150, 300, 64), (2, 32, 8, 129, 520, 40), (4, 40, 40, 20, 200, 96)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -100,7 +103,7 @@ def test_lengths_with_nan_behind_them(Tq, H, Hk, T, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("Tq", [1, 3, 140])
+@pytest.mark.parametrize("Tq", [1, 3, 140, 300])
 @pytest.mark.parametrize("H,Hk,T,D", [(2, 2, 77, 64), (2, 1, 520, 112), (1, 1, 1, 128), (4, 4, 300, 32)])
 def test_masks(Tq, H, Hk, T, D, dtype):
     from nunchaku_b200.ops import cross_attention
@@ -159,12 +162,12 @@ def test_packed(Tq, H, Hk, D, dtype):
     assert _lib.device_status() == (0, 0)
 
 
-@pytest.mark.parametrize("Tq", [2, 130])
-def test_layouts(Tq):
+@pytest.mark.parametrize("Tq,H", [(2, 4), (130, 4), (130, 32)])
+def test_layouts(Tq, H):
     """head-major, token-major, broadcast over batch or heads, an output inside a wider buffer"""
     from nunchaku_b200.ops import cross_attention
 
-    B, H, T, D = 2, 4, 150, 64
+    B, T, D = 2, 150, 64
     g = torch.Generator().manual_seed(3)
     q = torch.randn(B, H, Tq, D, generator=g).bfloat16().cuda()
     k1, v1 = (torch.randn(1, H, T, D, generator=g).bfloat16().cuda() for _ in range(2))
@@ -184,12 +187,12 @@ def test_layouts(Tq):
     assert torch.equal(hm.transpose(1, 2).reshape(B, Tq, H * D), ref)
 
 
-@pytest.mark.parametrize("Tq", [1, 150])
-def test_growing_scores_and_large_scale(Tq):
+@pytest.mark.parametrize("Tq,H", [(1, 2), (150, 2), (150, 16)])
+def test_growing_scores_and_large_scale(Tq, H):
     """the maximum rises from block to block by far more than the rescaling step; nearly one-hot weights"""
     from nunchaku_b200.ops import cross_attention
 
-    B, H, T, D = 2, 2, 900, 128
+    B, T, D = 2, 900, 128
     g = torch.Generator().manual_seed(8)
     q = torch.randn(B, H, Tq, D, generator=g).abs().bfloat16().cuda()
     k = (torch.randn(B, H, T, D, generator=g).abs() * torch.linspace(0.05, 3, T)[:, None]).bfloat16().cuda()
@@ -203,8 +206,8 @@ def test_growing_scores_and_large_scale(Tq):
 def test_long_state_lists():
     from nunchaku_b200.ops import cross_attention
 
-    for Tq, T in ((1, 40000), (200, 5000)):
-        q, k, v = _inputs(1, 2, 1, Tq, T, 64, torch.bfloat16, seed=T)
+    for Tq, T, H in ((1, 40000, 2), (200, 5000, 2), (130, 3000, 64)):
+        q, k, v = _inputs(1, H, H // 2, Tq, T, 64, torch.bfloat16, seed=T)
         _check(cross_attention(q, k, v), q, k, v, _keep(1, T), 0.125)
 
 
@@ -243,6 +246,29 @@ def test_stream_and_graph(Tq):
     lens.copy_(torch.tensor([7, 0], dtype=torch.int32))     # read on the device at replay
     g.replay()
     assert torch.equal(out, cross_attention(q, k, v, kv_lens=lens)) and (out[1] == 0).all() and not torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("form", ["lens", "mask", "packed"])
+def test_more_samples_than_one_launch_holds(form):
+    from nunchaku_b200.ops import cross_attention
+
+    B, H, Tq, T, D = 1600, 1, 17, 70, 16
+    q, k, v = _inputs(B, H, H, Tq, T, D, torch.bfloat16, seed=12)
+    g = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32)
+    keep = _keep(B, T, kv_lens=lens)
+    if form == "lens":
+        got = cross_attention(q, k, v, kv_lens=lens.cuda())
+    elif form == "mask":
+        keep = torch.rand(B, T, generator=g) < 0.3
+        keep[7] = False
+        got = cross_attention(q, k, v, mask=keep.cuda())
+    else:
+        rows = keep.flatten().nonzero().squeeze(1).cuda()
+        off = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)]).to(torch.int32).cuda()
+        flat = lambda t: t.transpose(1, 2).reshape(B * T, H, D)[rows].contiguous()
+        got = cross_attention(q, flat(k), flat(v), kv_offsets=off)
+    _check(got, q, k, v, keep, D ** -0.5)
 
 
 def test_python_layer_refuses():
