@@ -2,6 +2,8 @@
 
 Same constructor, parameter names, shapes and dtypes as the reference, so a reference
 ``state_dict`` loads unchanged; the packed parameters keep the reference's memory order.
+
+``W8A8Linear``: a linear layer with 8-bit weights (one scale per output channel) and 8-bit activations (one scale per token).
 """
 from __future__ import annotations
 
@@ -10,6 +12,7 @@ from torch import nn
 
 from ..ops.gemm import invalidate_prepared, svdq_gemm_w4a4_cuda
 from ..ops.quantize import svdq_quantize_w4a4_act_fuse_lora_cuda
+from ..ops.w8a8 import gemm_w8a8, quantize_w8a8
 
 
 class SVDQW4A4Linear(nn.Module):
@@ -114,3 +117,44 @@ class SVDQW4A4Linear(nn.Module):
             f"SVDQW4A4Linear(in_features={self.in_features}, out_features={self.out_features}, "
             f"rank={self.rank}, precision={self.precision}, act_unsigned={self.act_unsigned})"
         )
+
+
+class W8A8Linear(nn.Module):
+    """``y = x W^T + bias`` through :func:`nunchaku_b200.ops.gemm_w8a8`: ``qweight`` int8 [out, in] with ``wscales`` fp32 [out] (the plain
+    row-major order, nothing packed), activations quantised per token.  ``in_features`` a multiple of 16, ``out_features`` of 8."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, torch_dtype: torch.dtype = torch.bfloat16,
+                 device: str | torch.device | None = None):
+        super().__init__()
+        if in_features % 16 or out_features % 8:
+            raise ValueError("in_features must be a multiple of 16 and out_features of 8")
+        device = torch.device("cpu") if device is None else device
+        self.in_features, self.out_features, self.torch_dtype = in_features, out_features, torch_dtype
+        self.qweight = nn.Parameter(torch.zeros(out_features, in_features, dtype=torch.int8, device=device), requires_grad=False)
+        self.wscales = nn.Parameter(torch.zeros(out_features, dtype=torch.float32, device=device), requires_grad=False)
+        self.bias = nn.Parameter(torch.zeros(out_features, dtype=torch_dtype, device=device), requires_grad=False) if bias else None
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, linear: nn.Linear) -> "W8A8Linear":
+        """Quantise a bf16 / fp16 ``nn.Linear`` that is on the GPU: one symmetric scale per output channel."""
+        m = cls(linear.in_features, linear.out_features, linear.bias is not None, linear.weight.dtype, linear.weight.device)
+        codes, scales = quantize_w8a8(linear.weight.detach())
+        m.qweight.copy_(codes)
+        m.wscales.copy_(scales)
+        if m.bias is not None:
+            m.bias.copy_(linear.bias)
+        return m
+
+    def quantize(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        return quantize_w8a8(x)
+
+    def forward_quant(self, codes: torch.Tensor, scales: torch.Tensor, output: torch.Tensor | None = None) -> torch.Tensor:
+        return gemm_w8a8(codes, self.qweight, scales, self.wscales, bias=self.bias, out=output, out_dtype=self.torch_dtype)
+
+    def forward(self, x: torch.Tensor, output: torch.Tensor | None = None) -> torch.Tensor:
+        codes, scales = self.quantize(x)
+        return self.forward_quant(codes, scales, output)
+
+    def __repr__(self):
+        return f"W8A8Linear(in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None})"

@@ -8,6 +8,9 @@ reference's: ``qkv_proj`` (its output feeds the linear attention kernel), ``out_
 ``q_linear`` and ``out_proj``, ``inverted_conv`` (SiLU fused into its GEMM epilogue) and ``point_conv`` (its quantiser
 gates the (value, gate) pairs: ``fuse_glu``).  The depthwise 3 x 3 convolution, cross attention (torch SDPA), the
 ``kv_linear`` of the caption and the modulation are plain bf16 torch ops, as they are outside the W4A4 path.
+Captions of their own lengths (``caption_lens``, or packed ones with ``caption_offsets``: the reference's ``cu_seqlens_txt``,
+SanaModel.cpp:147-190) go through this library's ``cross_attention``; ``quantize_caption_int8_`` turns the captions' path into W8A8:
+the caption states are normalised and quantised once and every block's ``kv_linear`` runs on those codes.
 ``precision=None`` builds the same model from bf16 ``nn.Linear`` masters (the twin the quantised model is compared
 with in the tests); ``quantize_`` turns such a model into the W4A4 one.
 
@@ -24,10 +27,12 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from ..ops.attention import cross_attention
 from ..ops.fused import gate_residual, layernorm_modulate, litela_attention
 from ..ops.gemm import svdq_gemm_w4a4_cuda
 from ..ops.quantize import svdq_quantize_w4a4_act_fuse_lora_cuda
-from .linear import SVDQW4A4Linear
+from ..ops.w8a8 import quantize_w8a8, rms_norm_quantize_w8a8
+from .linear import SVDQW4A4Linear, W8A8Linear
 from .random_init import random_w4a4_linear
 
 
@@ -131,12 +136,19 @@ class SanaCrossAttention(nn.Module):
         self.kv_linear = nn.Linear(dim, 2 * dim, device=device, dtype=dtype)
         self.out_proj = PaddedW4A4(dim, dim, rank, precision, True, g, device)
 
-    def forward(self, x, cond):
+    def forward(self, x, cond, cond_lens=None, cond_offsets=None):
+        """x: [B, S, C]; cond: [B, T, C], the first ``cond_lens[b]`` (int32 [B]) states of each sample if given, or packed [total, C] with
+        ``cond_offsets`` (int32 [B + 1]); or, with an 8-bit ``kv_linear``, their (codes, scales)."""
         B, S, C = x.shape
         D = C // self.heads
         q = self.q_linear(x).reshape(B, S, self.heads, D).transpose(1, 2)
-        kv = self.kv_linear(cond).view(B, cond.shape[1], 2, self.heads, D)
+        kv = self.kv_linear.forward_quant(*cond) if isinstance(cond, tuple) else self.kv_linear(cond)
+        kv = kv.view(*kv.shape[:-1], 2, self.heads, D)
+        if cond_offsets is not None:
+            return self.out_proj(cross_attention(q, kv[:, 0], kv[:, 1], kv_offsets=cond_offsets))
         k, v = kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+        if cond_lens is not None:
+            return self.out_proj(cross_attention(q, k, v, kv_lens=cond_lens))
         o = F.scaled_dot_product_attention(q, k, v)
         return self.out_proj(o.transpose(1, 2).reshape(B, S, C))
 
@@ -184,13 +196,13 @@ class SanaBlock(nn.Module):
         self.cross_attn = SanaCrossAttention(dim, cross_heads, rank, precision, g, device, dtype)
         self.ff = SanaGLUMBConv(dim, hidden, rank, precision, g, device, dtype)
 
-    def forward(self, x, cond, t6, H, W):
+    def forward(self, x, cond, t6, H, W, cond_lens=None, cond_offsets=None):
         B, S, C = x.shape
         m = (self.scale_shift_table[None] + t6.view(B, 6, C)).unbind(1)   # shift, scale, gate (attention), shift, scale, gate (MLP)
         fused = self.attn.qkv_proj.master is None
         n = _ln_mod(x, m[1], m[0], fused)
         x = _gated(x, m[2], self.attn(n), fused)
-        x = _gated(x, None, self.cross_attn(x, cond), fused)
+        x = _gated(x, None, self.cross_attn(x, cond, cond_lens, cond_offsets), fused)
         n = _ln_mod(x, m[4], m[3], fused)
         return _gated(x, m[5], self.ff(n, H, W), fused)
 
@@ -199,13 +211,15 @@ class SanaTransformer(nn.Module):
     """SANA-1.6B geometry by default; every size can be shrunk for tests."""
 
     def __init__(self, dim=2240, cross_heads=20, hidden=5600, n_blocks=20, in_channels=32, caption_dim=2304,
-                 precision="int4", rank=32, seed=0, device="cuda", dtype=torch.bfloat16):
+                 precision="int4", rank=32, seed=0, device="cuda", dtype=torch.bfloat16, caption_norm: bool = False):
         super().__init__()
         g = torch.Generator(device=device).manual_seed(seed)
         kw = dict(device=device, dtype=dtype)
         self.dim = dim
         self.patch_embed = nn.Linear(in_channels, dim, **kw)
         self.caption_proj = nn.Sequential(nn.Linear(caption_dim, dim, **kw), nn.GELU(approximate="tanh"), nn.Linear(dim, dim, **kw))
+        # RMSNorm behind the caption's projection (the published checkpoints have one, diffusers' ``caption_norm``; off: the states go in as they are)
+        self.caption_norm = nn.RMSNorm(dim, eps=1e-5, **kw) if caption_norm else None
         self.time_mlp = nn.Sequential(nn.Linear(256, dim, **kw), nn.SiLU(), nn.Linear(dim, dim, **kw))
         self.adaln_single = nn.Linear(dim, 6 * dim, **kw)
         self.blocks = nn.ModuleList([SanaBlock(dim, cross_heads, hidden, rank, precision, g, device, dtype) for _ in range(n_blocks)])
@@ -232,8 +246,27 @@ class SanaTransformer(nn.Module):
                 mod.quantize_(precision)
         return self
 
-    def forward(self, latents, caption, timestep, img_hw: tuple[int, int]):
-        """latents [B, H*W, C_in], caption [B, T, caption_dim], timestep [B]."""
+    @torch.no_grad()
+    def quantize_caption_int8_(self):
+        """Turn every block's ``kv_linear`` into its W8A8 layer; the caption states are then quantised once per forward for all of them."""
+        for blk in self.blocks:
+            if not isinstance(blk.cross_attn.kv_linear, W8A8Linear):
+                blk.cross_attn.kv_linear = W8A8Linear.from_linear(blk.cross_attn.kv_linear)
+        return self
+
+    def _caption_states(self, caption):
+        cond = self.caption_proj(caption)
+        if len(self.blocks) == 0 or not isinstance(self.blocks[0].cross_attn.kv_linear, W8A8Linear):
+            return cond if self.caption_norm is None else self.caption_norm(cond)
+        if self.caption_norm is None:
+            return quantize_w8a8(cond)
+        return rms_norm_quantize_w8a8(cond, self.caption_norm.weight, eps=self.caption_norm.eps)[:2]
+
+    def forward(self, latents, caption, timestep, img_hw: tuple[int, int], caption_lens=None, caption_offsets=None):
+        """latents [B, H*W, C_in], caption [B, T, caption_dim], timestep [B].  Captions of their own lengths: ``caption_lens`` (int32 [B]: the
+        first so many of the T states count), or ``caption`` packed [total, caption_dim] with ``caption_offsets`` (int32 [B + 1])."""
+        if caption_lens is not None and caption_offsets is not None:
+            raise ValueError("caption_lens or caption_offsets, not both")
         dt = latents.dtype
         half = 128
         freqs = torch.exp(-math.log(10000.0) * torch.arange(half, device=latents.device, dtype=torch.float32) / half)
@@ -241,10 +274,10 @@ class SanaTransformer(nn.Module):
         temb = self.time_mlp(torch.cat([ang.cos(), ang.sin()], dim=-1).to(dt))
         t6 = self.adaln_single(F.silu(temb))
         x = self.patch_embed(latents)
-        cond = self.caption_proj(caption)
+        cond = self._caption_states(caption)
         H, W = img_hw
         for blk in self.blocks:
-            x = blk(x, cond, t6, H, W)
+            x = blk(x, cond, t6, H, W, caption_lens, caption_offsets)
         sh, sc = (self.final_table[None] + temb[:, None]).unbind(1)
         x = F.layer_norm(x, (self.dim,), eps=1e-6) * (1 + sc.unsqueeze(1)) + sh.unsqueeze(1)
         return self.proj_out(x)
