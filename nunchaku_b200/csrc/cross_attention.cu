@@ -73,9 +73,9 @@ constexpr int CT_TABLE_BYTES = 6 * 1024;            // the samples' ranges or ma
 constexpr int CT_TMEM_COLS = 256;                   // S: 2 x 64, O: 128
 constexpr int CT_WAIT_LOOKS = 1 << 20;              // each of up to a microsecond
 constexpr float CT_RESCALE_STEP = 8.f;
-#ifndef CT_ITEM_COST
-#define CT_ITEM_COST 16
-#endif
+// What it takes to change queries and hand the output over, in tenths of a block of 64 states' time (32 x 20 x 1024 x <=300 x 112 packed:
+// 134 us at 8, 103.5 at 14, 104.5 at 16, 107.5 at 18)
+constexpr int CT_ITEM_COST = 16;
 static_assert(2 * (CT_SMEM + CT_TABLE_BYTES + 1024) <= 228 * 1024 && CT_TABLE_BYTES >= CT_MASK_STATES / 8 + 8, "two CTAs per SM");
 
 struct CrossTileShared {
@@ -164,6 +164,13 @@ struct CrossItems {
 
 // What an item costs, in tenths of a block of 64 states: its blocks, and what it takes to change queries and hand the output over.
 __device__ __forceinline__ float cross_item_cost(int count) { return static_cast<float>(10 * ((count + CT_BN - 1) / CT_BN) + CT_ITEM_COST); }
+
+// largest of three; a NaN stays one (fmaxf drops it)
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 template <bool F16, bool MASK>
 __global__ void __launch_bounds__(CT_THREADS, 2)
@@ -474,14 +481,15 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             return (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
         };
-        auto max32 = [&](const uint32_t (&a)[32]) {
-            float m0 = __uint_as_float(a[0]), m1 = __uint_as_float(a[1]);
+        auto max32 = [&](const uint32_t (&a)[32], float m0) {   // and of m0
+            float m1 = __uint_as_float(a[0]);
 #pragma unroll
-            for (int i = 2; i < 30; i += 4) {
-                m0 = max3(m0, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
-                m1 = max3(m1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
+            for (int i = 1; i < 29; i += 4) {
+                m0 = max3_nan(m0, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
+                m1 = max3_nan(m1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
             }
-            return max3(m0, m1, fmaxf(__uint_as_float(a[30]), __uint_as_float(a[31])));
+            m1 = max3_nan(m1, __uint_as_float(a[29]), __uint_as_float(a[30]));
+            return max3_nan(m0, m1, __uint_as_float(a[31]));
         };
         auto hide = [&](uint32_t (&a)[32], uint32_t bits) {
             if (bits != 0xffffffffu) {
@@ -508,16 +516,17 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 if (two) tc_ld_32x32b_x32(st + 32, a1);
                 tc_wait_ld();
                 hide(a0, MASK ? it.bits(j)[0] : valid >= 32 ? 0xffffffffu : (1u << valid) - 1u);
-                float mx = max32(a0);
+                // (Not below a finite bound: a block of which nothing is to be seen, ahead of others, has only -inf, whose exponentials are 0
+                // whatever the finite maximum.  A score that is NaN makes the maximum and with it the whole row NaN.)
+                float mx = max32(a0, -3e38f);
                 if (two) {
                     hide(a1, MASK ? it.bits(j)[1] : valid >= 64 ? 0xffffffffu : (1u << (valid - 32)) - 1u);
-                    mx = fmaxf(mx, max32(a1));
+                    mx = max32(a1, mx);
                 }
-                // (a block of which nothing is to be seen, ahead of others: its exponentials are of -inf whatever the finite maximum is)
-                const float ms = MASK ? fmaxf(mx * p.scale_log2, -1e30f) : mx * p.scale_log2;
+                const float ms = max3_nan(mx * p.scale_log2, -1e30f, -1e30f);
                 if (j == 0) {
                     m_used = ms;
-                } else if (const bool grow = ms > m_used + CT_RESCALE_STEP; __any_sync(0xffffffffu, grow)) {
+                } else if (const bool grow = !(ms <= m_used + CT_RESCALE_STEP); __any_sync(0xffffffffu, grow)) {
                     // O is written by the previous P V product until it has completed
                     if (!(ok = ct_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, sh, 970))) break;
                     tc_fence_after_sync();
@@ -812,6 +821,7 @@ cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
         atomicExch(&p.status[1], 880 + warp);
     }
+    __syncwarp();   // the producer's lanes among them
     // Every CTA of the cluster has started (its shared memory may be written from here on); the wait is at the joining below.
     if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     __syncthreads();
@@ -991,7 +1001,8 @@ static int launch_cross_rows_dim(const CUtensorMap& tk, const CUtensorMap& tv, c
 extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* stream) {
     using namespace svdq;
     SVDQ_CHECK_ARG(a && a->q && a->k && a->v && a->out, "cross_attention: null tensor pointer");
-    SVDQ_CHECK_ARG(a->batch > 0 && a->heads > 0 && a->kv_heads > 0 && a->q_len > 0 && a->kv_len > 0 && a->batch <= 65535 && a->heads <= 65535,
+    SVDQ_CHECK_ARG(a->batch > 0 && a->heads > 0 && a->kv_heads > 0 && a->q_len > 0 && a->kv_len > 0 && a->batch <= 65535 && a->heads <= 65535 &&
+                       a->q_len <= (1 << 30) && a->kv_len <= (1 << 30),
                    "cross_attention: bad sizes");
     SVDQ_CHECK_ARG(a->heads % a->kv_heads == 0, "cross_attention: kv_heads (%d) must divide heads (%d)", a->kv_heads, a->heads);
     SVDQ_CHECK_ARG(a->head_dim > 0 && a->head_dim <= 128 && a->head_dim % 8 == 0, "cross_attention: head_dim %d (multiples of 8 up to 128)", a->head_dim);

@@ -145,7 +145,7 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         // copies of one issuing warp are worked off one after the other, in about the time a stage's products take)
         const bool wgt = warp & 1;
         const uint32_t turn = warp >> 1, bytes = wgt ? bnh * W8_BK : W8_A_BYTES;
-        uint32_t it = 0;      // W8S_STAGES so far
+        uint32_t it = 0;      // stages so far
         bool ok = true;
         for (int tile = pair; tile < ntiles && ok; tile += npairs) {
             const int row = wgt ? (tile / p.tiles_m) * p.bn + rank * bnh : (tile % p.tiles_m) * (2 * W8_BM) + rank * W8_BM;
@@ -163,6 +163,8 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                 __syncwarp();
             }
         }
+        if (!ok)   // The copies still in flight land on the leader's barriers, whose phases may never complete: wait many times a copy's time.
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     } else if (warp == W8_MMA_WARP && rank == 0) {
         // ------------------------------------------------------------------ MMA issuer
         const uint32_t idesc = idesc_i8(2 * W8_BM, p.bn, true);
@@ -326,7 +328,8 @@ w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
 
     if (warp == 0) {
         if (lane == 0) {
-            for (int i = 0; i < ks1 - ks0; ++i) {
+            int i = 0;
+            for (; i < ks1 - ks0; ++i) {
                 const int s = i % W8S_STAGES;
                 if (!mbar_wait(&sh->empty[s], ((i / W8S_STAGES) & 1) ^ 1, W8_WAIT_CYCLES)) {
                     atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
@@ -338,6 +341,8 @@ w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
                 tma_load_2d(st, &tm_w, &sh->full[s], (ks0 + i) * W8_BK, n0);
                 tma_load_2d(st + W8S_W_BYTES, &tm_t, &sh->full[s], (ks0 + i) * W8_BK, 0);
             }
+            for (int k = i > W8S_STAGES ? i - W8S_STAGES : 0; k < i; ++k)   // leave with none of the copies in flight, whatever the others met
+                mbar_wait(&sh->full[k % W8S_STAGES], (k / W8S_STAGES) & 1, W8_WAIT_CYCLES);
         }
     } else if (warp == 1) {
         constexpr uint32_t idesc = idesc_i8(W8S_BW, W8S_TOKENS, true);
@@ -465,6 +470,7 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args* a, void* stream) {
     using namespace svdq;
     SVDQ_CHECK_ARG(a && a->act && a->wgt && a->ascales && a->wscales && a->out, "gemm_w8a8: null pointer");
     SVDQ_CHECK_ARG(a->M > 0 && a->N > 0 && a->N % 8 == 0, "gemm_w8a8: M (%d) must be positive and N (%d) a positive multiple of 8", a->M, a->N);
+    SVDQ_CHECK_ARG(a->M <= (1 << 30) && a->N <= (1 << 30), "gemm_w8a8: at most 2^30 rows and columns");
     SVDQ_CHECK_ARG(a->K > 0 && a->K % 16 == 0 && a->K <= W8_MAX_K, "gemm_w8a8: K (%d) must be a positive multiple of 16, at most %d", a->K, W8_MAX_K);
     SVDQ_CHECK_ARG(a->dtype == SVDQ_DTYPE_BF16 || a->dtype == SVDQ_DTYPE_FP16, "gemm_w8a8: bad dtype %d", a->dtype);
     SVDQ_CHECK_ARG(a->out_stride >= a->N && a->out_stride % 8 == 0, "gemm_w8a8: the output's row stride must be a multiple of 8, at least N");

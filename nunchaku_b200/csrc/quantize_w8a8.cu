@@ -146,7 +146,8 @@ quantize_w8a8_kernel(const Quant8Params p) {
         // Per-row scalars, which every thread computes: kept to a few instructions (with four full divisions and a root the kernel was
         // bound by them).
         const bool finite = top < __int_as_float(0x7f800000) && ss < __int_as_float(0x7f800000);   // false for NaN
-        const float up = top < 1e-30f ? 1.2676506002282294e30f : 1.0f;   // 2^100 (exact) for a row whose 127 / top would leave fp32
+        // 2^100 or 2^-100 (exact) for a row whose 127 / top would leave fp32, or its reciprocal lose bits
+        const float up = top < 1e-30f ? 1.2676506002282294e30f : top > 1e30f ? 7.888609052210118e-31f : 1.0f;
         const float inv = top > 0.f ? 127.0f * __frcp_rn(top * up) : 0.f;
         // 127 / top to twice the precision: a value of half the row's largest, common among 16-bit inputs, stands exactly on the tie 63.5,
         // and is to be told from its neighbours by the quotient, not by the rounding of the reciprocal
@@ -191,7 +192,8 @@ int quantize_w8a8_impl(const svdq_quantize_w8a8_args* a, void* stream) {
     SVDQ_CHECK_ARG(!a->residual || a->weight, "quantize_w8a8: the residual form needs a norm weight");
     SVDQ_CHECK_ARG(a->x_stride >= a->cols && a->x_stride % 8 == 0 && (!a->residual || (a->residual_stride >= a->cols && a->residual_stride % 8 == 0)),
                    "quantize_w8a8: row strides must be multiples of 8 elements, at least cols");
-    SVDQ_CHECK_ARG(!a->weight || a->eps >= 0.f, "quantize_w8a8: eps must not be negative");
+    // (with less, a row whose squares vanish in fp32 would be divided by zero)
+    SVDQ_CHECK_ARG(!a->weight || a->eps >= 1e-30f, "quantize_w8a8: eps must be at least 1e-30");
     SVDQ_CHECK_ARG(aligned(a->x, 16) && aligned(a->residual, 16) && aligned(a->weight, 16) && aligned(a->hidden, 16) && aligned(a->codes, 16) &&
                        aligned(a->scales, 4),
                    "quantize_w8a8: tensors must be 16-byte aligned");

@@ -121,13 +121,13 @@ class SVDQW4A4Linear(nn.Module):
 
 class W8A8Linear(nn.Module):
     """``y = x W^T + bias`` through :func:`nunchaku_b200.ops.gemm_w8a8`: ``qweight`` int8 [out, in] with ``wscales`` fp32 [out] (the plain
-    row-major order, nothing packed), activations quantised per token.  ``in_features`` a multiple of 16, ``out_features`` of 8."""
+    row-major order, nothing packed), activations quantised per token.  ``in_features`` a multiple of 16 up to 16384, ``out_features`` of 8."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, torch_dtype: torch.dtype = torch.bfloat16,
                  device: str | torch.device | None = None):
         super().__init__()
-        if in_features % 16 or out_features % 8:
-            raise ValueError("in_features must be a multiple of 16 and out_features of 8")
+        if in_features % 16 or in_features > 16384 or out_features % 8:
+            raise ValueError("in_features must be a multiple of 16 up to 16384 and out_features of 8")
         device = torch.device("cpu") if device is None else device
         self.in_features, self.out_features, self.torch_dtype = in_features, out_features, torch_dtype
         self.qweight = nn.Parameter(torch.zeros(out_features, in_features, dtype=torch.int8, device=device), requires_grad=False)

@@ -119,6 +119,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
         raise ValueError("the last dimension of q, k and v must be contiguous")
     if min(B, H, Tq, D, Hk, T) == 0:
         raise ValueError("cross_attention: empty tensors (where no sample has states, k and v still need one row, of any content)")
+    if max(B, H, Tq, T, D) > 2**30:
+        raise ValueError("cross_attention: at most 2**30 samples, heads and tokens")
     ret = out
     if out is None:
         C = H * D

@@ -45,8 +45,8 @@ def _quantize(x, weight, residual, eps):
     shape = x.shape
     cols = shape[-1] if shape else 0
     n = x.numel()
-    if n == 0 or cols % 16:
-        raise ValueError("x must be [..., C] with at least one row and C a positive multiple of 16")
+    if n == 0 or cols % 16 or cols > 2**30:
+        raise ValueError("x must be [..., C] with at least one row and C a positive multiple of 16 (up to 16384)")
     dev = x.device
     if x.is_contiguous():
         rows, x_stride = n // cols, cols
@@ -92,11 +92,11 @@ def rms_norm_quantize_w8a8(x: torch.Tensor, weight: torch.Tensor, residual: torc
 
     x, residual: bf16 or fp16 [..., C] (rows may be strided), weight [C] of the same dtype.  Returns (codes int8 like x, scales fp32
     [...], hidden): hidden = x + residual rounded to x's dtype (the residual stream; fp16 saturates), None without a residual.  The norm
-    works on the fp32 sum.  A row whose sum of squares is not finite has scale NaN (and codes 0)."""
+    works on the fp32 sum.  eps: at least 1e-30.  A row whose sum of squares is not finite has scale NaN (and codes 0)."""
     if weight is None:
         raise ValueError("weight is required (quantize_w8a8 is the form without the norm)")
-    if not eps >= 0:
-        raise ValueError("eps must not be negative")
+    if not eps >= 1e-30:
+        raise ValueError("eps must be at least 1e-30")
     return _quantize(x, weight, residual, eps)
 
 
@@ -108,7 +108,7 @@ def dequantize_w8a8(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.
     if scales.dtype != torch.float32 or scales.device != codes.device or not scales.is_contiguous():
         raise ValueError("scales must be a contiguous fp32 tensor on codes' device")
     cols = codes.shape[-1] if codes.dim() else 0
-    if codes.numel() == 0 or cols % 16 or scales.shape != codes.shape[:-1]:
+    if codes.numel() == 0 or cols % 16 or cols > 2**30 or scales.shape != codes.shape[:-1]:
         raise ValueError("codes must be [..., C] with at least one row and C a positive multiple of 16, scales [...]")
     code = dtype_code(out_dtype)
     out = torch.empty_like(codes, dtype=out_dtype)
@@ -122,7 +122,7 @@ def gemm_w8a8(act: torch.Tensor, wgt: torch.Tensor, ascales: torch.Tensor, wscal
     """``(act @ wgt.T) * ascales[:, None] * wscales (+ bias)`` for int8 ``act`` [..., K] and ``wgt`` [N, K], fp32 ``ascales`` [...] (one
     per token) and ``wscales`` [N].  The integer sum is exact; scales and bias are applied in fp32 with one rounding to the output's type.
 
-    K: a multiple of 16 up to 131056; N: a multiple of 8; any number of rows from one on.  ``out`` [..., N] bf16 / fp16 may be rows of a
+    K: a multiple of 16 up to 131056; N: a multiple of 8; 1 to 2**30 rows.  ``out`` [..., N] bf16 / fp16 may be rows of a
     wider buffer (unit column stride, one row stride that is a multiple of 8); by default a new tensor of ``out_dtype`` (bias's dtype,
     else bf16)."""
     dev = act.device
@@ -149,6 +149,8 @@ def gemm_w8a8(act: torch.Tensor, wgt: torch.Tensor, ascales: torch.Tensor, wscal
     if bias is not None and (bias.shape != (N,) or bias.dtype != dtype or not bias.is_contiguous() or bias.device != dev):
         raise ValueError("bias must be a contiguous [N] of the output's dtype on act's device")
     rows = act.numel() // K
+    if max(rows, N, K) > 2**30:
+        raise ValueError("gemm_w8a8: at most 2**30 rows and columns")
     if out is None:
         out = torch.empty_strided((rows, N), (N, 1), dtype=dtype, device=dev)
         if len(shape) != 2:

@@ -56,6 +56,11 @@ def test_refuses(lib, bad):
     assert _call(lib, **bad) == lib.SVDQ_ERR_INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("big", [dict(q_len=2 ** 30 + 1), dict(kv_len=2 ** 30 + 1), dict(kv_len=2 ** 31 - 1)])
+def test_refuses_more_tokens_than_its_indices_count(lib, big):
+    assert _call(lib, **big) == lib.SVDQ_ERR_INVALID_ARGUMENT
+
+
 def test_refuses_null_and_a_mask_that_is_too_long(lib):
     assert lib.load().svdq_cross_attention(None, None) == lib.SVDQ_ERR_INVALID_ARGUMENT
     assert _call(lib, mask=64, mask_stride=70000, kv_len=32769) == lib.SVDQ_ERR_UNSUPPORTED

@@ -203,6 +203,77 @@ def test_growing_scores_and_large_scale(Tq, H):
     _check(cross_attention(q, k, v, scale=0.5), q, k, v, _keep(B, T), 0.5)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32)])
+def test_a_bad_state_that_is_to_be_seen_is_not_hidden(Tq, H, dtype):
+    """a NaN in one state of K (at every place of a block in turn) or V shows in every row that sees it, and nowhere else"""
+    from nunchaku_b200.ops import cross_attention
+
+    B, T, D = 2, 100, 64
+    for part in (1, 2):
+        for at in range(0, T, 1 if Tq == 3 else 5):
+            qkv = _inputs(B, H, H, Tq, T, D, dtype, seed=at)
+            if at == 0:
+                clean = [cross_attention(*_inputs(B, H, H, Tq, T, D, dtype, seed=s)) for s in range(T)]
+            qkv[part][1, H - 1, at, 7] = float("nan")
+            got = cross_attention(*qkv)
+            bad = got.isnan()
+            assert bad[1, :, (H - 1) * D + 7].all() and (part == 2 or bad[1, :, (H - 1) * D:].all())
+            bad[1, :, (H - 1) * D + 7] = False
+            if part == 1:
+                bad[1, :, (H - 1) * D:] = False
+            assert not bad.any()
+            assert torch.equal(got[0], clean[at][0]) and torch.equal(got[1, :, :(H - 1) * D], clean[at][1, :, :(H - 1) * D])
+
+
+@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32)])
+def test_states_of_minus_infinity(Tq, H):
+    """scores of -inf (whole blocks of them, ahead of others and behind) weigh nothing"""
+    from nunchaku_b200.ops import cross_attention
+
+    B, T, D = 1, 300, 64
+    q, k, v = _inputs(B, H, H, Tq, T, D, torch.bfloat16, seed=3)
+    q = q.abs() + 0.25
+    keep = torch.ones(B, T, dtype=torch.bool)
+    for lo, hi in ((0, 70), (0, 1), (100, 260), (299, 300)):
+        k2 = k.clone()
+        k2[:, :, lo:hi] = -float("inf")
+        keep2 = keep.clone()
+        keep2[:, lo:hi] = False
+        k3 = k.clone()
+        _check(cross_attention(q, k2, v), q, k3, v, keep2, D ** -0.5)
+
+
+def test_two_calls_at_once():
+    """on two streams, each call's result as when alone"""
+    from nunchaku_b200.ops import cross_attention
+
+    cases = [_inputs(2, 4, 4, 1, 900, 112, torch.bfloat16, seed=1), _inputs(2, 20, 20, 300, 300, 112, torch.bfloat16, seed=2),
+             _inputs(2, 20, 20, 300, 300, 112, torch.bfloat16, seed=3)]
+    ref = [cross_attention(*c).clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(cross_attention(*cases[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, r) for i, r in enumerate(ref) for g in got[i])
+
+
+def test_heads_and_samples_of_one_buffer():
+    """q, k, v expanded over samples and heads (stride 0)"""
+    from nunchaku_b200.ops import cross_attention
+
+    for Tq, H in ((2, 4), (140, 32)):
+        q, k, v = _inputs(1, 1, 1, Tq, 130, 72, torch.bfloat16, seed=5)
+        got = cross_attention(q.expand(3, H, -1, -1), k.expand(3, H, -1, -1), v.expand(3, H, -1, -1))
+        one = cross_attention(q.expand(3, H, -1, -1).contiguous(), k.expand(3, H, -1, -1).contiguous(), v.expand(3, H, -1, -1).contiguous())
+        assert torch.equal(got, one)
+        _check(got[:, :, :72], q.expand(3, 1, -1, -1), k.expand(3, 1, -1, -1), v.expand(3, 1, -1, -1), _keep(3, 130), 72 ** -0.5)
+
+
 def test_long_state_lists():
     from nunchaku_b200.ops import cross_attention
 

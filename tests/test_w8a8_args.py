@@ -52,6 +52,21 @@ def test_quantiser_refuses(lib, bad):
     assert lib.load().svdq_quantize_w8a8(ctypes.byref(_q(lib, **bad)), None) == lib.SVDQ_ERR_INVALID_ARGUMENT
 
 
+def test_more_rows_than_an_int_counts_and_an_eps_of_zero(lib):
+    assert lib.load().svdq_quantize_w8a8(ctypes.byref(_q(lib, weight=64, eps=0.0)), None) == lib.SVDQ_ERR_INVALID_ARGUMENT
+    for big in (dict(M=2 ** 30 + 1), dict(N=2 ** 30 + 8, out_stride=2 ** 31)):
+        d = dict(act=64, wgt=64, ascales=64, wscales=64, out=64, out_stride=16, M=1, N=16, K=64)
+        assert lib.load().svdq_gemm_w8a8(ctypes.byref(lib.GemmW8A8Args(**{**d, **big})), None) == lib.SVDQ_ERR_INVALID_ARGUMENT
+
+
+def test_w8a8_linear_refuses_sizes_its_operators_do_not_take():
+    from nunchaku_b200.models import W8A8Linear
+
+    for k, n in ((24, 16), (16400, 16), (32, 12)):
+        with pytest.raises(ValueError):
+            W8A8Linear(k, n)
+
+
 def test_quantiser_refuses_null_and_too_wide(lib):
     assert lib.load().svdq_quantize_w8a8(None, None) == lib.SVDQ_ERR_INVALID_ARGUMENT
     assert lib.load().svdq_quantize_w8a8(ctypes.byref(_q(lib, cols=16400, x_stride=16400)), None) == lib.SVDQ_ERR_UNSUPPORTED

@@ -113,6 +113,37 @@ def test_smallest_and_largest_magnitudes():
     assert codes[0, 3] == 127 and codes.abs().sum() == 127
 
 
+def test_ties_of_rows_up_to_the_largest_numbers():
+    """values of half the row's largest stand on the tie 63.5 exactly: 64 (to even), whatever the row's magnitude"""
+    from nunchaku_b200.ops import quantize_w8a8
+
+    x = torch.zeros(254, 32, dtype=torch.bfloat16)
+    x[:, 5] = torch.tensor([1.0 + k / 128 for k in range(127)] * 2).bfloat16() * torch.tensor([2.0 ** 126] * 127 + [2.0 ** -100] * 127).bfloat16()
+    x[:, 6], x[:, 7] = x[:, 5] / 2, -x[:, 5] / 2
+    codes, scales = quantize_w8a8(x.cuda())
+    assert (codes[:, 5] == 127).all() and (codes[:, 6] == 64).all() and (codes[:, 7] == -64).all() and codes.float().abs().sum() == 254 * 255
+    _check((codes, scales), x)
+
+
+def test_two_calls_at_once():
+    """on two streams, each call's result as when alone"""
+    from nunchaku_b200.ops import gemm_w8a8, quantize_w8a8
+
+    x = [_rand(M, 512, seed=30 + M, dtype=torch.bfloat16).cuda() for M in (3, 700)]
+    w, sw = quantize_w8a8(_rand(264, 512, seed=33, dtype=torch.bfloat16).cuda())
+    step = lambda t: gemm_w8a8(*(lambda c, s: (c, w, s))(*quantize_w8a8(t)), sw)
+    ref = [step(t).clone() for t in x]
+    streams = [torch.cuda.Stream() for _ in x]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(step(x[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, r) for i, r in enumerate(ref) for g in got[i])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(16,), (1, 48), (3, 5, 272), (4000, 2240)])
 def test_dequantize(shape, dtype):
