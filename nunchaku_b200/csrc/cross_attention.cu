@@ -213,6 +213,8 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tmem_alloc(&sh->tmem_base, CT_TMEM_COLS);
         tmem_relinquish();
     }
+    pdl_launch_dependents();
+    pdl_wait();   // nothing above touches global memory
     // the samples' ranges and mask bits
     if constexpr (MASK) {
         for (int b = tid; b < p.batch; b += CT_THREADS) ranges[b] = make_int2(0, 0);
@@ -954,8 +956,17 @@ static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const
     auto kern = cross_tile_kernel<F16, MASK>;
     static std::atomic<uint64_t> attr_done{0};
     if (int rc = ensure_dynamic_smem(kern, CT_SMEM + CT_TABLE_BYTES, attr_done)) return rc;
-    kern<<<grid, CT_THREADS, CT_SMEM + table_bytes, stream>>>(tq, tk, tv, p);
-    SVDQ_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(CT_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = CT_SMEM + table_bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // the prologue may run under the predecessor's tail
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, p));
     return SVDQ_OK;
 }
 
