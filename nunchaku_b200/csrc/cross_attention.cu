@@ -11,24 +11,38 @@
 //
 // Two kernels.
 //
-// cross_tile_kernel (many queries): one CTA owns 128 query rows of one (batch, head) and walks the states in blocks of 128:
-// Q K^T and P V as tcgen05.mma kind::f16 with S, P and O in tensor memory (S: 128 columns, O: 128), as in attention.cu, but
-// sized for short state lists: 98 KB of shared memory and 256 TMEM columns, so that two CTAs share an SM and one's prologue,
-// exponentials and store run under the other's products (with 300 states a CTA only has three blocks; a CTA alone on its
-// SM, as attention.cu's, would spend half its life filling and draining).  One K and one V slot suffice: K is free as soon as
-// its Q K^T is done, a block ahead of the softmax, V is first needed behind it.  The last block's products, loads and
-// exponentials are cut to the states that exist (N of Q K^T and K-steps of P V in sixteens, the rest in halves of 64).
-// Warps 0-3: softmax, one query row per thread; 4: producer; 5: MMA issuer; 6: zeroes rows of V whose state is not to be seen.
+// cross_tile_kernel (many queries): an item is 128 query rows of one (batch, head); its states are walked in blocks of 64 with Q K^T
+// and P V as tcgen05.mma kind::f16, S, P and O in tensor memory and a running maximum per row (O is rescaled only when a maximum has
+// grown by more than 2^8, as in attention.cu).  State lists are short here (a caption has up to 300 states, five blocks), so filling
+// and draining count as much as the loop: CTAs are resident, two to an SM, and each works through a run of items; warps are
+// specialised so that an item's output, the next one's queries and the products of both lie behind one another:
+//   warps 0-3 softmax (one query row per thread), 4-7 output (O / l, through shared memory in whole rows), 8 MMA issuer, 9 producer of
+//   Q and K, 10 producer of V, 11 nothing (registers are re-divided by fours).
+// Two S buffers of 64 columns: a block's Q K^T runs under the previous block's exponentials.  K and V have two slots each.  The last
+// block's products, loads and exponentials are cut to the states that exist (in sixteens, sixteens and 32s).
+// Items lie in the order batch, tile, head: the heads' channels are neighbours in token-major rows, and a row of 224 bytes shares
+// its DRAM bursts with them (one block of states, 32 x 20 x 1024 x 64 x 112: 94 us with tiles innermost, 65 so).  A CTA's run of items
+// is cut from the samples' lengths on the device, so that all runs cost alike.
+// What bounds it: 32 x 20 x 1024 x <=300 x 112, packed, moves 342 MB (52 us at the copy rate) and takes 105 us, 65 us of that for the first
+// block of every item and about 20 for each further one (full lists of 300: 168 us).  Without its stores it takes 17 us less, without its
+// exponentials 5 to 8, without its loads 3 to 7: no single unit, but the chain S -> maximum -> P -> P V -> O -> output, with which two CTAs fill
+// half of the issue slots (53 %), a fifth of the tensor pipe and half of the DRAM's time (states are read again by some of a sample's later
+// tiles, 307 MB against 195).  The code of all roles has to stay small: at 80 KB it ran 30 % slower than at 47, and with the output's loop
+// unrolled (70 KB) it took twice as long.  Tried and no faster: 256 query rows per CTA over the same K and V with a second Q
+// buffer (65 -> 69 and 168 -> 145 us on 64 and 300 states, 105 -> 107 on the packed ones), an issuer warp per product, the output by TMA
+// from Q's buffer (which then comes free late: 51 against 42 us on 64 states of 64 channels), waits without suspension; queries and output
+// first to leave L2 (300 states 5 % faster, 64 states as much slower).
 //
 // cross_rows_kernel (few query rows per stored head: the serving form for single tokens): bound by streaming K and V once.
 // Up to 16 rows (queries x heads that share a stored head) are the M side of mma.sync m16n8k16; four warps take 16 of every 64
-// states each, with their own running maximum; tiles come through a three-stage cp.async ring whose copies write zeros for states that
-// are not to be seen; the states are split over a cluster of up to 8 CTAs and joined through distributed shared memory in one launch.
+// states each, with their own running maximum; a producer warp brings K and V by TMA through a ring of two 64-state stages; the states are
+// split over a cluster of up to 8 CTAs, which push their sums to one another through distributed shared memory and join them in the
+// same launch.  16 x 24 (8 stored) x 1 x <=4096 x 128, lengths as they come: 33 us = 4.95 TB/s (floor 25; the longest sample's CTAs finish
+// last); one token of 20 heads over 300 states: 5.3 us, of which an empty launch takes more than two and the joining one and a half.
 //
 // Every wait is bounded; a role whose wait runs out records SVDQ_ERR_TIMEOUT and leaves its loop.
 #include "attention_common.cuh"
 #include "host_common.h"
-
 
 namespace svdq {
 
@@ -73,8 +87,8 @@ constexpr int CT_TABLE_BYTES = 6 * 1024;            // the samples' ranges or ma
 constexpr int CT_TMEM_COLS = 256;                   // S: 2 x 64, O: 128
 constexpr int CT_WAIT_LOOKS = 1 << 20;              // each of up to a microsecond
 constexpr float CT_RESCALE_STEP = 8.f;
-// What it takes to change queries and hand the output over, in tenths of a block of 64 states' time (32 x 20 x 1024 x <=300 x 112 packed:
-// 134 us at 8, 103.5 at 14, 104.5 at 16, 107.5 at 18)
+// What it takes to change queries and hand the output over, in tenths of a block of 64 states' time (32 x 20 x 1024 x <=300 x 112, packed:
+// 134 us at 8, 112 at 12, 109 at 16, 110 at 20)
 constexpr int CT_ITEM_COST = 16;
 static_assert(2 * (CT_SMEM + CT_TABLE_BYTES + 1024) <= 228 * 1024 && CT_TABLE_BYTES >= CT_MASK_STATES / 8 + 8, "two CTAs per SM");
 
@@ -283,124 +297,124 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #define CT_ITEMS(name) Items name(p, ranges, words, edge[0], edge[1], b_first, h_first, t_first)
 
     if (warp >= 8) {
-    reg_dealloc<CT_REGS_OTHER>();
-    if (warp == CT_MMA_WARP) {
-        // ------------------------------------------------------------------ MMA issuer (the whole warp walks the loop, one elected lane issues)
-        const int ksteps = (p.dim + 15) >> 4;                    // of 16 channels; channels past the head read as zeros
-        const uint32_t idesc_pv = idesc_h16(CT_BM, 0, F16, true) | (static_cast<uint32_t>(ksteps * 2) << 17);
-        const uint64_t qd = smem_desc_sw128(smem_u32(q_s)), kd = smem_desc_sw128(smem_u32(k_s));
-        const uint64_t vd = smem_desc_sw128_mn(smem_u32(v_s), CT_KV_HALF, 1024);
-        const uint32_t hi_k = static_cast<uint32_t>(qd >> 32), hi_v = static_cast<uint32_t>(vd >> 32);
-        const uint32_t q_lo = static_cast<uint32_t>(qd), k_lo = static_cast<uint32_t>(kd), v_lo = static_cast<uint32_t>(vd);
-        // Two walks over the blocks: `s` for Q K^T, up to one block ahead inside an item, and `o` for P V.  (Each product is issued at
-        // one place: the kernel's code has to stay in the instruction caches with five roles at work.)
-        CT_ITEMS(s);
-        CT_ITEMS(o);
-        int sj = 0, oj = 0;
-        uint32_t m = 0, n = 0, s_items = 0, o_items = 0, plain = 0;   // blocks and items so far; plain: phase bit of v_full per slot
-        bool s_there = true;
-        while (true) {
-            if (sj == s.blocks && s_there) {
-                sj = 0;
-                s_there = s.advance();
-            }
-            if (oj == o.blocks) {
-                oj = 0;
-                if (!o.advance()) break;
-                ++o_items;
-            }
-            // S = Q K_j^T over the block's states, rounded up to 16: now if no scores are left to work on, ahead of P V if K has landed
-            const bool landed = s_there && m == n + 1 && s.item == o.item && __all_sync(0xffffffffu, mbar_test_wait(&sh->k_full[m & 1], (m >> 1) & 1));
-            if (landed || (s_there && m == n)) {
-                if (sj == 0 && !ct_wait(&sh->q_full, s_items++ & 1, sh, 910)) break;
-                if (!landed && !ct_wait(&sh->k_full[m & 1], (m >> 1) & 1, sh, 911)) break;
+        reg_dealloc<CT_REGS_OTHER>();
+        if (warp == CT_MMA_WARP) {
+            // ------------------------------------------------------------------ MMA issuer (the whole warp walks the loop, one elected lane issues)
+            const int ksteps = (p.dim + 15) >> 4;                    // of 16 channels; channels past the head read as zeros
+            const uint32_t idesc_pv = idesc_h16(CT_BM, 0, F16, true) | (static_cast<uint32_t>(ksteps * 2) << 17);
+            const uint64_t qd = smem_desc_sw128(smem_u32(q_s)), kd = smem_desc_sw128(smem_u32(k_s));
+            const uint64_t vd = smem_desc_sw128_mn(smem_u32(v_s), CT_KV_HALF, 1024);
+            const uint32_t hi_k = static_cast<uint32_t>(qd >> 32), hi_v = static_cast<uint32_t>(vd >> 32);
+            const uint32_t q_lo = static_cast<uint32_t>(qd), k_lo = static_cast<uint32_t>(kd), v_lo = static_cast<uint32_t>(vd);
+            // Two walks over the blocks: `s` for Q K^T, up to one block ahead inside an item, and `o` for P V.  (Each product is issued at
+            // one place: the kernel's code has to stay in the instruction caches with five roles at work.)
+            CT_ITEMS(s);
+            CT_ITEMS(o);
+            int sj = 0, oj = 0;
+            uint32_t m = 0, n = 0, s_items = 0, o_items = 0, plain = 0;   // blocks and items so far; plain: phase bit of v_full per slot
+            bool s_there = true;
+            while (true) {
+                if (sj == s.blocks && s_there) {
+                    sj = 0;
+                    s_there = s.advance();
+                }
+                if (oj == o.blocks) {
+                    oj = 0;
+                    if (!o.advance()) break;
+                    ++o_items;
+                }
+                // S = Q K_j^T over the block's states, rounded up to 16: now if no scores are left to work on, ahead of P V if K has landed
+                const bool landed = s_there && m == n + 1 && s.item == o.item && __all_sync(0xffffffffu, mbar_test_wait(&sh->k_full[m & 1], (m >> 1) & 1));
+                if (landed || (s_there && m == n)) {
+                    if (sj == 0 && !ct_wait(&sh->q_full, s_items++ & 1, sh, 910)) break;
+                    if (!landed && !ct_wait(&sh->k_full[m & 1], (m >> 1) & 1, sh, 911)) break;
+                    tc_fence_after_sync();
+                    const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((s.valid(sj) + 15) >> 4) << 18);
+                    const uint32_t d = tmem + (m & 1) * CT_BN, k0 = k_lo + (m & 1) * (CT_KV_BYTES >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk)
+                            if (kk < ksteps)
+                                tc_mma_f16_lo(d, q_lo + (kk >> 2) * (CT_Q_HALF >> 4) + (kk & 3) * 2, k0 + (kk >> 2) * (CT_KV_HALF >> 4) + (kk & 3) * 2, hi_k,
+                                              idesc, kk > 0);
+                        tc_commit(&sh->s_full[m & 1]);
+                    }
+                    __syncwarp();
+                    ++m;
+                    ++sj;
+                    if (m == n + 1) continue;   // look for one more
+                }
+                const uint32_t slot = n & 1;
+                if (oj == 0 && o_items > 1 && !ct_wait(&sh->o_free, o_items & 1, sh, 915)) break;   // the previous item's O has been read
+                if (!o.holes(oj)) {   // otherwise P is only handed over behind it
+                    if (!ct_wait(&sh->v_full[slot], (plain >> slot) & 1, sh, 920)) break;
+                    plain ^= 1u << slot;
+                }
+                if (!ct_wait(&sh->p_full[slot], (n >> 1) & 1, sh, 930)) break;
                 tc_fence_after_sync();
-                const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((s.valid(sj) + 15) >> 4) << 18);
-                const uint32_t d = tmem + (m & 1) * CT_BN, k0 = k_lo + (m & 1) * (CT_KV_BYTES >> 4);
+                const int steps = (o.valid(oj) + 15) >> 4;
+                const uint32_t a = tmem + slot * CT_BN, v0 = v_lo + slot * (CT_KV_BYTES >> 4);
                 if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        if (kk < ksteps)
-                            tc_mma_f16_lo(d, q_lo + (kk >> 2) * (CT_Q_HALF >> 4) + (kk & 3) * 2, k0 + (kk >> 2) * (CT_KV_HALF >> 4) + (kk & 3) * 2, hi_k,
-                                          idesc, kk > 0);
-                    tc_commit(&sh->s_full[m & 1]);
+                    for (int k4 = 0; k4 < 4; ++k4)
+                        if (k4 < steps) tc_mma_f16_ts_lo(tmem + 2 * CT_BN, a + k4 * 8, v0 + k4 * 128, hi_v, idesc_pv, (oj | k4) ? 1u : 0u);
+                    tc_commit(&sh->pv_done[slot]);
                 }
                 __syncwarp();
-                ++m;
-                ++sj;
-                if (m == n + 1) continue;   // look for one more
+                ++n;
+                ++oj;
             }
-            const uint32_t slot = n & 1;
-            if (oj == 0 && o_items > 1 && !ct_wait(&sh->o_free, o_items & 1, sh, 915)) break;   // the previous item's O has been read
-            if (!o.holes(oj)) {   // otherwise P is only handed over behind it
-                if (!ct_wait(&sh->v_full[slot], (plain >> slot) & 1, sh, 920)) break;
-                plain ^= 1u << slot;
+        } else if (warp == CT_QK_WARP || warp == CT_V_WARP) {
+            // ------------------------------------------------------------------ producers: one warp for Q and K, one for V (the copies of one issuing
+            // warp are worked off one after the other)
+            const bool v_warp = warp == CT_V_WARP;
+            const CUtensorMap* map = v_warp ? &tm_v : &tm_k;
+            uint64_t* free_bar = v_warp ? sh->pv_done : sh->s_full;
+            CT_ITEMS(it);
+            uint32_t n = 0, items = 0;
+            uint32_t used = 0, phase = 0;   // per slot and kind of V block (bit 2 * slot + holes): any copy yet, and the next one's phase bit
+            auto full_of = [&](int slot, int holes) { return (!v_warp ? sh->k_full : holes ? sh->vh_full : sh->v_full) + slot; };
+            bool ok = true;
+            while (ok && it.advance()) {
+                const int kv_head = it.head / p.group;
+                if (!v_warp) {
+                    // block n - 1 was the previous item's last
+                    if (n > 0 && !ct_wait(&sh->s_full[(n - 1) & 1], ((n - 1) >> 1) & 1, sh, 900)) break;
+                    ++items;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh->q_full, halves * CT_Q_HALF);
+#pragma unroll 1
+                        for (int h = 0; h < halves; ++h)
+                            tma_load_4d(q_s + h * CT_Q_HALF, &tm_q, &sh->q_full, h * 64, it.tile * CT_BM, it.head * p.q_hmul, it.batch * p.q_bmul);
+                    }
+                    __syncwarp();
+                }
+                const int z = kv_head * (v_warp ? p.v_hmul : p.k_hmul), w = p.st.kv_offsets ? 0 : it.batch * (v_warp ? p.v_bmul : p.k_bmul);
+                for (int j = 0; j < it.blocks; ++j, ++n) {
+                    const int slot = n & 1;
+                    if (n > 1 && !ct_wait(free_bar + slot, ((n - 2) >> 1) & 1, sh, 901 + v_warp)) {
+                        ok = false;
+                        break;
+                    }
+                    const int holes = v_warp && it.holes(j);
+                    used |= 1u << (2 * slot + holes);
+                    phase ^= 1u << (2 * slot + holes);
+                    if (lane == 0) {
+                        uint64_t* full = full_of(slot, holes);
+                        uint8_t* to = (v_warp ? v_s : k_s) + slot * CT_KV_BYTES;
+                        mbar_arrive_expect_tx(full, halves * CT_KV_HALF);
+#pragma unroll 1
+                        for (int h = 0; h < halves; ++h) tma_load_4d(to + h * CT_KV_HALF, map, full, h * 64, it.start + j * CT_BN, z, w);
+                    }
+                    __syncwarp();
+                }
             }
-            if (!ct_wait(&sh->p_full[slot], (n >> 1) & 1, sh, 930)) break;
-            tc_fence_after_sync();
-            const int steps = (o.valid(oj) + 15) >> 4;
-            const uint32_t a = tmem + slot * CT_BN, v0 = v_lo + slot * (CT_KV_BYTES >> 4);
-            if (elect_one()) {
-#pragma unroll
-                for (int k4 = 0; k4 < 4; ++k4)
-                    if (k4 < steps) tc_mma_f16_ts_lo(tmem + 2 * CT_BN, a + k4 * 8, v0 + k4 * 128, hi_v, idesc_pv, (oj | k4) ? 1u : 0u);
-                tc_commit(&sh->pv_done[slot]);
-            }
-            __syncwarp();
-            ++n;
-            ++oj;
+            // leave with none of this warp's copies in flight (where all went well they have all been waited for)
+            if (items) ct_wait(&sh->q_full, (items & 1) ^ 1, sh, 903);
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i)
+                if ((used >> i) & 1u) ct_wait(full_of(i >> 1, i & 1), ((phase >> i) & 1u) ^ 1u, sh, 904);
         }
-    } else if (warp == CT_QK_WARP || warp == CT_V_WARP) {
-        // ------------------------------------------------------------------ producers: one warp for Q and K, one for V (the copies of one issuing
-        // warp are worked off one after the other)
-        const bool v_warp = warp == CT_V_WARP;
-        const CUtensorMap* map = v_warp ? &tm_v : &tm_k;
-        uint64_t* free_bar = v_warp ? sh->pv_done : sh->s_full;
-        CT_ITEMS(it);
-        uint32_t n = 0, items = 0;
-        uint32_t used = 0, phase = 0;   // per slot and kind of V block (bit 2 * slot + holes): any copy yet, and the next one's phase bit
-        auto full_of = [&](int slot, int holes) { return (!v_warp ? sh->k_full : holes ? sh->vh_full : sh->v_full) + slot; };
-        bool ok = true;
-        while (ok && it.advance()) {
-            const int kv_head = it.head / p.group;
-            if (!v_warp) {
-                // block n - 1 was the previous item's last
-                if (n > 0 && !ct_wait(&sh->s_full[(n - 1) & 1], ((n - 1) >> 1) & 1, sh, 900)) break;
-                ++items;
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&sh->q_full, halves * CT_Q_HALF);
-#pragma unroll 1
-                    for (int h = 0; h < halves; ++h)
-                        tma_load_4d(q_s + h * CT_Q_HALF, &tm_q, &sh->q_full, h * 64, it.tile * CT_BM, it.head * p.q_hmul, it.batch * p.q_bmul);
-                }
-                __syncwarp();
-            }
-            const int z = kv_head * (v_warp ? p.v_hmul : p.k_hmul), w = p.st.kv_offsets ? 0 : it.batch * (v_warp ? p.v_bmul : p.k_bmul);
-            for (int j = 0; j < it.blocks; ++j, ++n) {
-                const int slot = n & 1;
-                if (n > 1 && !ct_wait(free_bar + slot, ((n - 2) >> 1) & 1, sh, 901 + v_warp)) {
-                    ok = false;
-                    break;
-                }
-                const int holes = v_warp && it.holes(j);
-                used |= 1u << (2 * slot + holes);
-                phase ^= 1u << (2 * slot + holes);
-                if (lane == 0) {
-                    uint64_t* full = full_of(slot, holes);
-                    uint8_t* to = (v_warp ? v_s : k_s) + slot * CT_KV_BYTES;
-                    mbar_arrive_expect_tx(full, halves * CT_KV_HALF);
-#pragma unroll 1
-                    for (int h = 0; h < halves; ++h) tma_load_4d(to + h * CT_KV_HALF, map, full, h * 64, it.start + j * CT_BN, z, w);
-                }
-                __syncwarp();
-            }
-        }
-        // leave with none of this warp's copies in flight (where all went well they have all been waited for)
-        if (items) ct_wait(&sh->q_full, (items & 1) ^ 1, sh, 903);
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i)
-            if ((used >> i) & 1u) ct_wait(full_of(i >> 1, i & 1), ((phase >> i) & 1u) ^ 1u, sh, 904);
-    }
     } else if (warp >= 4) {
         reg_dealloc<CT_REGS_OUTPUT>();
         // ------------------------------------------------------------------ output: O / l -> global memory, while the softmax warps are at the
@@ -442,8 +456,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 for (int u = 0; u < 4; ++u) {
                     uint32_t w4[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                    {
+                    for (int e = 0; e < 4; ++e) {
                         const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[u * 8 + 2 * e]), __uint_as_float(o[u * 8 + 2 * e + 1])), make_float2(inv, inv));
                         w4[e] = pack_h16<F16>(v.x, v.y);
                     }
