@@ -20,7 +20,7 @@
 // w8a8_skinny_kernel (few tokens, the serving form): there every weight is used for a handful of rows and the kernel streams
 // weights.  The operands change places: 128 weight rows are the M side of the product, up to 16 tokens its N side, and K is split
 // over a cluster of up to 8 CTAs to fill the SMs.  The int32 partial sums are exchanged through distributed shared memory (integers: the order
-// does not matter).  Bound by the weights' bytes and, at these sizes, by launch and latency: 8 x 13440 x 2240 7.4 us = 4.1 TB/s (floor 4.6).
+// does not matter).  Bound by the weights' bytes and, at these sizes, by launch and latency: 8 x 13440 x 2240 8 to 9 us = 3.6 TB/s (floor 4.6).
 //
 // Every wait is bounded; a role whose wait runs out records SVDQ_ERR_TIMEOUT and leaves its loop.
 #include <cuda_bf16.h>
@@ -499,7 +499,10 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args* a, void* stream) {
     const int kstages = (a->K + W8_BK - 1) / W8_BK;
     CUtensorMap ta, tb;
     if (a->M <= W8S_TOKENS) {
-        // K over as many CTAs as give every SM one (more cost more in joining than they bring)
+        // Few tokens: against the other kernel 9.0 to 12.0 us on 8 x 13440 x 2240 and 7.7 to 15.6 on 16 x 4096 x 4096; with 64 tokens in steps
+        // of 16 it took 26 us on 64 x 4480 x 2240, the other 7.4.
+        // K over as many CTAs as give every SM one (16 x 4096 x 4096: 11.4 us unsplit, 7.7 so); more cost more in joining than they bring
+        // (8 x 13440 x 2240: 19.5 us with up to four per SM, 9.0 so)
         const int tiles = (a->N + W8S_BW - 1) / W8S_BW;
         int split = 1;
         while (split < W8S_MAX_SPLIT && tiles * split < sms && 2 * split <= kstages) split *= 2;
@@ -509,8 +512,8 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args* a, void* stream) {
     }
     const int max_pairs = sms / 2;
     p.tiles_m = (a->M + 2 * W8_BM - 1) / (2 * W8_BM);
-    // tile width: the one whose rounds over the pairs take the least, a round costing its width plus a fixed part (64 x 4480 x 2240: 7.4 us with the
-    // 64 columns that this takes, 26 with 256; 8192 x 4096 x 4096: 87 us with 256, where 64 would load twice the bytes per product)
+    // tile width: the one whose rounds over the pairs take the least, a round costing its width plus a fixed part
+    // (always 256 / always 64 / this, us: 32 x 4096 x 4096 13.4 / 9.8 / 9.8; 2147 x 4480 x 2240 25.9 / 36.4 / 21.7; 8192 x 4096 x 4096 88 / 183 / 88)
     long long best = -1;
     for (int bn = W8_BN_MAX; bn >= 64; bn -= 32) {
         const long long tiles = static_cast<long long>(p.tiles_m) * ((a->N + bn - 1) / bn);
