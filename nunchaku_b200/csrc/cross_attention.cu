@@ -35,9 +35,9 @@
 //
 // cross_rows_kernel (few query rows per stored head: the serving form for single tokens): bound by streaming K and V once.
 // Up to 16 rows (queries x heads that share a stored head) are the M side of mma.sync m16n8k16; four warps take 16 of every 64
-// states each, with their own running maximum; a producer warp brings K and V by TMA through a ring of two 64-state stages; the states are
-// split over a cluster of up to 8 CTAs, which push their sums to one another through distributed shared memory and join them in the
-// same launch.  16 x 24 (8 stored) x 1 x <=4096 x 128, lengths as they come: 33 us = 4.95 TB/s (floor 25; the longest sample's CTAs finish
+// states each, with their own running maximum; a producer warp brings K and V by TMA through a ring of two or three 64-state stages; the states are
+// split over a cluster of up to 16 CTAs, which push their sums to one another through distributed shared memory and join them in the
+// same launch.  16 x 24 (8 stored) x 1 x <=4096 x 128, lengths as they come: 31 us = 5.3 TB/s (floor 25; the longest sample's CTAs finish
 // last); one token of 20 heads over 300 states: 5.3 us, of which an empty launch takes more than two and the joining one and a half.
 //
 // Every wait is bounded; a role whose wait runs out records SVDQ_ERR_TIMEOUT and leaves its loop.
@@ -607,9 +607,8 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 }
 
 // ---------------------------------------------------------------------------------------------------------------- few query rows
-constexpr int CR_WARPS = 4, CR_THREADS = 32 * (CR_WARPS + 1), CR_KEYS = 16, CR_ROWS = 16, CR_MAX_SPLIT = 8;
+constexpr int CR_WARPS = 4, CR_THREADS = 32 * (CR_WARPS + 1), CR_KEYS = 16, CR_ROWS = 16, CR_MAX_SPLIT = 16;
 constexpr int CR_TILE = CR_WARPS * CR_KEYS;          // states of a tile: 16 per warp
-constexpr int CR_STAGES = 2;
 constexpr long long CR_WAIT_CYCLES = 600000000ll;   // ~0.3 s
 constexpr int CR_HALF_BYTES = CR_TILE * 128;         // 64 states x 64 channels
 
@@ -628,11 +627,16 @@ struct CrossRowsParams {
 // [16, 24 over 8, 1 over <= 4096, 128])
 __host__ __device__ constexpr int cross_rows_per_sm(int nk) { return nk > 7 ? 2 : nk > 4 ? 3 : nk > 2 ? 4 : 6; }
 
+// stages of the ring: as many as the shared memory of that many CTAs takes (a third at 128 channels: 33 -> 31 us on the case above; full lists of
+// 4096 go from 42 to 44)
+__host__ __device__ constexpr int cross_rows_stages(int nk) { return nk > 7 ? 3 : nk > 4 ? 2 : nk > 2 ? 3 : 2; }
+
 template <int NK>
 struct CrossRowsSizes {
+    static constexpr int STAGES = cross_rows_stages(NK);
     static constexpr int HALVES = NK > 4 ? 2 : 1;
     static constexpr int STAGE = 2 * HALVES * CR_HALF_BYTES;    // K and V
-    static constexpr int RING = CR_STAGES * STAGE;
+    static constexpr int RING = STAGES * STAGE;
     static constexpr int COLS = NK * 16;
     // afterwards over the ring: the warps' partial sums [4][16][COLS], maxima and sums [4][16] each
     static_assert(RING >= CR_WARPS * CR_ROWS * (COLS + 2) * 4, "the partial sums lie over the ring");
@@ -669,14 +673,14 @@ cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     extern __shared__ __align__(1024) uint8_t cr_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cr_smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::RING);
-    uint64_t* empty = full + CR_STAGES;
+    uint64_t* empty = full + S::STAGES;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int split = 1 << log_split, rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
     const int pairix = blockIdx.x >> log_split, batch = pairix / p.kv_heads, kv_head = pairix % p.kv_heads;
     const int r0 = blockIdx.y * CR_ROWS, rows = min(CR_ROWS, p.q_rows - r0);
     if (tid == 0) {
 #pragma unroll
-        for (int i = 0; i < CR_STAGES; ++i) {
+        for (int i = 0; i < S::STAGES; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], CR_WARPS);
         }
@@ -701,8 +705,8 @@ cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             int i = 0;
 #pragma unroll 1
             for (int tile = t0; tile < t1; ++tile, ++i) {
-                const int s = i % CR_STAGES;
-                if (!mbar_wait(&empty[s], ((i / CR_STAGES) & 1) ^ 1, CR_WAIT_CYCLES)) {
+                const int s = i % S::STAGES;
+                if (!mbar_wait(&empty[s], ((i / S::STAGES) & 1) ^ 1, CR_WAIT_CYCLES)) {
                     ok = false;
                     break;
                 }
@@ -716,7 +720,7 @@ cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
                 }
             }
             if (!ok)   // leave with none of the copies in flight
-                for (int k = i > CR_STAGES ? i - CR_STAGES : 0; k < i; ++k) mbar_wait(&full[k % CR_STAGES], (k / CR_STAGES) & 1, CR_WAIT_CYCLES);
+                for (int k = i > S::STAGES ? i - S::STAGES : 0; k < i; ++k) mbar_wait(&full[k % S::STAGES], (k / S::STAGES) & 1, CR_WAIT_CYCLES);
         }
     } else {
         // ------------------------------------------------------------------ consumers
@@ -758,10 +762,10 @@ cross_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         uint32_t next_bits = t0 < t1 ? visible(t0) : 0u;
 #pragma unroll 1
         for (int tile = t0; tile < t1; ++tile) {
-            const int i = tile - t0, slot = i % CR_STAGES;
+            const int i = tile - t0, slot = i % S::STAGES;
             const uint32_t bits = next_bits;
             if (tile + 1 < t1) next_bits = visible(tile + 1);
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (i / CR_STAGES) & 1, CR_WAIT_CYCLES)))) break;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (i / S::STAGES) & 1, CR_WAIT_CYCLES)))) break;
             if (bits) {
                 const uint32_t ks = base + slot * S::STAGE, vs = ks + S::HALVES * CR_HALF_BYTES;
                 float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -987,7 +991,7 @@ template <bool F16, int NK>
 static int launch_cross_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CrossRowsParams& p, int pairs, int split, cudaStream_t stream) {
     auto kern = cross_rows_kernel<F16, NK>;
     static std::atomic<uint64_t> attr_done{0};
-    if (int rc = ensure_dynamic_smem(kern, CrossRowsSizes<NK>::smem(CR_ROWS, CR_MAX_SPLIT), attr_done)) return rc;
+    if (int rc = ensure_dynamic_smem(kern, CrossRowsSizes<NK>::smem(CR_ROWS, CR_MAX_SPLIT), attr_done, true)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(pairs * split, (p.q_rows + CR_ROWS - 1) / CR_ROWS, 1);
     cfg.blockDim = dim3(CR_THREADS, 1, 1);
@@ -1073,7 +1077,10 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
     // 43 us with 256 CTAs, 47 with 512, 57 with 1024).
     const long long resident = static_cast<long long>(sms) * cross_rows_per_sm((a->head_dim + 15) / 16);
     int split = 1;
-    while (split < CR_MAX_SPLIT && ctas * split * 2 <= resident && 2 * split <= tiles) split *= 2;
+    while (split < 8 && ctas * split * 2 <= resident && 2 * split <= tiles) split *= 2;
+    // 16 where every CTA still has four tiles (1 x 24 heads (8 stored) x 30000 x 128: 38.5 -> 29 us, 1 x 20 x 4096 x 112: 13 -> 11.5; with one
+    // tile each 1 x 24 x 1200 x 64 goes from 6.6 to 8.7).  Such clusters fit a GPC's SMs less well: three quarters of the places are counted on.
+    if (split == 8 && ctas * 16 <= resident * 3 / 4 && tiles >= 4 * 16) split = 16;
     const long long q_items = static_cast<long long>(a->batch) * a->heads * ((a->q_len + CT_BM - 1) / CT_BM);
     const double rows_alone = 0.65 * static_cast<double>((tiles + split - 1) / split),
                  rows_shared = (a->head_dim > 64 ? 0.53 : 0.26) * static_cast<double>(ctas) * static_cast<double>(tiles) / sms;

@@ -57,7 +57,7 @@ int current_device(int* dev);
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per (kernel, device): `done` is a function-local static
 // bit mask, one bit per device ordinal, guarded by one mutex for all kernels (set-up only happens a few times).
 template <typename Kernel>
-inline int ensure_dynamic_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+inline int ensure_dynamic_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done, bool large_clusters = false) {
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
     const uint64_t bit = 1ull << dev;
@@ -67,6 +67,10 @@ inline int ensure_dynamic_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t
     if (done.load(std::memory_order_relaxed) & bit) return SVDQ_OK;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (e != cudaSuccess) return fail(SVDQ_ERR_CUDA, "cudaFuncSetAttribute(max dynamic shared memory = %zu) failed: %s", bytes, cudaGetErrorString(e));
+    if (large_clusters) {   // more than 8 CTAs
+        const cudaError_t c = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (c != cudaSuccess) return fail(SVDQ_ERR_CUDA, "cudaFuncSetAttribute(non-portable cluster size) failed: %s", cudaGetErrorString(c));
+    }
     done.fetch_or(bit, std::memory_order_release);
     return SVDQ_OK;
 }
