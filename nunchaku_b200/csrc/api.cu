@@ -142,7 +142,7 @@ static int cached_tmap(CUtensorMap* out, const TmapKey& k) {
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r = fn(&e.map, static_cast<CUtensorMapDataType>(k.elem), static_cast<cuuint32_t>(k.rank), const_cast<void*>(k.base),
                           k.dims, k.strides, k.box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          k.swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          k.swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : k.swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         e.valid = false;
@@ -163,7 +163,7 @@ int make_tmap_2d(CUtensorMap* map, const void* base, int elem, uint64_t inner, u
     k.dims[0] = inner; k.dims[1] = rows;
     k.strides[0] = row_bytes;
     k.box[0] = box_inner; k.box[1] = box_rows;
-    k.elem = elem; k.rank = 2; k.swizzle = swizzle128 ? 1 : 0;
+    k.elem = elem; k.rank = 2; k.swizzle = swizzle128 ? 128 : 0;
     return cached_tmap(map, k);
 }
 
@@ -182,7 +182,7 @@ int make_tmap_3d(CUtensorMap* map, const void* base, int elem, uint64_t d0, uint
 }
 
 int make_tmap_nd(CUtensorMap* map, const void* base, int elem, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                 const uint32_t* box, bool swizzle128) {
+                 const uint32_t* box, int swizzle) {
     SVDQ_CHECK_ARG(rank >= 2 && rank <= 4 && aligned(base, 16), "tensor map: rank 2..4 and a 16-byte aligned base");
     TmapKey k;
     std::memset(&k, 0, sizeof(k));
@@ -195,7 +195,7 @@ int make_tmap_nd(CUtensorMap* map, const void* base, int elem, int rank, const u
             k.strides[i] = strides_bytes[i];
         }
     }
-    k.elem = elem; k.rank = rank; k.swizzle = swizzle128 ? 1 : 0;
+    k.elem = elem; k.rank = rank; k.swizzle = swizzle;
     return cached_tmap(map, k);
 }
 

@@ -465,7 +465,7 @@ static int attn_tmap(CUtensorMap* map, const void* base, int dtype, int batch, i
                                  static_cast<uint64_t>(batch > 1 ? stride[0] : stride[1]) * 2};
     const uint32_t box[4] = {64, AT_BN, 1, 1};
     return make_tmap_nd(map, base, dtype == SVDQ_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                        dims, strides, box, true);
+                        dims, strides, box, 128);
 }
 
 template <bool F16>

@@ -16,7 +16,7 @@
 // grown by more than 2^8, as in attention.cu).  State lists are short here (a caption has up to 300 states, five blocks), so filling
 // and draining count as much as the loop: CTAs are resident, two to an SM, and each works through a run of items; warps are
 // specialised so that an item's output, the next one's queries and the products of both lie behind one another:
-//   warps 0-3 softmax (one query row per thread), 4-7 output (O / l, through shared memory in whole rows), 8 MMA issuer, 9 producer of
+//   warps 0-3 softmax (one query row per thread), 4-7 output (O / l, through shared memory and on by TMA), 8 MMA issuer, 9 producer of
 //   Q and K, 10 producer of V, 11 nothing (registers are re-divided by fours).
 // Two S buffers of 64 columns: a block's Q K^T runs under the previous block's exponentials.  K and V have two slots each.  The last
 // block's products, loads and exponentials are cut to the states that exist (in sixteens, sixteens and 32s).
@@ -25,12 +25,13 @@
 // is cut from the samples' lengths on the device, so that all runs cost alike.
 // What bounds it: 32 x 20 x 1024 x <=300 x 112, packed, moves 342 MB (52 us at the copy rate) and takes 105 us, 65 us of that for the first
 // block of every item and about 20 for each further one (full lists of 300: 168 us).  Without its stores it takes 17 us less, without its
-// exponentials 5 to 8, without its loads 3 to 7: no single unit, but the chain S -> maximum -> P -> P V -> O -> output, with which two CTAs fill
+// exponentials 5 to 8, without its loads 3 to 7: no single unit (a quarter of the exponentials on the FMA pipe, as in attention.cu, gains
+// nothing here and costs 5 % over 4096 states), but the chain S -> maximum -> P -> P V -> O -> output, with which two CTAs fill
 // half of the issue slots (53 %), a fifth of the tensor pipe and half of the DRAM's time (states are read again by some of a sample's later
 // tiles, 307 MB against 195).  The code of all roles has to stay small: at 80 KB it ran 30 % slower than at 47, and with the output's loop
 // unrolled (70 KB) it took twice as long.  Tried and no faster: 256 query rows per CTA over the same K and V with a second Q
-// buffer (65 -> 69 and 168 -> 145 us on 64 and 300 states, 105 -> 107 on the packed ones), an issuer warp per product, the output by TMA
-// from Q's buffer (which then comes free late: 51 against 42 us on 64 states of 64 channels), waits without suspension; queries and output
+// buffer (65 -> 69 and 168 -> 145 us on 64 and 300 states, 105 -> 107 on the packed ones), an issuer warp per product, two threads per row (105 ->
+// 117), the output out of Q's buffer (which then comes free late: 51 against 42 us on 64 states of 64 channels), waits without suspension; queries and output
 // first to leave L2 (300 states 5 % faster, 64 states as much slower).
 //
 // cross_rows_kernel (few query rows per stored head: the serving form for single tokens): bound by streaming K and V once.
@@ -105,11 +106,9 @@ static_assert(sizeof(CrossTileShared) <= CT_BAR_BYTES, "barrier block");
 
 struct CrossTileParams {
     CrossStates st;
-    uint8_t* out;
-    long long os[3];                                      // batch, head, token strides in bytes
     int q_len, dim, group, heads, q_tiles, items, batch;  // item = (batch * q_tiles + tile) * heads + head
     int mask_words;                                       // 32-bit words of mask bits per sample
-    int q_bmul, q_hmul, k_bmul, k_hmul, v_bmul, v_hmul;   // 0 where that dimension is broadcast (stride 0): its coordinate is then 0
+    int q_bmul, q_hmul, k_bmul, k_hmul, v_bmul, v_hmul, o_bmul, o_hmul;   // 0 where that dimension is broadcast (stride 0): its coordinate is then 0
     float scale_log2;
     int* status;
 };
@@ -189,7 +188,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 template <bool F16, bool MASK>
 __global__ void __launch_bounds__(CT_THREADS, 2)
 cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const __grid_constant__ CrossTileParams p) {
+                  const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ CrossTileParams p) {
     extern __shared__ __align__(1024) uint8_t ct_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ct_smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_s = smem;
@@ -222,6 +221,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
+        prefetch_tmap(&tm_o);
     }
     if (warp == CT_MMA_WARP) {
         tmem_alloc(&sh->tmem_base, CT_TMEM_COLS);
@@ -427,7 +427,6 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         while (it.template advance<true>()) {
             n += it.blocks;
             const int row0 = it.tile * CT_BM + quad * 32;
-            uint8_t* out = p.out + it.batch * p.os[0] + it.head * p.os[1] + row0 * p.os[2];
             float inv = 0.f;
             if (it.blocks) {
                 const uint32_t last = n - 1;
@@ -451,27 +450,29 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0u;   // no states: zeros
                 }
-                // through shared memory, so that a store instruction covers eight rows' 64 bytes and not 32 rows' 16 (L1 takes one line a cycle)
+                // into a box of 32 rows x 32 channels (64-byte swizzle) and on by TMA (with stores of the warps' own 1 to 2 % slower)
+                uint32_t w[16];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    uint32_t w4[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[u * 8 + 2 * e]), __uint_as_float(o[u * 8 + 2 * e + 1])), make_float2(inv, inv));
-                        w4[e] = pack_h16<F16>(v.x, v.y);
-                    }
-                    *reinterpret_cast<uint4*>(box + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                for (int i = 0; i < 16; ++i) {
+                    const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), make_float2(inv, inv));
+                    w[i] = pack_h16<F16>(v.x, v.y);
                 }
+                if (lane == 0) bulk_wait_group_read<0>();   // the previous copy has read the box
                 __syncwarp();
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int r = u * 8 + (lane >> 2), piece = lane & 3;
-                    const uint4 v = *reinterpret_cast<const uint4*>(box + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-                    if (row0 + r < p.q_len && c + piece * 8 < p.dim) *reinterpret_cast<uint4*>(out + r * p.os[2] + 2 * (c + piece * 8)) = v;
+                for (int u = 0; u < 4; ++u)
+                    *reinterpret_cast<uint4*>(box + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {   // rows behind the last and channels past the head are cut off by the copy
+                    if (row0 < p.q_len) tma_store_4d(&tm_o, box, c, row0, it.head * p.o_hmul, it.batch * p.o_bmul);
+                    bulk_commit_group();
                 }
                 __syncwarp();
             }
         }
+        if (lane == 0) bulk_wait_group<0>();
+        __syncwarp();
     } else {
         reg_alloc<CT_REGS_SOFTMAX>();
         // ------------------------------------------------------------------ softmax: thread = one query row
@@ -485,12 +486,8 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             for (int i = 0; i < 16; ++i) {
                 const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), sc2, nm2);
                 float2 r;
-                if ((i & 3) == 3) {   // a quarter on the FMA pipe, as in attention.cu
-                    r = exp2_fma2(x);
-                } else {
-                    r.x = ex2(x.x);
-                    r.y = ex2(x.y);
-                }
+                r.x = ex2(x.x);
+                r.y = ex2(x.y);
                 sum2[i & 1] = __fadd2_rn(sum2[i & 1], r);
                 w[i] = pack_h16<F16>(r.x, r.y);
             }
@@ -954,7 +951,7 @@ struct CrossTensor {
 
 // 4-D tiled map (channel, token, head, batch).  A dimension of one, or broadcast with stride 0, is encoded with one entry and some
 // valid stride; *bmul / *hmul say whether its coordinate counts.
-static int cross_tmap(CUtensorMap* map, const CrossTensor& t, int dim, int dtype, int box_rows, int* bmul, int* hmul) {
+static int cross_tmap(CUtensorMap* map, const CrossTensor& t, int dim, int dtype, int box_rows, int* bmul, int* hmul, int box_channels = 64) {
     const int64_t any = dim;   // a multiple of 8
     *bmul = t.batch > 1 && t.stride[0] != 0;
     *hmul = t.heads > 1 && t.stride[1] != 0;
@@ -962,13 +959,13 @@ static int cross_tmap(CUtensorMap* map, const CrossTensor& t, int dim, int dtype
                               static_cast<uint64_t>(*bmul ? t.batch : 1)};
     const uint64_t strides[3] = {2 * static_cast<uint64_t>(t.tokens > 1 ? t.stride[2] : any), 2 * static_cast<uint64_t>(*hmul ? t.stride[1] : any),
                                  2 * static_cast<uint64_t>(*bmul ? t.stride[0] : any)};
-    const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), 1, 1};
+    const uint32_t box[4] = {static_cast<uint32_t>(box_channels), static_cast<uint32_t>(box_rows), 1, 1};
     return make_tmap_nd(map, t.base, dtype == SVDQ_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims, strides,
-                        box, true);
+                        box, box_channels == 64 ? 128 : 64);
 }
 
 template <bool F16, bool MASK>
-static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CrossTileParams& p, int grid, int table_bytes,
+static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const CrossTileParams& p, int grid, int table_bytes,
                              cudaStream_t stream) {
     auto kern = cross_tile_kernel<F16, MASK>;
     static std::atomic<uint64_t> attr_done{0};
@@ -983,7 +980,7 @@ static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, p));
+    SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, to, p));
     return SVDQ_OK;
 }
 
@@ -1131,20 +1128,19 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         p.group = group;
         p.scale_log2 = scale_log2;
         if (int rc = status_words(&p.status)) return rc;
-        p.out = static_cast<uint8_t*>(a->out) + 2 * b0 * a->o_stride[0];
-        for (int i = 0; i < 3; ++i) p.os[i] = 2 * a->o_stride[i];
         p.heads = a->heads;
         p.q_tiles = q_tiles;
         p.batch = nb;
         p.items = nb * a->heads * q_tiles;
         p.mask_words = mask_words;
-        CUtensorMap mq, mk, mv;
+        CUtensorMap mq, mk, mv, mo;
         if (int rc = cross_tmap(&mq, from(tq, 1), a->head_dim, a->dtype, CT_BM, &p.q_bmul, &p.q_hmul)) return rc;
         if (int rc = cross_tmap(&mk, from(tk, !a->kv_offsets), a->head_dim, a->dtype, CT_BN, &p.k_bmul, &p.k_hmul)) return rc;
         if (int rc = cross_tmap(&mv, from(tv, !a->kv_offsets), a->head_dim, a->dtype, CT_BN, &p.v_bmul, &p.v_hmul)) return rc;
+        if (int rc = cross_tmap(&mo, from(to, 1), a->head_dim, a->dtype, 32, &p.o_bmul, &p.o_hmul, 32)) return rc;
         const int grid = p.items < 2 * sms ? p.items : 2 * sms, bytes = nb * (8 + 4 * mask_words);   // two CTAs per SM work through the items
-        const int rc = a->mask ? (f16 ? launch_cross_tile<true, true>(mq, mk, mv, p, grid, bytes, st) : launch_cross_tile<false, true>(mq, mk, mv, p, grid, bytes, st))
-                               : (f16 ? launch_cross_tile<true, false>(mq, mk, mv, p, grid, bytes, st) : launch_cross_tile<false, false>(mq, mk, mv, p, grid, bytes, st));
+        const int rc = a->mask ? (f16 ? launch_cross_tile<true, true>(mq, mk, mv, mo, p, grid, bytes, st) : launch_cross_tile<false, true>(mq, mk, mv, mo, p, grid, bytes, st))
+                               : (f16 ? launch_cross_tile<true, false>(mq, mk, mv, mo, p, grid, bytes, st) : launch_cross_tile<false, false>(mq, mk, mv, mo, p, grid, bytes, st));
         if (rc) return rc;
     }
     return SVDQ_OK;

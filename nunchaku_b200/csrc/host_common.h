@@ -87,7 +87,7 @@ int make_tmap_3d(CUtensorMap* map, const void* base, int elem, uint64_t d0, uint
 // Tiled map of rank 2..4 (dimension 0 innermost and contiguous; `strides_bytes` for dimensions 1..rank-1, in any order of
 // magnitude); out-of-range boxes read zeros.
 int make_tmap_nd(CUtensorMap* map, const void* base, int elem, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                 const uint32_t* box, bool swizzle128);
+                 const uint32_t* box, int swizzle /*bytes: 0, 64, 128*/);
 
 // Pointer / shape / alignment / architecture checks shared by the GEMM entry points.
 int check_gemm_common(const svdq_gemm_args* a);
