@@ -351,7 +351,7 @@ typedef struct svdq_quantize_w8a8_args {
                                  when that one is contiguous                                     */
     int64_t rows, x_stride, residual_stride;   /* strides: multiples of 8, at least cols          */
     int32_t cols;             /* multiple of 16, at most 16384                                   */
-    float eps;
+    float eps;                /* with a weight: at least 1e-30                                   */
     int32_t dtype;
 } svdq_quantize_w8a8_args;
 int svdq_quantize_w8a8(const svdq_quantize_w8a8_args* args, void* stream);
@@ -379,7 +379,7 @@ typedef struct svdq_gemm_w8a8_args {
     const void* bias;         /* NULL, or [N] of the output's type                               */
     void* out;                /* bf16 / fp16 (`dtype`) [M, N], row stride out_stride elements     */
     int64_t out_stride;       /* multiple of 8, at least N                                       */
-    int32_t M, N, K;          /* N a multiple of 8, K of 16 (at most 131056)                     */
+    int32_t M, N, K;          /* N a multiple of 8, K of 16 (at most 131056); M, N at most 2^30   */
     int32_t dtype;
 } svdq_gemm_w8a8_args;
 int svdq_gemm_w8a8(const svdq_gemm_w8a8_args* args, void* stream);
@@ -404,7 +404,7 @@ typedef struct svdq_cross_attention_args {
     const void* mask;         /* NULL, or bytes [batch, kv_len] on the device: states whose byte is not 0 exist              */
     int64_t mask_stride;      /* bytes between the mask's rows                                   */
     int32_t batch, heads, kv_heads, q_len, kv_len, head_dim;      /* at most one of kv_lens, kv_offsets, mask; kv_len <= 32768
-                                                                     with a mask                 */
+                                                                     with a mask; batch, heads <= 65535, q_len, kv_len <= 2^30     */
     float scale;              /* positive                                                        */
     int32_t dtype;            /* SVDQ_DTYPE_* of q, k, v and out                                 */
 } svdq_cross_attention_args;

@@ -530,12 +530,12 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 hide(a0, MASK ? it.bits(j)[0] : valid >= 32 ? 0xffffffffu : (1u << valid) - 1u);
                 // (Not below a finite bound: a block of which nothing is to be seen, ahead of others, has only -inf, whose exponentials are 0
                 // whatever the finite maximum.  A score that is NaN makes the maximum and with it the whole row NaN.)
-                float mx = max32(a0, -3e38f);
+                float mx = max32(a0, -INFINITY);
                 if (two) {
                     hide(a1, MASK ? it.bits(j)[1] : valid >= 64 ? 0xffffffffu : (1u << (valid - 32)) - 1u);
                     mx = max32(a1, mx);
                 }
-                const float ms = max3_nan(mx * p.scale_log2, -1e30f, -1e30f);
+                const float ms = max3_nan(mx * p.scale_log2, -3e38f, -3e38f);
                 if (j == 0) {
                     m_used = ms;
                 } else if (const bool grow = !(ms <= m_used + CT_RESCALE_STEP); __any_sync(0xffffffffu, grow)) {

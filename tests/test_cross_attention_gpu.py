@@ -244,6 +244,26 @@ def test_states_of_minus_infinity(Tq, H):
         _check(cross_attention(q, k2, v), q, k3, v, keep2, D ** -0.5)
 
 
+@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_scores_of_the_largest_magnitudes(Tq, H, masked):
+    """scores down to -1e37: the state of the largest alone is seen, wherever it stands"""
+    from nunchaku_b200.ops import cross_attention
+
+    T, D = 200, 64
+    q = torch.full((1, H, Tq, D), 2.0 ** 61, dtype=torch.bfloat16, device="cuda")
+    v = torch.randn(1, H, T, D, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    mask = torch.ones(1, T, dtype=torch.bool, device="cuda")
+    for at in (0, 63, 64, 130, 199):
+        k = torch.full((1, H, T, D), -2.0 ** 60, dtype=torch.bfloat16, device="cuda")
+        k[:, :, at] = -2.0 ** 59
+        if masked:
+            mask[:] = True
+            mask[0, :64] = at < 64          # a first block of which nothing is to be seen
+        got = cross_attention(q, k, v, mask=mask if masked else None)
+        assert torch.equal(got.view(1, Tq, H, D), v[:, :, at][:, None].expand(1, Tq, H, D))
+
+
 def test_two_calls_at_once():
     """on two streams, each call's result as when alone"""
     from nunchaku_b200.ops import cross_attention

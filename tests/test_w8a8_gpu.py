@@ -6,6 +6,8 @@ exact one where the exact quotient lies within 127 * 6 u (127 * 2 u) of a half. 
 terms per thread plus ten tree steps is off by at most 43 u, its root by half of that, and the few products behind it by 6 u.
 GEMM: the integer sum is exact; its conversion, the two products and the addition are off by at most 4 u of
 |product| + |bias|, and the output by half a step of its type."""
+import ctypes
+
 import pytest
 import torch
 
@@ -123,6 +125,21 @@ def test_ties_of_rows_up_to_the_largest_numbers():
     codes, scales = quantize_w8a8(x.cuda())
     assert (codes[:, 5] == 127).all() and (codes[:, 6] == 64).all() and (codes[:, 7] == -64).all() and codes.float().abs().sum() == 254 * 255
     _check((codes, scales), x)
+
+
+@pytest.mark.parametrize("onto", ["x", "residual"])
+def test_residual_stream_in_place(onto):
+    """through the C interface, hidden may be x or the residual"""
+    x, r, w = (_rand(*s, seed=40 + i, dtype=torch.bfloat16).cuda() for i, s in enumerate([(3000, 2240), (3000, 2240), (2240,)]))
+    from nunchaku_b200.ops import rms_norm_quantize_w8a8
+
+    ref = rms_norm_quantize_w8a8(x, w, residual=r)
+    codes, scales, hidden = torch.empty_like(ref[0]), torch.empty_like(ref[1]), x if onto == "x" else r
+    args = _lib.QuantizeW8A8Args(x.data_ptr(), r.data_ptr(), w.data_ptr(), codes.data_ptr(), scales.data_ptr(), hidden.data_ptr(), 3000, 2240, 2240,
+                                 2240, 1e-6, 0)
+    _lib.check(_lib.load().svdq_quantize_w8a8(ctypes.byref(args), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(codes, ref[0]) and torch.equal(scales, ref[1]) and torch.equal(hidden, ref[2])
 
 
 def test_two_calls_at_once():
