@@ -7,7 +7,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_size_t, c_void_p
+import struct
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SVDQ_B200_LIB") or os.path.join(_HERE, "libsvdq_b200.so")
@@ -300,6 +301,20 @@ class LiteLAArgs(Structure):
     ]
 
 
+_FORMATS = {c_void_p: "P", c_int64: "q", c_int32: "i", c_float: "f"}
+
+
+def _packer(cls):
+    """Positional field values -> the bytes of one ``cls``: a fifth of the time that building the ctypes object takes (1 to 3 us of a call of
+    10), and a number that does not fit its field raises instead of losing bits.  Null pointers are 0."""
+    s = struct.Struct("".join(_FORMATS[t] for _, t in cls._fields_) + "0P")
+    assert s.size == ctypes.sizeof(cls)
+    return s.pack
+
+
+pack_quantize_w8a8, pack_dequantize_w8a8 = _packer(QuantizeW8A8Args), _packer(DequantizeW8A8Args)
+pack_gemm_w8a8, pack_cross_attention = _packer(GemmW8A8Args), _packer(CrossAttentionArgs)
+
 # every symbol include/svdq_b200.h declares: (restype, argtypes)
 EXPORTS = {
     "svdq_quantize_w4a4_act_fuse_lora": (c_int32, [POINTER(QuantizeArgs), c_void_p]),
@@ -315,10 +330,10 @@ EXPORTS = {
     "svdq_litela": (c_int32, [POINTER(LiteLAArgs), c_void_p]),
     "svdq_attention": (c_int32, [POINTER(AttentionArgs), c_void_p]),
     "svdq_quantize_w4a4_wgt": (c_int32, [POINTER(QuantizeWgtArgs), c_void_p]),
-    "svdq_cross_attention": (c_int32, [POINTER(CrossAttentionArgs), c_void_p]),
-    "svdq_quantize_w8a8": (c_int32, [POINTER(QuantizeW8A8Args), c_void_p]),
-    "svdq_dequantize_w8a8": (c_int32, [POINTER(DequantizeW8A8Args), c_void_p]),
-    "svdq_gemm_w8a8": (c_int32, [POINTER(GemmW8A8Args), c_void_p]),
+    "svdq_cross_attention": (c_int32, [c_void_p, c_void_p]),
+    "svdq_quantize_w8a8": (c_int32, [c_void_p, c_void_p]),
+    "svdq_dequantize_w8a8": (c_int32, [c_void_p, c_void_p]),
+    "svdq_gemm_w8a8": (c_int32, [c_void_p, c_void_p]),
     "svdq_device_status": (c_int32, [POINTER(c_int32), POINTER(c_int32)]),
     "svdq_last_error_string": (c_char_p, []),
     "svdq_version": (c_int32, []),

@@ -20,30 +20,11 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_
         : "memory");
 }
 
-// D[tmem] (+)= A[smem] * B[smem], 16-bit operands, fp32 accumulation, one CTA.
-__device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// The same with A in tensor memory: lane = row, every 32-bit column holds two consecutive K elements (the lower index in
-// the lower half), so a K-step of 16 is 8 columns.
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// The two forms with descriptors given as 32-bit halves: the upper half (strides, swizzle) is a constant of the kernel and
-// the lower half (start address in 16-byte units, leading byte offset) moves by small immediates, so that an unrolled
-// issue loop needs no 64-bit arithmetic.  A and B share the upper half in the first form.
+// D[tmem] (+)= A[smem] * B[smem], 16-bit operands, fp32 accumulation, one CTA; in the second form A is in tensor memory: lane = row, every
+// 32-bit column holds two consecutive K elements (the lower index in the lower half), so a K-step of 16 is 8 columns.
+// Descriptors are given as 32-bit halves: the upper half (strides, swizzle) is a constant of the kernel and the lower half (start
+// address in 16-byte units, leading byte offset) moves by small immediates, so that an unrolled issue loop needs no 64-bit
+// arithmetic.  A and B share the upper half in the first form.
 __device__ __forceinline__ void tc_mma_f16_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc,
                                               uint32_t accumulate) {
     asm volatile(

@@ -89,8 +89,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
         raise ValueError("at most one of kv_lens, mask and kv_offsets")
     if k.shape != v.shape:
         raise ValueError("k and v must have the same shape")
-    lens_ptr = off_ptr = mask_ptr = None
-    mask_stride = 0
+    lens_ptr = off_ptr = mask_ptr = mask_stride = 0
     if kv_offsets is not None:
         if k.dim() != 3 or k.shape[2] != D:
             raise ValueError("with kv_offsets, k and v are packed [total, kv_heads, D]")
@@ -137,7 +136,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
             if out.shape != q.shape or out.stride(3) != 1:
                 raise ValueError("out must be [batch, tokens_q, heads*D] or [batch, heads, tokens_q, D]")
             os = out.stride()[:3]
-    args = _lib.CrossAttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), ret.data_ptr(), *qs[:3], *ks, *vs, *os, lens_ptr, off_ptr, mask_ptr, mask_stride,
+    args = _lib.pack_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), ret.data_ptr(), *qs[:3], *ks, *vs, *os, lens_ptr, off_ptr, mask_ptr, mask_stride,
                                    B, H, Hk, Tq, T, D, float(D ** -0.5 if scale is None else scale), dtype_code(dtype))
     launch(_lib.load().svdq_cross_attention, args, dev)
     return ret

@@ -57,8 +57,8 @@ def _quantize(x, weight, residual, eps):
     scales = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=dev)
     if len(shape) != 2:
         scales = scales.view(shape[:-1])
-    hidden_ptr = res_ptr = weight_ptr = hidden = None
-    res_stride = 0
+    hidden = None
+    hidden_ptr = res_ptr = weight_ptr = res_stride = 0
     if weight is not None:
         _check_half("weight", weight, x)
         if weight.shape != (cols,) or not weight.is_contiguous():
@@ -72,7 +72,7 @@ def _quantize(x, weight, residual, eps):
         hidden = torch.empty_like(x, memory_format=torch.contiguous_format)
         res_ptr, hidden_ptr = residual.data_ptr(), hidden.data_ptr()
     launch(_lib.load().svdq_quantize_w8a8,
-           _lib.QuantizeW8A8Args(x.data_ptr(), res_ptr, weight_ptr, codes.data_ptr(), scales.data_ptr(), hidden_ptr, rows, x_stride, res_stride,
+           _lib.pack_quantize_w8a8(x.data_ptr(), res_ptr, weight_ptr, codes.data_ptr(), scales.data_ptr(), hidden_ptr, rows, x_stride, res_stride,
                                  cols, eps, dtype_code(x.dtype)), dev)
     return codes, scales, hidden
 
@@ -113,7 +113,7 @@ def dequantize_w8a8(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.
     code = dtype_code(out_dtype)
     out = torch.empty_like(codes, dtype=out_dtype)
     launch(_lib.load().svdq_dequantize_w8a8,
-           _lib.DequantizeW8A8Args(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel() // cols, cols, code), codes.device)
+           _lib.pack_dequantize_w8a8(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel() // cols, cols, code), codes.device)
     return out
 
 
@@ -159,6 +159,6 @@ def gemm_w8a8(act: torch.Tensor, wgt: torch.Tensor, ascales: torch.Tensor, wscal
     else:
         stride = _rows("out", out, N)[1]
     launch(_lib.load().svdq_gemm_w8a8,
-           _lib.GemmW8A8Args(act.data_ptr(), wgt.data_ptr(), ascales.data_ptr(), wscales.data_ptr(), None if bias is None else bias.data_ptr(),
+           _lib.pack_gemm_w8a8(act.data_ptr(), wgt.data_ptr(), ascales.data_ptr(), wscales.data_ptr(), 0 if bias is None else bias.data_ptr(),
                              out.data_ptr(), stride, rows, N, K, code), dev)
     return out
