@@ -404,7 +404,8 @@ typedef struct svdq_cross_attention_args {
     const void* mask;         /* NULL, or bytes [batch, kv_len] on the device: states whose byte is not 0 exist              */
     int64_t mask_stride;      /* bytes between the mask's rows                                   */
     int32_t batch, heads, kv_heads, q_len, kv_len, head_dim;      /* at most one of kv_lens, kv_offsets, mask; kv_len <= 32768
-                                                                     with a mask; batch, heads <= 65535, q_len, kv_len <= 2^30     */
+                                                                     with a mask; batch, heads <= 65535; q_len, kv_len <= 2^30, and
+                                                                     q_len * heads / kv_heads <= 2^20 - 16 where kv_len > 2^22     */
     float scale;              /* positive                                                        */
     int32_t dtype;            /* SVDQ_DTYPE_* of q, k, v and out                                 */
 } svdq_cross_attention_args;

@@ -87,6 +87,7 @@ constexpr int CT_SMEM = 1024 + CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + CT_STAG
 constexpr int CT_TABLE_BYTES = 6 * 1024;            // the samples' ranges or mask bits
 constexpr int CT_TMEM_COLS = 256;                   // S: 2 x 64, O: 128
 constexpr int CT_WAIT_LOOKS = 1 << 20;              // each of up to a microsecond
+constexpr int CT_MAX_STATES = 1 << 22;              // about 70 ms an item: its output warps wait that long, and are not to give up on it
 constexpr float CT_RESCALE_STEP = 8.f;
 // What it takes to change queries and hand the output over, in tenths of a block of 64 states' time (32 x 20 x 1024 x <=300 x 112, packed:
 // 134 us at 8, 112 at 12, 109 at 16, 110 at 20)
@@ -1083,7 +1084,8 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
                  rows_shared = (a->head_dim > 64 ? 0.53 : 0.26) * static_cast<double>(ctas) * static_cast<double>(tiles) / sms;
     const double rows_us = 6.5 + (rows_alone > rows_shared ? rows_alone : rows_shared);
     const double tile_us = 5.0 + (q_items <= sms ? 0.8 : 1.0 * static_cast<double>((q_items + 2 * sms - 1) / (2 * sms))) * static_cast<double>(tiles);
-    if ((q_rows <= CR_ROWS || rows_us < tile_us) && kv_pairs * CR_MAX_SPLIT < (1ll << 31) && q_rows <= CR_ROWS * 65535ll) {
+    // (no wait of the row kernel lasts longer than a few tiles, however many states there are)
+    if ((q_rows <= CR_ROWS || rows_us < tile_us || a->kv_len > CT_MAX_STATES) && kv_pairs * CR_MAX_SPLIT < (1ll << 31) && q_rows <= CR_ROWS * 65535ll) {
         CrossRowsParams p = {};
         p.st = states;
         p.q = static_cast<const uint8_t*>(a->q);
@@ -1104,6 +1106,8 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         return f16 ? launch_cross_rows_dim<true>(mk, mv, p, static_cast<int>(kv_pairs), split, st)
                    : launch_cross_rows_dim<false>(mk, mv, p, static_cast<int>(kv_pairs), split, st);
     }
+    if (a->kv_len > CT_MAX_STATES)
+        return fail(SVDQ_ERR_UNSUPPORTED, "cross_attention: more than %d states (got %d) for so many queries", CT_MAX_STATES, a->kv_len);
     // The kernel keeps its samples' ranges and mask bits in shared memory: launches of as many samples as fit (hundreds, without a mask).
     const int q_tiles = (a->q_len + CT_BM - 1) / CT_BM;
     const int mask_words = a->mask ? (a->kv_len + CT_BN - 1) / CT_BN * (CT_BN / 32) : 0;

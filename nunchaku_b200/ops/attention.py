@@ -75,7 +75,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: 
     Which states exist, at most one of: ``kv_lens`` int32 [B] (the first so many of each sample), ``mask`` bool [B, T] (those that are
     True; T up to 32768), ``kv_offsets`` int32 [B + 1] (k and v are then packed [total, Hk, D], sample b owning rows
     ``kv_offsets[b]:kv_offsets[b + 1]``); all on q's device, read there (lengths outside 0..T are clamped).  None: all T.  A sample without
-    states gets zeros; states that do not exist may hold anything, NaN included.
+    states gets zeros; states that do not exist may hold anything, NaN included.  With k and v longer than 2**22, Tq * H / Hk is at most
+    2**20 - 16.
     out: [B, Tq, H*D] (default: a new tensor) or a [B, H, Tq, D] view of one.  scale defaults to D ** -0.5 and must be positive."""
     dtype, dev = q.dtype, q.device
     if not q.is_cuda or dtype not in HALF_DTYPES:

@@ -302,6 +302,27 @@ def test_long_state_lists():
         _check(cross_attention(q, k, v), q, k, v, _keep(1, T), 0.125)
 
 
+def test_many_queries_over_millions_of_states():
+    """longer lists than the tile kernel takes.  Tolerance: every row's sums run through up to T / 32 additions in fp32 per lane and product,
+    each off by at most 2^-23 (the tensor cores may truncate), on top of the output's half step and the probabilities' (values are positive)"""
+    from nunchaku_b200.ops import cross_attention
+
+    T, Tq, D = 2 ** 22 + 100, 20480, 8
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(1, 1, Tq, D, generator=g).half().cuda()
+    k = torch.randn(1, 1, T, D, generator=g).half().cuda()
+    v = (torch.linspace(0, 2, T)[:, None] * torch.linspace(0.5, 1, D)).half()[None, None].cuda()
+    got = cross_attention(q, k, v)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == (0, 0)
+    rows = [0, 777, Tq - 1]
+    w = torch.softmax(D ** -0.5 * (q[0, 0, rows].double() @ k[0, 0].double().T), dim=-1)
+    exp = w @ v[0, 0].double()
+    assert ((got[0, rows].double() - exp).abs() <= exp * (2 * (T / 32) * 2.0 ** -23 + 2.0 ** -10)).all()
+    with pytest.raises(NotImplementedError):
+        cross_attention(torch.empty(1, 1, 2 ** 20, 8, dtype=torch.float16, device="cuda"), k, v)
+
+
 def test_states_beyond_32_bit_offsets():
     """a batch whose last sample starts more than 2^31 elements into the buffer"""
     from nunchaku_b200.ops import cross_attention
