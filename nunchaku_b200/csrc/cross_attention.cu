@@ -11,28 +11,29 @@
 //
 // Two kernels.
 //
-// cross_tile_kernel (many queries): an item is 128 query rows of one (batch, head); its states are walked in blocks of 64 with Q K^T
-// and P V as tcgen05.mma kind::f16, S, P and O in tensor memory and a running maximum per row (O is rescaled only when a maximum has
-// grown by more than 2^8, as in attention.cu).  State lists are short here (a caption has up to 300 states, five blocks), so filling
-// and draining count as much as the loop: CTAs are resident, two to an SM, and each works through a run of items; warps are
-// specialised so that an item's output, the next one's queries and the products of both lie behind one another:
-//   warps 0-3 softmax (one query row per thread), 4-7 output (O / l, through shared memory and on by TMA), 8 MMA issuer, 9 producer of
-//   Q and K, 10 producer of V, 11 nothing (registers are re-divided by fours).
-// Two S buffers of 64 columns: a block's Q K^T runs under the previous block's exponentials.  K and V have two slots each.  The last
-// block's products, loads and exponentials are cut to the states that exist (in sixteens, sixteens and 32s).
+// cross_tile_kernel (many queries): an item is 128 query rows of one (batch, head), or two times 128 over the same states (two tiles of
+// a head, or two heads that share a stored one); the states are walked in blocks of 64 with Q K^T and P V as tcgen05.mma kind::f16, S,
+// P and O in tensor memory and a running maximum per row (O is rescaled only when a maximum has grown by more than 2^8, as in
+// attention.cu).  State lists are short here (a caption has up to 300 states, five blocks), so filling and draining count as much as
+// the loop: CTAs are resident (one of two tiles, or two of one tile, to an SM), each works through a run of items, and warps are
+// specialised so that an item's output, the next one's queries and the products of both lie behind one another.  Per tile: four softmax
+// warps (one query row per thread), four output warps (O / l, through shared memory and on by TMA), an issuer for Q K^T and one for P V (an
+// MMA of these sizes takes longer to issue than to run); per CTA a producer of Q and K and one of V.
+// Two S buffers of 64 columns: a block's Q K^T runs under the previous block's exponentials.  K and V have two slots each, and with two
+// tiles Q has two buffers: the next item's queries are on their way while this one is worked on.  The last block's products, loads and
+// exponentials are cut to the states that exist (in sixteens, sixteens and 32s).
 // Items lie in the order batch, tile, head: the heads' channels are neighbours in token-major rows, and a row of 224 bytes shares
 // its DRAM bursts with them (one block of states, 32 x 20 x 1024 x 64 x 112: 94 us with tiles innermost, 65 so).  A CTA's run of items
 // is cut from the samples' lengths on the device, so that all runs cost alike.
-// What bounds it: 32 x 20 x 1024 x <=300 x 112, packed, moves 342 MB (52 us at the copy rate) and takes 105 us, 65 us of that for the first
-// block of every item and about 20 for each further one (full lists of 300: 168 us).  Without its stores it takes 17 us less, without its
-// exponentials 5 to 8, without its loads 3 to 7: no single unit (a quarter of the exponentials on the FMA pipe, as in attention.cu, gains
-// nothing here and costs 5 % over 4096 states), but the chain S -> maximum -> P -> P V -> O -> output, with which two CTAs fill
-// half of the issue slots (53 %), a fifth of the tensor pipe and half of the DRAM's time (states are read again by some of a sample's later
-// tiles, 307 MB against 195).  The code of all roles has to stay small: at 80 KB it ran 30 % slower than at 47, and with the output's loop
-// unrolled (70 KB) it took twice as long.  Tried and no faster: 256 query rows per CTA over the same K and V with a second Q
-// buffer (65 -> 69 and 168 -> 145 us on 64 and 300 states, 105 -> 107 on the packed ones), an issuer warp per product, two threads per row (105 ->
-// 117), the output out of Q's buffer (which then comes free late: 51 against 42 us on 64 states of 64 channels), waits without suspension; queries and output
-// first to leave L2 (300 states 5 % faster, 64 states as much slower).
+// What bounds it: 32 x 20 x 1024 x <=300 x 112, packed, moves 342 MB (52 us at the copy rate) and takes 96 us; 69 us with one block of 64 for
+// every item, about 17 for each further one (full lists of 300: 133 us).  Two waits set the pace.  The queries of an item come 2.5 us after
+// they are asked for, and the copy unit takes four cycles for a row of up to 128 bytes, whether query, state or output (with one tile at a
+// time and one Q buffer the same takes 105 us, full lists of 300 160).  And in a block the chain S -> maximum -> P -> P V is served by two
+// softmax warps per scheduler, which leave half of the issue slots empty.  The code of all roles has to stay small: at 80 KB it ran 30 % slower than at 47,
+// and with the output's loop unrolled (70 KB) it took twice as long.  Tried and no faster: a quarter of the exponentials on the FMA pipe,
+// as in attention.cu, two threads per row (105 -> 117), the output out of Q's buffer (which then comes free late), in boxes of 128-byte rows
+// (99 -> 125, by code and registers) or by the warps' own stores (1 to 2 %), waits without suspension, queries and output first to leave
+// L2 (300 states 5 % faster, 64 states as much slower).
 //
 // cross_rows_kernel (few query rows per stored head: the serving form for single tokens): bound by streaming K and V once.
 // Up to 16 rows (queries x heads that share a stored head) are the M side of mma.sync m16n8k16; four warps take 16 of every 64
@@ -74,40 +75,56 @@ constexpr int CT_Q_HALF = CT_BM * 128;              // 128 rows x 64 channels
 constexpr int CT_KV_HALF = CT_BN * 128;
 constexpr int CT_Q_BYTES = 2 * CT_Q_HALF, CT_KV_BYTES = 2 * CT_KV_HALF;
 constexpr int CT_SLOTS = 2;                         // of K and of V each
-constexpr int CT_THREADS = 12 * 32;
-constexpr int CT_MMA_WARP = 8, CT_QK_WARP = 9, CT_V_WARP = 10;   // 0-3 softmax, 4-7 output, 11 nothing
-// registers move inside the pool the CTA was launched with (384 threads x 80: two CTAs fill the file)
-constexpr int CT_REGS_SOFTMAX = 112, CT_REGS_OUTPUT = 64, CT_REGS_OTHER = 64;
-static_assert(CT_REGS_SOFTMAX + CT_REGS_OUTPUT + CT_REGS_OTHER <= 3 * 80, "register budget");
-constexpr int CT_MASK_STATES = 32768;               // longest state list a mask may cover (its bits are kept in shared memory)
 constexpr int CT_STAGE_BYTES = 4 * 32 * 64;         // output: 32 rows x 32 channels per output warp on their way to memory
-constexpr int CT_BAR_BYTES = 256;
-constexpr int CT_SUM_BYTES = 2 * CT_BM * 4;         // row sums of two items
-constexpr int CT_SMEM = 1024 + CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + CT_STAGE_BYTES + CT_SUM_BYTES + CT_BAR_BYTES;   // 106 KB: two CTAs per SM
+constexpr int CT_BAR_BYTES = 512;
+constexpr int CT_MASK_STATES = 32768;               // longest state list a mask may cover (its bits are kept in shared memory)
 constexpr int CT_TABLE_BYTES = 6 * 1024;            // the samples' ranges or mask bits
-constexpr int CT_TMEM_COLS = 256;                   // S: 2 x 64, O: 128
+constexpr int CT_TMEM_COLS = 256;                   // of a query tile.  S: 2 x 64, O: 128
 constexpr int CT_WAIT_LOOKS = 1 << 20;              // each of up to a microsecond
 constexpr int CT_MAX_STATES = 1 << 22;              // about 70 ms an item: its output warps wait that long, and are not to give up on it
 constexpr float CT_RESCALE_STEP = 8.f;
-// What it takes to change queries and hand the output over, in tenths of a block of 64 states' time (32 x 20 x 1024 x <=300 x 112, packed:
-// 134 us at 8, 112 at 12, 109 at 16, 110 at 20)
-constexpr int CT_ITEM_COST = 16;
-static_assert(2 * (CT_SMEM + CT_TABLE_BYTES + 1024) <= 228 * 1024 && CT_TABLE_BYTES >= CT_MASK_STATES / 8 + 8, "two CTAs per SM");
+static_assert(CT_TABLE_BYTES >= CT_MASK_STATES / 8 + 8, "the bits of one sample's mask");
 
+// TILES: query tiles that a CTA works on at a time, over the same states
+template <int TILES>
+struct CrossTileSizes {
+    static constexpr int Q_BUFFERS = TILES;             // two tiles leave room for the next item's queries as well
+    static constexpr int WARPS = TILES == 1 ? 12 : 24;
+    static constexpr int THREADS = 32 * WARPS;
+    // softmax, 4 per tile; output, 4 per tile; then
+    static constexpr int OUT_WARP = 4 * TILES, S_WARP = 8 * TILES, PV_WARP = S_WARP + TILES, QK_WARP = PV_WARP + TILES, V_WARP = QK_WARP + 1;
+    static_assert(V_WARP < WARPS, "warps");
+    // registers move inside the pool the CTA was launched with (80 a thread fill the file)
+    static constexpr int REGS_SOFTMAX = 112, REGS_OUTPUT = 64, REGS_OTHER = 64;
+    static_assert(4 * TILES * (REGS_SOFTMAX + REGS_OUTPUT) + (WARPS - 8 * TILES) * REGS_OTHER <= WARPS * 80, "register budget");
+    static constexpr int SUM_BYTES = 3 * TILES * CT_BM * 4;   // row sums of three items
+    static constexpr int SMEM = 1024 + Q_BUFFERS * TILES * CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + TILES * CT_STAGE_BYTES + SUM_BYTES + CT_BAR_BYTES;
+    static constexpr int PER_SM = TILES == 1 ? 2 : 1;
+    // what it takes to change queries and hand the output over, in tenths of a block of 64 states' time (32 x 20 x 1024 x <=300 x 112, packed: one
+    // tile 134 us at 8, 112 at 12, 109 at 16, 110 at 20; two 97.5 at 10, 96.3 at 13, 99.5 at 16, 101.5 at 20)
+    static constexpr int ITEM_COST = TILES == 1 ? 16 : 13;
+    static_assert(PER_SM * (SMEM + CT_TABLE_BYTES + 1024) <= 228 * 1024, "CTAs per SM");
+};
+
+template <int TILES>
 struct CrossTileShared {
-    // A slot of K is free when its Q K^T is done (s_full), one of V when its P V is (pv_done), Q when the item's last Q K^T is: the
-    // producers wait for those.  A block of V whose rows are all to be seen lands on v_full, which the issuer waits for; one with rows
-    // to be zeroed lands on vh_full, which the softmax warps wait for before they hand over P: so every barrier has one sequence of
-    // phases that its waiters follow without gaps.
-    uint64_t q_full, k_full[CT_SLOTS], v_full[CT_SLOTS], vh_full[CT_SLOTS], s_full[2], p_full[2], pv_done[2], l_full[2], o_free;
+    // A slot of K is free when every tile's Q K^T is done (s_full), one of V when every tile's P V is (pv_done): the producers wait for
+    // those.  A block of V whose rows are all to be seen lands on v_full; one with rows to be zeroed lands on vh_full, and who zeroes them
+    // arrives on vz_full.  Every barrier has one sequence of phases that its waiters follow without gaps.
+    uint64_t q_full[TILES], q_free[TILES], k_full[CT_SLOTS], v_full[CT_SLOTS], vh_full[CT_SLOTS], vz_full[CT_SLOTS];
+    struct {
+        uint64_t s_full[2], p_full[2], pv_done[2], l_full[3], o_free;
+    } tile[TILES];
     uint32_t tmem_base;
     int failed;            // the code of a wait that ran out
 };
-static_assert(sizeof(CrossTileShared) <= CT_BAR_BYTES, "barrier block");
+static_assert(sizeof(CrossTileShared<2>) <= CT_BAR_BYTES, "barrier block");
 
 struct CrossTileParams {
     CrossStates st;
-    int q_len, dim, group, heads, q_tiles, items, batch;  // item = (batch * q_tiles + tile) * heads + head
+    int q_len, dim, group, q_tiles, batch;
+    int units_h, units_t, items;                          // item = (batch * units_t + tile unit) * units_h + head unit
+    bool pair_heads;                                      // two tiles at a time: of two query heads that share a stored head, else of one head
     int mask_words;                                       // 32-bit words of mask bits per sample
     int q_bmul, q_hmul, k_bmul, k_hmul, v_bmul, v_hmul, o_bmul, o_hmul;   // 0 where that dimension is broadcast (stride 0): its coordinate is then 0
     float scale_log2;
@@ -116,7 +133,7 @@ struct CrossTileParams {
 
 // Bounded wait of a whole warp that lets the hardware suspend it between looks (polling takes issue slots from the softmax warps).
 // False, on every lane, when it runs out; the code is reported at the kernel's end.
-__device__ __forceinline__ bool ct_wait(uint64_t* bar, uint32_t parity, CrossTileShared* sh, int code) {
+__device__ __forceinline__ bool ct_wait(uint64_t* bar, uint32_t parity, int* failed, int code) {
     uint32_t ok = 0;
 #pragma unroll 1
     for (int i = 0; i < CT_WAIT_LOOKS && !ok; ++i)
@@ -128,31 +145,31 @@ __device__ __forceinline__ bool ct_wait(uint64_t* bar, uint32_t parity, CrossTil
             : "r"(smem_u32(bar)), "r"(parity), "r"(1000u)
             : "memory");
     if (__all_sync(0xffffffffu, ok != 0)) return true;
-    sh->failed = code;
+    *failed = code;
     return false;
 }
 
 // The items that a CTA works through, as each of its roles sees them: states [start, start + count) of the item's sample (with a mask:
 // up to the last one that is to be seen) in blocks of 64.  Starts in front of the first.
-template <bool MASK>
+template <bool MASK, int TILES>
 struct CrossItems {
     const CrossTileParams& p;
     const int2* ranges;
     const uint32_t* words;
-    int item, end, batch, head, tile, start, count, blocks;   // end: behind this CTA's last item
+    int item, end, batch, head_unit, tile_unit, start, count, blocks;   // end: behind this CTA's last item
 
     __device__ __forceinline__ CrossItems(const CrossTileParams& p_, const int2* r, const uint32_t* w, int first, int end_, int batch_, int head_, int tile_)
-        : p(p_), ranges(r), words(w), item(first - 1), end(end_), batch(batch_), head(head_ - 1), tile(tile_), start(0), count(0), blocks(0) {}
+        : p(p_), ranges(r), words(w), item(first - 1), end(end_), batch(batch_), head_unit(head_ - 1), tile_unit(tile_), start(0), count(0), blocks(0) {}
     // to the next item (EMPTY: even if it has no states); false behind the last
     template <bool EMPTY = false>
     __device__ __forceinline__ bool advance() {
 #pragma unroll 1
         do {
             if (++item >= end) return false;
-            if (++head == p.heads) {   // heads first: their channels lie next to each other in token-major rows
-                head = 0;
-                if (++tile == p.q_tiles) {
-                    tile = 0;
+            if (++head_unit == p.units_h) {   // heads first: their channels lie next to each other in token-major rows
+                head_unit = 0;
+                if (++tile_unit == p.units_t) {
+                    tile_unit = 0;
                     ++batch;
                 }
             }
@@ -163,6 +180,9 @@ struct CrossItems {
         } while (!EMPTY && blocks == 0);
         return true;
     }
+    // query head and tile of the CTA's tile t
+    __device__ __forceinline__ int head(int t) const { return TILES == 2 && p.pair_heads ? 2 * head_unit + t : head_unit; }
+    __device__ __forceinline__ int tile(int t) const { return TILES == 2 && !p.pair_heads ? 2 * tile_unit + t : tile_unit; }
     __device__ __forceinline__ int valid(int j) const { return min(count - j * CT_BN, CT_BN); }
     __device__ __forceinline__ const uint32_t* bits(int j) const { return words + batch * p.mask_words + 2 * j; }
     // some of the rows of V that P V reads (valid rounded up to 16) must not be seen and are not zeros already
@@ -176,8 +196,11 @@ struct CrossItems {
     }
 };
 
-// What an item costs, in tenths of a block of 64 states: its blocks, and what it takes to change queries and hand the output over.
-__device__ __forceinline__ float cross_item_cost(int count) { return static_cast<float>(10 * ((count + CT_BN - 1) / CT_BN) + CT_ITEM_COST); }
+// What an item costs, in tenths of a block's time.
+template <int TILES>
+__device__ __forceinline__ float cross_item_cost(int count) {
+    return static_cast<float>(10 * ((count + CT_BN - 1) / CT_BN) + CrossTileSizes<TILES>::ITEM_COST);
+}
 
 // largest of three; a NaN stays one (fmaxf drops it)
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -186,18 +209,37 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return d;
 }
 
-template <bool F16, bool MASK>
-__global__ void __launch_bounds__(CT_THREADS, 2)
+// Rows of a block of V whose states must not be seen -> zeros, up to the last that P V reads: eight lanes per row (and half), this lane's
+// rows from `r` on in steps of `step`.  By the softmax warps where a mask makes holes anywhere (by one warp a masked 6 x 16 x 1000 x 77 x 64
+// takes 18.4 us, so 15.6), by a P V issuer where at most 15 rows behind the last state are concerned (32 x 20 x 1024 x <=300 x 112: 99 against
+// 103).
+template <bool MASK, int TILES>
+__device__ __forceinline__ void zero_rows(const CrossItems<MASK, TILES>& it, uint8_t* v, int j, int halves, int r, int step, int lane) {
+    const int valid = it.valid(j), up = (valid + 15) & ~15;
+#pragma unroll 1
+    for (; r < up; r += step) {
+        bool zero = r >= valid;
+        if constexpr (MASK) zero = !((it.bits(j)[r >> 5] >> (r & 31)) & 1u);
+        if (zero)
+            for (int h = 0; h < halves; ++h) *reinterpret_cast<uint4*>(v + h * CT_KV_HALF + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+template <bool F16, bool MASK, int TILES>
+__global__ void __launch_bounds__(CrossTileSizes<TILES>::THREADS, CrossTileSizes<TILES>::PER_SM)
 cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                   const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ CrossTileParams p) {
+    using Sz = CrossTileSizes<TILES>;
     extern __shared__ __align__(1024) uint8_t ct_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ct_smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* q_s = smem;
-    uint8_t* k_s = q_s + CT_Q_BYTES;
+    uint8_t* q_s = smem;                                                    // [buffer][tile]
+    uint8_t* k_s = q_s + Sz::Q_BUFFERS * TILES * CT_Q_BYTES;
     uint8_t* v_s = k_s + CT_SLOTS * CT_KV_BYTES;
-    uint8_t* stage = v_s + CT_SLOTS * CT_KV_BYTES;
-    float* sums = reinterpret_cast<float*>(stage + CT_STAGE_BYTES);
-    CrossTileShared* sh = reinterpret_cast<CrossTileShared*>(stage + CT_STAGE_BYTES + CT_SUM_BYTES);
+    uint8_t* stage = v_s + CT_SLOTS * CT_KV_BYTES;                          // [output warp]
+    float* sums = reinterpret_cast<float*>(stage + TILES * CT_STAGE_BYTES);   // [3][tile][row]
+    auto* sh = reinterpret_cast<CrossTileShared<TILES>*>(reinterpret_cast<uint8_t*>(sums) + Sz::SUM_BYTES);
     uint8_t* table = reinterpret_cast<uint8_t*>(sh) + CT_BAR_BYTES;
     int2* ranges = reinterpret_cast<int2*>(table);
     uint32_t* words = reinterpret_cast<uint32_t*>(table + p.batch * 8);   // MASK: behind the ranges
@@ -206,17 +248,23 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int halves = p.dim > 64 ? 2 : 1;
 
     if (tid == 0) {
-        mbar_init(&sh->q_full, 1);
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < TILES; ++i) {
+            mbar_init(&sh->q_full[i], 1);
+            mbar_init(&sh->q_free[i], TILES);
+            for (int s = 0; s < 2; ++s) {
+                mbar_init(&sh->tile[i].s_full[s], 1);
+                mbar_init(&sh->tile[i].p_full[s], 4);
+                mbar_init(&sh->tile[i].pv_done[s], 1);
+            }
+            for (int s = 0; s < 3; ++s) mbar_init(&sh->tile[i].l_full[s], 4);
+            mbar_init(&sh->tile[i].o_free, 4);
+        }
+        for (int i = 0; i < CT_SLOTS; ++i) {
             mbar_init(&sh->k_full[i], 1);
             mbar_init(&sh->v_full[i], 1);
             mbar_init(&sh->vh_full[i], 1);
-            mbar_init(&sh->l_full[i], 4);
-            mbar_init(&sh->s_full[i], 1);
-            mbar_init(&sh->p_full[i], 4);
-            mbar_init(&sh->pv_done[i], 1);
+            mbar_init(&sh->vz_full[i], MASK ? 4 * TILES : 1);
         }
-        mbar_init(&sh->o_free, 4);
         sh->failed = 0;
         fence_mbar_init();
         prefetch_tmap(&tm_q);
@@ -224,18 +272,18 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         prefetch_tmap(&tm_v);
         prefetch_tmap(&tm_o);
     }
-    if (warp == CT_MMA_WARP) {
-        tmem_alloc(&sh->tmem_base, CT_TMEM_COLS);
+    if (warp == Sz::S_WARP) {
+        tmem_alloc(&sh->tmem_base, TILES * CT_TMEM_COLS);
         tmem_relinquish();
     }
     pdl_launch_dependents();
     pdl_wait();   // nothing above touches global memory
     // the samples' ranges and mask bits
     if constexpr (MASK) {
-        for (int b = tid; b < p.batch; b += CT_THREADS) ranges[b] = make_int2(0, 0);
+        for (int b = tid; b < p.batch; b += Sz::THREADS) ranges[b] = make_int2(0, 0);
         __syncthreads();
 #pragma unroll 1
-        for (int w = warp; w < p.batch * p.mask_words; w += CT_THREADS / 32) {
+        for (int w = warp; w < p.batch * p.mask_words; w += Sz::WARPS) {
             const int b = w / p.mask_words, at = (w - b * p.mask_words) * 32, i = at + lane;
             const uint32_t bits = __ballot_sync(0xffffffffu, i < p.st.kv_len && p.st.mask[b * p.st.mask_stride + i] != 0);
             if (lane == 0) {
@@ -244,7 +292,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
         }
     } else {
-        for (int b = tid; b < p.batch; b += CT_THREADS) {
+        for (int b = tid; b < p.batch; b += Sz::THREADS) {
             int2 r;
             cross_range(p.st, b, r.x, r.y);
             ranges[b] = r;
@@ -256,11 +304,11 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t tmem = sh->tmem_base;
     // This CTA's share: a run of items, cut so that the CTAs' costs are alike.  An item belongs to the CTA in whose span of the whole
     // cost its own begins.  (Every warp for itself, 32 samples a turn; a CTA's end and the next one's start are the same computation.)
-    const int per_batch = p.heads * p.q_tiles;
+    const int per_batch = p.units_h * p.units_t;
     int edge[2] = {static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.x) + 1};
     if (gridDim.x < p.items) {
         float total = 0.f;
-        for (int b = lane; b < p.batch; b += 32) total += cross_item_cost(ranges[b].y);
+        for (int b = lane; b < p.batch; b += 32) total += cross_item_cost<TILES>(ranges[b].y);
 #pragma unroll
         for (int m = 16; m >= 1; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
 #pragma unroll
@@ -273,7 +321,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll 1
             for (int b0 = 0; b0 < p.batch && blockIdx.x + e < gridDim.x; b0 += 32) {
                 const int b = b0 + lane;
-                const float c = b < p.batch ? cross_item_cost(ranges[b].y) : 0.f;
+                const float c = b < p.batch ? cross_item_cost<TILES>(ranges[b].y) : 0.f;
                 float to = c;   // cost up to and including sample b
 #pragma unroll 1
                 for (int m = 1; m < 32; m <<= 1) {
@@ -293,147 +341,191 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             else edge[1] = found;
         }
     }
-    const int b_first = edge[0] / per_batch, t_first = (edge[0] - b_first * per_batch) / p.heads, h_first = edge[0] - (b_first * p.q_tiles + t_first) * p.heads;
-    using Items = CrossItems<MASK>;
+    const int b_first = edge[0] / per_batch, t_first = (edge[0] - b_first * per_batch) / p.units_h,
+              h_first = edge[0] - (b_first * p.units_t + t_first) * p.units_h;
+    using Items = CrossItems<MASK, TILES>;
+    int* const failed = &sh->failed;
 #define CT_ITEMS(name) Items name(p, ranges, words, edge[0], edge[1], b_first, h_first, t_first)
 
-    if (warp >= 8) {
-        reg_dealloc<CT_REGS_OTHER>();
-        if (warp == CT_MMA_WARP) {
-            // ------------------------------------------------------------------ MMA issuer (the whole warp walks the loop, one elected lane issues)
-            const int ksteps = (p.dim + 15) >> 4;                    // of 16 channels; channels past the head read as zeros
-            const uint32_t idesc_pv = idesc_h16(CT_BM, 0, F16, true) | (static_cast<uint32_t>(ksteps * 2) << 17);
-            const uint64_t qd = smem_desc_sw128(smem_u32(q_s)), kd = smem_desc_sw128(smem_u32(k_s));
-            const uint64_t vd = smem_desc_sw128_mn(smem_u32(v_s), CT_KV_HALF, 1024);
-            const uint32_t hi_k = static_cast<uint32_t>(qd >> 32), hi_v = static_cast<uint32_t>(vd >> 32);
-            const uint32_t q_lo = static_cast<uint32_t>(qd), k_lo = static_cast<uint32_t>(kd), v_lo = static_cast<uint32_t>(vd);
-            // Two walks over the blocks: `s` for Q K^T, up to one block ahead inside an item, and `o` for P V.  (Each product is issued at
-            // one place: the kernel's code has to stay in the instruction caches with five roles at work.)
-            CT_ITEMS(s);
-            CT_ITEMS(o);
-            int sj = 0, oj = 0;
-            uint32_t m = 0, n = 0, s_items = 0, o_items = 0, plain = 0;   // blocks and items so far; plain: phase bit of v_full per slot
-            bool s_there = true;
-            while (true) {
-                if (sj == s.blocks && s_there) {
-                    sj = 0;
-                    s_there = s.advance();
-                }
-                if (oj == o.blocks) {
-                    oj = 0;
-                    if (!o.advance()) break;
-                    ++o_items;
-                }
-                // S = Q K_j^T over the block's states, rounded up to 16: now if no scores are left to work on, ahead of P V if K has landed
-                const bool landed = s_there && m == n + 1 && s.item == o.item && __all_sync(0xffffffffu, mbar_test_wait(&sh->k_full[m & 1], (m >> 1) & 1));
-                if (landed || (s_there && m == n)) {
-                    if (sj == 0 && !ct_wait(&sh->q_full, s_items++ & 1, sh, 910)) break;
-                    if (!landed && !ct_wait(&sh->k_full[m & 1], (m >> 1) & 1, sh, 911)) break;
+    if (warp >= Sz::S_WARP) {
+        reg_dealloc<Sz::REGS_OTHER>();
+        const int ksteps = (p.dim + 15) >> 4;                    // of 16 channels; channels past the head read as zeros
+        if (warp < Sz::PV_WARP) {
+            // -------------------------------------------------------------- issuer of a tile's Q K^T (the whole warp walks the loop, one elected lane
+            // issues).  The two products have a warp each: an MMA of these sizes takes longer to issue than to run.
+            const int tile = TILES == 1 ? 0 : warp - Sz::S_WARP;
+            auto& bar = sh->tile[tile];
+            const uint32_t s_tmem = tmem + tile * CT_TMEM_COLS;
+            const uint64_t qd = smem_desc_sw128(smem_u32(q_s + tile * CT_Q_BYTES)), kd = smem_desc_sw128(smem_u32(k_s));
+            const uint32_t hi = static_cast<uint32_t>(qd >> 32), q_lo = static_cast<uint32_t>(qd), k_lo = static_cast<uint32_t>(kd);
+            CT_ITEMS(it);
+            uint32_t n = 0, items = 0;
+            bool ok = true;
+            while (ok && it.advance()) {
+                const uint32_t q_buf = items % Sz::Q_BUFFERS, q0 = q_lo + q_buf * (TILES * CT_Q_BYTES >> 4);
+                if (!ct_wait(&sh->q_full[q_buf], (items / Sz::Q_BUFFERS) & 1, failed, 910)) break;
+                ++items;
+#pragma unroll 1
+                for (int j = 0; j < it.blocks; ++j, ++n) {
+                    const uint32_t slot = n & 1;
+                    // S = Q K_j^T over the block's states, rounded up to 16, where P of two blocks ago was
+                    if (!(ok = ct_wait(&sh->k_full[slot], (n >> 1) & 1, failed, 911) && (n < 2 || ct_wait(&bar.pv_done[slot], ((n - 2) >> 1) & 1, failed, 912))))
+                        break;
                     tc_fence_after_sync();
-                    const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((s.valid(sj) + 15) >> 4) << 18);
-                    const uint32_t d = tmem + (m & 1) * CT_BN, k0 = k_lo + (m & 1) * (CT_KV_BYTES >> 4);
+                    const uint32_t idesc = idesc_h16(CT_BM, 0, F16, false) | (static_cast<uint32_t>((it.valid(j) + 15) >> 4) << 18);
+                    const uint32_t d = s_tmem + slot * CT_BN, k0 = k_lo + slot * (CT_KV_BYTES >> 4);
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
                             if (kk < ksteps)
-                                tc_mma_f16_lo(d, q_lo + (kk >> 2) * (CT_Q_HALF >> 4) + (kk & 3) * 2, k0 + (kk >> 2) * (CT_KV_HALF >> 4) + (kk & 3) * 2, hi_k,
+                                tc_mma_f16_lo(d, q0 + (kk >> 2) * (CT_Q_HALF >> 4) + (kk & 3) * 2, k0 + (kk >> 2) * (CT_KV_HALF >> 4) + (kk & 3) * 2, hi,
                                               idesc, kk > 0);
-                        tc_commit(&sh->s_full[m & 1]);
+                        tc_commit(&bar.s_full[slot]);
+                        if (j + 1 == it.blocks) tc_commit(&sh->q_free[q_buf]);
                     }
                     __syncwarp();
-                    ++m;
-                    ++sj;
-                    if (m == n + 1) continue;   // look for one more
                 }
-                const uint32_t slot = n & 1;
-                if (oj == 0 && o_items > 1 && !ct_wait(&sh->o_free, o_items & 1, sh, 915)) break;   // the previous item's O has been read
-                if (!o.holes(oj)) {   // otherwise P is only handed over behind it
-                    if (!ct_wait(&sh->v_full[slot], (plain >> slot) & 1, sh, 920)) break;
-                    plain ^= 1u << slot;
-                }
-                if (!ct_wait(&sh->p_full[slot], (n >> 1) & 1, sh, 930)) break;
-                tc_fence_after_sync();
-                const int steps = (o.valid(oj) + 15) >> 4;
-                const uint32_t a = tmem + slot * CT_BN, v0 = v_lo + slot * (CT_KV_BYTES >> 4);
-                if (elect_one()) {
-#pragma unroll
-                    for (int k4 = 0; k4 < 4; ++k4)
-                        if (k4 < steps) tc_mma_f16_ts_lo(tmem + 2 * CT_BN, a + k4 * 8, v0 + k4 * 128, hi_v, idesc_pv, (oj | k4) ? 1u : 0u);
-                    tc_commit(&sh->pv_done[slot]);
-                }
-                __syncwarp();
-                ++n;
-                ++oj;
             }
-        } else if (warp == CT_QK_WARP || warp == CT_V_WARP) {
-            // ------------------------------------------------------------------ producers: one warp for Q and K, one for V (the copies of one issuing
-            // warp are worked off one after the other)
-            const bool v_warp = warp == CT_V_WARP;
-            const CUtensorMap* map = v_warp ? &tm_v : &tm_k;
-            uint64_t* free_bar = v_warp ? sh->pv_done : sh->s_full;
+        } else if (warp < Sz::QK_WARP) {
+            // -------------------------------------------------------------- issuer of a tile's P V
+            const int tile = TILES == 1 ? 0 : warp - Sz::PV_WARP;
+            auto& bar = sh->tile[tile];
+            const uint32_t t_tmem = tmem + tile * CT_TMEM_COLS;
+            const uint32_t idesc = idesc_h16(CT_BM, 0, F16, true) | (static_cast<uint32_t>(ksteps * 2) << 17);
+            const uint64_t vd = smem_desc_sw128_mn(smem_u32(v_s), CT_KV_HALF, 1024);
+            const uint32_t hi = static_cast<uint32_t>(vd >> 32), v_lo = static_cast<uint32_t>(vd);
             CT_ITEMS(it);
-            uint32_t n = 0, items = 0;
-            uint32_t used = 0, phase = 0;   // per slot and kind of V block (bit 2 * slot + holes): any copy yet, and the next one's phase bit
-            auto full_of = [&](int slot, int holes) { return (!v_warp ? sh->k_full : holes ? sh->vh_full : sh->v_full) + slot; };
+            uint32_t n = 0, items = 0, phase = 0;   // phase: bits of v_full and vz_full per slot
             bool ok = true;
             while (ok && it.advance()) {
-                const int kv_head = it.head / p.group;
-                if (!v_warp) {
-                    // block n - 1 was the previous item's last
-                    if (n > 0 && !ct_wait(&sh->s_full[(n - 1) & 1], ((n - 1) >> 1) & 1, sh, 900)) break;
-                    ++items;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&sh->q_full, halves * CT_Q_HALF);
+                ++items;
 #pragma unroll 1
-                        for (int h = 0; h < halves; ++h)
-                            tma_load_4d(q_s + h * CT_Q_HALF, &tm_q, &sh->q_full, h * 64, it.tile * CT_BM, it.head * p.q_hmul, it.batch * p.q_bmul);
+                for (int j = 0; j < it.blocks; ++j, ++n) {
+                    const uint32_t slot = n & 1;
+                    const int up = (it.valid(j) + 15) & ~15;
+                    const uint32_t kind = 2 * slot + it.holes(j);   // bit of `phase`
+                    if constexpr (!MASK)   // rows of V behind the last state -> zeros
+                        if (tile == 0 && (kind & 1)) {
+                            if (!(ok = ct_wait(&sh->vh_full[slot], (phase >> kind) & 1, failed, 950))) break;
+                            zero_rows(it, v_s + slot * CT_KV_BYTES, j, halves, it.valid(j) + (lane >> 3), 4, lane);
+                            if (lane == 0) mbar_arrive(&sh->vz_full[slot]);
+                            __syncwarp();
+                        }
+                    uint64_t* v_there = (kind & 1 ? sh->vz_full : sh->v_full) + slot;
+                    if (!(ok = (j > 0 || items == 1 || ct_wait(&bar.o_free, items & 1, failed, 915)) &&   // the previous item's O has been read
+                               ct_wait(v_there, (phase >> kind) & 1, failed, 920) && ct_wait(&bar.p_full[slot], (n >> 1) & 1, failed, 930)))
+                        break;
+                    phase ^= 1u << kind;
+                    tc_fence_after_sync();
+                    const uint32_t a = t_tmem + slot * CT_BN, v0 = v_lo + slot * (CT_KV_BYTES >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k4 = 0; k4 < 4; ++k4)
+                            if (k4 * 16 < up) tc_mma_f16_ts_lo(t_tmem + 2 * CT_BN, a + k4 * 8, v0 + k4 * 128, hi, idesc, (j | k4) ? 1u : 0u);
+                        tc_commit(&bar.pv_done[slot]);
                     }
                     __syncwarp();
                 }
-                const int z = kv_head * (v_warp ? p.v_hmul : p.k_hmul), w = p.st.kv_offsets ? 0 : it.batch * (v_warp ? p.v_bmul : p.k_bmul);
+            }
+        } else if (warp == Sz::QK_WARP) {
+            // -------------------------------------------------------------- producer of Q and K (the copies of one issuing warp are worked off one
+            // after the other, so that V has its own)
+            CT_ITEMS(qi);
+            CT_ITEMS(it);
+            uint32_t n = 0, items = 0;   // blocks of K, items of Q asked for
+            // the next item's queries, if there is one, as soon as the buffer's last user is through with it
+            auto load_q = [&]() {
+                if (!qi.advance()) return true;
+                const uint32_t buf = items % Sz::Q_BUFFERS;
+                if (items >= Sz::Q_BUFFERS && !ct_wait(&sh->q_free[buf], (items / Sz::Q_BUFFERS - 1) & 1, failed, 900)) return false;
+                ++items;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sh->q_full[buf], TILES * halves * CT_Q_HALF);
+#pragma unroll 1
+                    for (int t = 0; t < TILES; ++t)
+#pragma unroll 1
+                        for (int h = 0; h < halves; ++h)
+                            tma_load_4d(q_s + (buf * TILES + t) * CT_Q_BYTES + h * CT_Q_HALF, &tm_q, &sh->q_full[buf], h * 64, qi.tile(t) * CT_BM,
+                                        qi.head(t) * p.q_hmul, qi.batch * p.q_bmul);
+                }
+                __syncwarp();
+                return true;
+            };
+            bool ok = TILES == 1 || load_q();
+            while (ok && it.advance()) {
+                if (TILES == 1 && !(ok = load_q())) break;
+                const int z = it.head(0) / p.group * p.k_hmul, w = p.st.kv_offsets ? 0 : it.batch * p.k_bmul;
                 for (int j = 0; j < it.blocks; ++j, ++n) {
                     const int slot = n & 1;
-                    if (n > 1 && !ct_wait(free_bar + slot, ((n - 2) >> 1) & 1, sh, 901 + v_warp)) {
-                        ok = false;
-                        break;
-                    }
-                    const int holes = v_warp && it.holes(j);
-                    used |= 1u << (2 * slot + holes);
-                    phase ^= 1u << (2 * slot + holes);
+                    for (int t = 0; t < TILES && ok; ++t) ok = n < 2 || ct_wait(&sh->tile[t].s_full[slot], ((n - 2) >> 1) & 1, failed, 901);
+                    if (!ok) break;
                     if (lane == 0) {
-                        uint64_t* full = full_of(slot, holes);
-                        uint8_t* to = (v_warp ? v_s : k_s) + slot * CT_KV_BYTES;
-                        mbar_arrive_expect_tx(full, halves * CT_KV_HALF);
+                        mbar_arrive_expect_tx(&sh->k_full[slot], halves * CT_KV_HALF);
 #pragma unroll 1
-                        for (int h = 0; h < halves; ++h) tma_load_4d(to + h * CT_KV_HALF, map, full, h * 64, it.start + j * CT_BN, z, w);
+                        for (int h = 0; h < halves; ++h)
+                            tma_load_4d(k_s + slot * CT_KV_BYTES + h * CT_KV_HALF, &tm_k, &sh->k_full[slot], h * 64, it.start + j * CT_BN, z, w);
                     }
                     __syncwarp();
+                    // behind the second block, whose slot says that the previous item's Q K^T are done
+                    if (TILES == 2 && j == min(1, it.blocks - 1) && !(ok = load_q())) {
+                        ++n;
+                        break;
+                    }
                 }
             }
             // leave with none of this warp's copies in flight (where all went well they have all been waited for)
-            if (items) ct_wait(&sh->q_full, (items & 1) ^ 1, sh, 903);
+            for (uint32_t i = items > Sz::Q_BUFFERS ? items - Sz::Q_BUFFERS : 0; i < items; ++i)
+                ct_wait(&sh->q_full[i % Sz::Q_BUFFERS], (i / Sz::Q_BUFFERS) & 1, failed, 903);
+            for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i) ct_wait(&sh->k_full[i & 1], (i >> 1) & 1, failed, 904);
+        } else if (warp == Sz::V_WARP) {
+            // -------------------------------------------------------------- producer of V
+            CT_ITEMS(it);
+            uint32_t n = 0, used = 0, phase = 0;   // blocks; per slot and kind (bit 2 * slot + holes): any copy yet, and the next one's phase bit
+            bool ok = true;
+            while (ok && it.advance()) {
+                const int z = it.head(0) / p.group * p.v_hmul, w = p.st.kv_offsets ? 0 : it.batch * p.v_bmul;
+                for (int j = 0; j < it.blocks; ++j, ++n) {
+                    const int slot = n & 1;
+                    for (int t = 0; t < TILES && ok; ++t) ok = n < 2 || ct_wait(&sh->tile[t].pv_done[slot], ((n - 2) >> 1) & 1, failed, 902);
+                    if (!ok) break;
+                    const bool holes = it.holes(j);
+                    used |= 1u << (2 * slot + holes);
+                    phase ^= 1u << (2 * slot + holes);
+                    if (lane == 0) {
+                        uint64_t* full = (holes ? sh->vh_full : sh->v_full) + slot;
+                        mbar_arrive_expect_tx(full, halves * CT_KV_HALF);
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i)
-                if ((used >> i) & 1u) ct_wait(full_of(i >> 1, i & 1), ((phase >> i) & 1u) ^ 1u, sh, 904);
+                        for (int h = 0; h < halves; ++h) tma_load_4d(v_s + slot * CT_KV_BYTES + h * CT_KV_HALF, &tm_v, full, h * 64, it.start + j * CT_BN, z, w);
+                    }
+                    __syncwarp();
+                }
+            }
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i)   // as above
+                if ((used >> i) & 1u) ct_wait((i & 1 ? sh->vh_full : sh->v_full) + (i >> 1), ((phase >> i) & 1u) ^ 1u, failed, 905);
         }
-    } else if (warp >= 4) {
-        reg_dealloc<CT_REGS_OUTPUT>();
+    } else if (warp >= Sz::OUT_WARP) {
+        reg_dealloc<Sz::REGS_OUTPUT>();
         // ------------------------------------------------------------------ output: O / l -> global memory, while the softmax warps are at the
         // next item already
-        const int quad = warp & 3;
-        const uint32_t o_tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 2 * CT_BN;
-        uint8_t* box = stage + quad * (CT_STAGE_BYTES / 4);   // [32 rows][64 bytes], 16-byte pieces swizzled by row / 2
+        const int quad = warp & 3, tile = TILES == 1 ? 0 : (warp - Sz::OUT_WARP) >> 2;
+        auto& bar = sh->tile[tile];
+        const uint32_t o_tmem = tmem + tile * CT_TMEM_COLS + (static_cast<uint32_t>(quad * 32) << 16) + 2 * CT_BN;
+        uint8_t* box = stage + (warp - Sz::OUT_WARP) * (CT_STAGE_BYTES / 4);   // [32 rows][64 bytes], 16-byte pieces swizzled by row / 2
         CT_ITEMS(it);
-        uint32_t n = 0, done = 0;   // blocks and items with states so far
+        uint32_t n = 0, at = 0, phase = 0;   // blocks so far; the item's buffer of sums, phase bit of its barrier
         while (it.template advance<true>()) {
             n += it.blocks;
-            const int row0 = it.tile * CT_BM + quad * 32;
+            const int row0 = it.tile(tile) * CT_BM + quad * 32;
             float inv = 0.f;
             if (it.blocks) {
                 const uint32_t last = n - 1;
-                if (!ct_wait(&sh->l_full[done & 1], (done >> 1) & 1, sh, 980) || !ct_wait(&sh->pv_done[last & 1], (last >> 1) & 1, sh, 981)) break;
-                inv = 1.f / sums[(done & 1) * CT_BM + quad * 32 + lane];
-                ++done;
+                if (!ct_wait(&bar.l_full[at], phase, failed, 980) || !ct_wait(&bar.pv_done[last & 1], (last >> 1) & 1, failed, 981)) break;
+                inv = 1.f / sums[(at * TILES + tile) * CT_BM + quad * 32 + lane];
+                if (++at == 3) {
+                    at = 0;
+                    phase ^= 1;
+                }
                 tc_fence_after_sync();
             }
 #pragma unroll 1
@@ -445,7 +537,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     if (c + 32 >= p.dim) {   // all of O has been read: the next item's P V may overwrite it
                         tc_fence_before_sync();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh->o_free);
+                        if (lane == 0) mbar_arrive(&bar.o_free);
                     }
                 } else {
 #pragma unroll
@@ -466,7 +558,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {   // rows behind the last and channels past the head are cut off by the copy
-                    if (row0 < p.q_len) tma_store_4d(&tm_o, box, c, row0, it.head * p.o_hmul, it.batch * p.o_bmul);
+                    if (row0 < p.q_len) tma_store_4d(&tm_o, box, c, row0, it.head(tile) * p.o_hmul, it.batch * p.o_bmul);
                     bulk_commit_group();
                 }
                 __syncwarp();
@@ -475,9 +567,11 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (lane == 0) bulk_wait_group<0>();
         __syncwarp();
     } else {
-        reg_alloc<CT_REGS_SOFTMAX>();
+        reg_alloc<Sz::REGS_SOFTMAX>();
         // ------------------------------------------------------------------ softmax: thread = one query row
-        const uint32_t s_tmem = tmem + (static_cast<uint32_t>(warp * 32) << 16), o_tmem = s_tmem + 2 * CT_BN;
+        const int quad = warp & 3, tile = TILES == 1 ? 0 : warp >> 2;
+        auto& bar = sh->tile[tile];
+        const uint32_t s_tmem = tmem + tile * CT_TMEM_COLS + (static_cast<uint32_t>(quad * 32) << 16), o_tmem = s_tmem + 2 * CT_BN;
         const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
         // 32 states -> 16 columns of packed 16-bit pairs, and their sum
         auto exp32 = [&](const uint32_t (&a)[32], float m, uint32_t (&w)[16]) {
@@ -494,15 +588,15 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             return (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
         };
-        auto max32 = [&](const uint32_t (&a)[32], float m0) {   // and of m0
-            float m1 = __uint_as_float(a[0]);
+        auto max32 = [&](const uint32_t (&a)[32], float least) {   // and of `least`
+            float m[4] = {least, __uint_as_float(a[0]), __uint_as_float(a[1]), __uint_as_float(a[2])};
 #pragma unroll
-            for (int i = 1; i < 29; i += 4) {
-                m0 = max3_nan(m0, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
-                m1 = max3_nan(m1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
-            }
-            m1 = max3_nan(m1, __uint_as_float(a[29]), __uint_as_float(a[30]));
-            return max3_nan(m0, m1, __uint_as_float(a[31]));
+            for (int i = 3; i < 27; i += 8)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) m[c] = max3_nan(m[c], __uint_as_float(a[i + 2 * c]), __uint_as_float(a[i + 2 * c + 1]));
+            m[0] = max3_nan(m[0], __uint_as_float(a[27]), __uint_as_float(a[28]));
+            m[1] = max3_nan(m[1], __uint_as_float(a[29]), __uint_as_float(a[30]));
+            return max3_nan(m[0], max3_nan(m[1], m[2], m[3]), __uint_as_float(a[31]));
         };
         auto hide = [&](uint32_t (&a)[32], uint32_t bits) {
             if (bits != 0xffffffffu) {
@@ -512,7 +606,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
         };
         CT_ITEMS(it);
-        uint32_t n = 0, done = 0, hole_phase = 0;   // blocks, items with states; hole_phase: phase bit of vh_full per slot
+        uint32_t n = 0, at = 0, hole_phase = 0;   // blocks; the item's buffer of sums; phase bits of vh_full per slot
         bool ok = true;
         while (ok && it.advance()) {
             float m_used = 0.f, l = 0.f;
@@ -520,7 +614,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             for (int j = 0; j < it.blocks; ++j, ++n) {
                 const uint32_t slot = n & 1, st = s_tmem + slot * CT_BN;
                 const int valid = it.valid(j);
-                if (!(ok = ct_wait(&sh->s_full[slot], (n >> 1) & 1, sh, 960))) break;
+                if (!(ok = ct_wait(&bar.s_full[slot], (n >> 1) & 1, failed, 960))) break;
                 tc_fence_after_sync();
                 // Scores that do not count are replaced by -inf (selected, not added: they may be anything).
                 uint32_t a0[32], a1[32], w[16];
@@ -541,7 +635,7 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     m_used = ms;
                 } else if (const bool grow = !(ms <= m_used + CT_RESCALE_STEP); __any_sync(0xffffffffu, grow)) {
                     // O is written by the previous P V product until it has completed
-                    if (!(ok = ct_wait(&sh->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, sh, 970))) break;
+                    if (!(ok = ct_wait(&bar.pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, failed, 970))) break;
                     tc_fence_after_sync();
                     const float alpha = grow ? ex2(m_used - ms) : 1.f;
                     l *= alpha;
@@ -563,32 +657,26 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     l += exp32(a1, m_used, w);
                     tc_st_32x32b_x16(st + 16, w);
                 }
-                if (it.holes(j)) {   // rows of V that must not be seen -> zeros: four rows per warp and turn, eight lanes per row (and half)
-                    if (!(ok = ct_wait(&sh->vh_full[slot], (hole_phase >> slot) & 1, sh, 950))) break;
-                    hole_phase ^= 1u << slot;
-                    const int up = (valid + 15) & ~15;
-#pragma unroll 1
-                    for (int r = (MASK ? 0 : valid & ~15) + warp * 4 + (lane >> 3); r < up; r += 16) {
-                        bool zero = r >= valid;
-                        if constexpr (MASK) zero = !((it.bits(j)[r >> 5] >> (r & 31)) & 1u);
-                        if (zero)
-                            for (int h = 0; h < halves; ++h)
-                                *reinterpret_cast<uint4*>(v_s + slot * CT_KV_BYTES + h * CT_KV_HALF + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                if constexpr (MASK)
+                    if (it.holes(j)) {
+                        if (!(ok = ct_wait(&sh->vh_full[slot], (hole_phase >> slot) & 1, failed, 950))) break;
+                        hole_phase ^= 1u << slot;
+                        zero_rows(it, v_s + slot * CT_KV_BYTES, j, halves, warp * 4 + (lane >> 3), 16 * TILES, lane);
+                        if (lane == 0) mbar_arrive(&sh->vz_full[slot]);
                     }
-                    fence_proxy_async_smem();
-                }
                 tc_wait_st();
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->p_full[slot]);
+                if (lane == 0) mbar_arrive(&bar.p_full[slot]);
             }
             if (!ok) break;
-            // Two buffers (and barriers) in turn: an item's P V waits until the output warps have read the previous item's O and sums, and
-            // the scores of the item after it come behind that P V; so the buffer written here was read two items ago.
-            sums[(done & 1) * CT_BM + warp * 32 + lane] = l;
+            // Three buffers (and barriers) in turn.  The scores of this item's last block were only asked for when all but the last of the P V
+            // ahead of them were done; with one block per item that is the P V of the item two ahead, which waited until the output warps had
+            // read O and sums of the item three ahead: whose buffer and barrier these are.
+            sums[(at * TILES + tile) * CT_BM + quad * 32 + lane] = l;
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->l_full[done & 1]);
-            ++done;
+            if (lane == 0) mbar_arrive(&bar.l_full[at]);
+            at = at == 2 ? 0 : at + 1;
         }
     }
 #undef CT_ITEMS
@@ -598,9 +686,9 @@ cross_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         atomicExch(&p.status[0], SVDQ_ERR_TIMEOUT);
         atomicExch(&p.status[1], sh->failed);
     }
-    if (warp == CT_MMA_WARP) {
+    if (warp == Sz::S_WARP) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem, CT_TMEM_COLS);
+        tmem_dealloc(tmem, TILES * CT_TMEM_COLS);
     }
 }
 
@@ -965,16 +1053,16 @@ static int cross_tmap(CUtensorMap* map, const CrossTensor& t, int dim, int dtype
                         box, box_channels == 64 ? 128 : 64);
 }
 
-template <bool F16, bool MASK>
-static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const CrossTileParams& p, int grid, int table_bytes,
-                             cudaStream_t stream) {
-    auto kern = cross_tile_kernel<F16, MASK>;
+template <bool F16, bool MASK, int TILES>
+static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const CrossTileParams& p, int sms, cudaStream_t stream) {
+    using Sz = CrossTileSizes<TILES>;
+    auto kern = cross_tile_kernel<F16, MASK, TILES>;
     static std::atomic<uint64_t> attr_done{0};
-    if (int rc = ensure_dynamic_smem(kern, CT_SMEM + CT_TABLE_BYTES, attr_done)) return rc;
+    if (int rc = ensure_dynamic_smem(kern, Sz::SMEM + CT_TABLE_BYTES, attr_done)) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(CT_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = CT_SMEM + table_bytes;
+    cfg.gridDim = dim3(p.items < Sz::PER_SM * sms ? p.items : Sz::PER_SM * sms, 1, 1);   // all resident; each works through its share of the items
+    cfg.blockDim = dim3(Sz::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = Sz::SMEM + p.batch * (8 + 4 * p.mask_words);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // the prologue may run under the predecessor's tail
@@ -983,6 +1071,11 @@ static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const
     cfg.numAttrs = 1;
     SVDQ_CUDA(cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, to, p));
     return SVDQ_OK;
+}
+template <bool F16, bool MASK>
+static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const CrossTileParams& p, int tiles, int sms,
+                             cudaStream_t stream) {
+    return tiles == 2 ? launch_cross_tile<F16, MASK, 2>(tq, tk, tv, to, p, sms, stream) : launch_cross_tile<F16, MASK, 1>(tq, tk, tv, to, p, sms, stream);
 }
 
 template <bool F16, int NK>
@@ -1113,6 +1206,10 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
     const int mask_words = a->mask ? (a->kv_len + CT_BN - 1) / CT_BN * (CT_BN / 32) : 0;
     const int most = CT_TABLE_BYTES / (8 + 4 * mask_words);
     SVDQ_CHECK_ARG(static_cast<long long>(a->heads) * q_tiles * (a->batch < most ? a->batch : most) < (1ll << 30), "cross_attention: too many query tiles");
+    // Two tiles over the same states where there are more tiles than places for one-tile CTAs and they go into pairs, of one head or of two that
+    // share a stored head (one tile / two, us: 32 x 20 x 1024 x 192 x 112 104 / 93, x 320 171 / 136, x 64 65 / 69; 3 x 20 x 1024 x 300 x 112 23 / 21;
+    // with fewer tiles, 1 x 20 x 1000 x 77 x 64 6.7 / 7.2; with a tile twice to make nine a pair, 32 x 20 x 1152 x 200 x 112 115 / 122).
+    const int tiles_at_once = q_items > 2 * sms && (group % 2 == 0 || q_tiles % 2 == 0) ? 2 : 1;
     for (int b0 = 0; b0 < a->batch; b0 += most) {
         const int nb = a->batch - b0 < most ? a->batch - b0 : most;
         auto from = [&](CrossTensor t, int count) {
@@ -1132,19 +1229,20 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args* a, void* st
         p.group = group;
         p.scale_log2 = scale_log2;
         if (int rc = status_words(&p.status)) return rc;
-        p.heads = a->heads;
         p.q_tiles = q_tiles;
         p.batch = nb;
-        p.items = nb * a->heads * q_tiles;
+        p.pair_heads = group % 2 == 0;
+        p.units_h = tiles_at_once == 2 && p.pair_heads ? a->heads / 2 : a->heads;
+        p.units_t = tiles_at_once == 2 && !p.pair_heads ? q_tiles / 2 : q_tiles;
+        p.items = nb * p.units_h * p.units_t;
         p.mask_words = mask_words;
         CUtensorMap mq, mk, mv, mo;
         if (int rc = cross_tmap(&mq, from(tq, 1), a->head_dim, a->dtype, CT_BM, &p.q_bmul, &p.q_hmul)) return rc;
         if (int rc = cross_tmap(&mk, from(tk, !a->kv_offsets), a->head_dim, a->dtype, CT_BN, &p.k_bmul, &p.k_hmul)) return rc;
         if (int rc = cross_tmap(&mv, from(tv, !a->kv_offsets), a->head_dim, a->dtype, CT_BN, &p.v_bmul, &p.v_hmul)) return rc;
         if (int rc = cross_tmap(&mo, from(to, 1), a->head_dim, a->dtype, 32, &p.o_bmul, &p.o_hmul, 32)) return rc;
-        const int grid = p.items < 2 * sms ? p.items : 2 * sms, bytes = nb * (8 + 4 * mask_words);   // two CTAs per SM work through the items
-        const int rc = a->mask ? (f16 ? launch_cross_tile<true, true>(mq, mk, mv, mo, p, grid, bytes, st) : launch_cross_tile<false, true>(mq, mk, mv, mo, p, grid, bytes, st))
-                               : (f16 ? launch_cross_tile<true, false>(mq, mk, mv, mo, p, grid, bytes, st) : launch_cross_tile<false, false>(mq, mk, mv, mo, p, grid, bytes, st));
+        const int rc = a->mask ? (f16 ? launch_cross_tile<true, true>(mq, mk, mv, mo, p, tiles_at_once, sms, st) : launch_cross_tile<false, true>(mq, mk, mv, mo, p, tiles_at_once, sms, st))
+                               : (f16 ? launch_cross_tile<true, false>(mq, mk, mv, mo, p, tiles_at_once, sms, st) : launch_cross_tile<false, false>(mq, mk, mv, mo, p, tiles_at_once, sms, st));
         if (rc) return rc;
     }
     return SVDQ_OK;

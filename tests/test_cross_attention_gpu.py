@@ -69,7 +69,9 @@ SIZES = [(1, 1, 1, 1, 1, 8), (1, 20, 20, 1, 300, 112), (3, 4, 2, 1, 65, 128), (2
          (1, 2, 1, 64, 190, 24), (1, 1, 1, 100, 1153, 80), (3, 1, 1, 40, 64, 48), (1, 2, 2, 70, 192, 104),
          # row tiles of 16 over long lists, split; many heads: 128-row tiles over several blocks (which of the two runs goes by their times)
          (1, 4, 2, 40, 1000, 72), (2, 6, 2, 30, 700, 128), (1, 1, 1, 500, 900, 32), (1, 16, 16, 140, 300, 112), (1, 16, 4, 150, 257, 128),
-         (2, 32, 32, 150, 300, 64), (2, 32, 8, 129, 520, 40), (4, 40, 40, 20, 200, 96)]
+         (2, 32, 32, 150, 300, 64), (2, 32, 8, 129, 520, 40), (4, 40, 40, 20, 200, 96),
+         # more 128-row tiles than there are places: two at a time over the same states, of one head or of two that share a stored one
+         (2, 80, 80, 150, 300, 112), (1, 160, 80, 129, 130, 72), (3, 60, 60, 256, 64, 128), (1, 310, 155, 100, 200, 24), (5, 20, 20, 500, 65, 16)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -83,7 +85,7 @@ def test_all_states(B, H, Hk, Tq, T, D, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("Tq", [1, 5, 150])
-@pytest.mark.parametrize("H,Hk,T,D", [(2, 2, 300, 112), (4, 2, 128, 64), (3, 3, 700, 128), (2, 1, 40, 32)])
+@pytest.mark.parametrize("H,Hk,T,D", [(2, 2, 300, 112), (4, 2, 128, 64), (3, 3, 700, 128), (2, 1, 40, 32), (18, 18, 300, 112), (20, 10, 200, 24)])
 def test_lengths_with_nan_behind_them(Tq, H, Hk, T, D, dtype):
     from nunchaku_b200.ops import cross_attention
 
@@ -104,7 +106,7 @@ def test_lengths_with_nan_behind_them(Tq, H, Hk, T, D, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("Tq", [1, 3, 140, 300])
-@pytest.mark.parametrize("H,Hk,T,D", [(2, 2, 77, 64), (2, 1, 520, 112), (1, 1, 1, 128), (4, 4, 300, 32)])
+@pytest.mark.parametrize("H,Hk,T,D", [(2, 2, 77, 64), (2, 1, 520, 112), (1, 1, 1, 128), (4, 4, 300, 32), (22, 22, 200, 64), (24, 12, 450, 96)])
 def test_masks(Tq, H, Hk, T, D, dtype):
     from nunchaku_b200.ops import cross_attention
 
@@ -132,7 +134,7 @@ def test_masks(Tq, H, Hk, T, D, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("Tq", [1, 6, 200])
-@pytest.mark.parametrize("H,Hk,D", [(2, 2, 112), (4, 2, 64), (3, 1, 128)])
+@pytest.mark.parametrize("H,Hk,D", [(2, 2, 112), (4, 2, 64), (3, 1, 128), (20, 20, 112), (20, 10, 40)])
 def test_packed(Tq, H, Hk, D, dtype):
     from nunchaku_b200.ops import cross_attention
 
@@ -162,7 +164,7 @@ def test_packed(Tq, H, Hk, D, dtype):
     assert _lib.device_status() == (0, 0)
 
 
-@pytest.mark.parametrize("Tq,H", [(2, 4), (130, 4), (130, 32)])
+@pytest.mark.parametrize("Tq,H", [(2, 4), (130, 4), (130, 32), (130, 100)])
 def test_layouts(Tq, H):
     """head-major, token-major, broadcast over batch or heads, an output inside a wider buffer"""
     from nunchaku_b200.ops import cross_attention
@@ -187,7 +189,7 @@ def test_layouts(Tq, H):
     assert torch.equal(hm.transpose(1, 2).reshape(B, Tq, H * D), ref)
 
 
-@pytest.mark.parametrize("Tq,H", [(1, 2), (150, 2), (150, 16)])
+@pytest.mark.parametrize("Tq,H", [(1, 2), (150, 2), (150, 16), (150, 80)])
 def test_growing_scores_and_large_scale(Tq, H):
     """the maximum rises from block to block by far more than the rescaling step; nearly one-hot weights"""
     from nunchaku_b200.ops import cross_attention
@@ -204,7 +206,7 @@ def test_growing_scores_and_large_scale(Tq, H):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32)])
+@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32), (140, 80)])
 def test_a_bad_state_that_is_to_be_seen_is_not_hidden(Tq, H, dtype):
     """a NaN in one state of K (at every place of a block in turn) or V shows in every row that sees it, and nowhere else"""
     from nunchaku_b200.ops import cross_attention
@@ -226,7 +228,7 @@ def test_a_bad_state_that_is_to_be_seen_is_not_hidden(Tq, H, dtype):
             assert torch.equal(got[0], clean[at][0]) and torch.equal(got[1, :, :(H - 1) * D], clean[at][1, :, :(H - 1) * D])
 
 
-@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32)])
+@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32), (140, 160)])
 def test_states_of_minus_infinity(Tq, H):
     """scores of -inf (whole blocks of them, ahead of others and behind) weigh nothing"""
     from nunchaku_b200.ops import cross_attention
@@ -244,7 +246,7 @@ def test_states_of_minus_infinity(Tq, H):
         _check(cross_attention(q, k2, v), q, k3, v, keep2, D ** -0.5)
 
 
-@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32)])
+@pytest.mark.parametrize("Tq,H", [(3, 2), (140, 32), (140, 160)])
 @pytest.mark.parametrize("masked", [False, True])
 def test_scores_of_the_largest_magnitudes(Tq, H, masked):
     """scores down to -1e37: the state of the largest alone is seen, wherever it stands"""
@@ -269,7 +271,7 @@ def test_two_calls_at_once():
     from nunchaku_b200.ops import cross_attention
 
     cases = [_inputs(2, 4, 4, 1, 900, 112, torch.bfloat16, seed=1), _inputs(2, 20, 20, 300, 300, 112, torch.bfloat16, seed=2),
-             _inputs(2, 20, 20, 300, 300, 112, torch.bfloat16, seed=3)]
+             _inputs(2, 20, 20, 300, 300, 112, torch.bfloat16, seed=3), _inputs(2, 80, 80, 256, 300, 112, torch.bfloat16, seed=4)]
     ref = [cross_attention(*c).clone() for c in cases]
     streams = [torch.cuda.Stream() for _ in cases]
     torch.cuda.synchronize()
@@ -286,7 +288,7 @@ def test_heads_and_samples_of_one_buffer():
     """q, k, v expanded over samples and heads (stride 0)"""
     from nunchaku_b200.ops import cross_attention
 
-    for Tq, H in ((2, 4), (140, 32)):
+    for Tq, H in ((2, 4), (140, 32), (140, 64)):
         q, k, v = _inputs(1, 1, 1, Tq, 130, 72, torch.bfloat16, seed=5)
         got = cross_attention(q.expand(3, H, -1, -1), k.expand(3, H, -1, -1), v.expand(3, H, -1, -1))
         one = cross_attention(q.expand(3, H, -1, -1).contiguous(), k.expand(3, H, -1, -1).contiguous(), v.expand(3, H, -1, -1).contiguous())
