@@ -96,7 +96,8 @@ struct CrossTileSizes {
     static_assert(V_WARP < WARPS, "warps");
     // registers move inside the pool the CTA was launched with (80 a thread fill the file)
     static constexpr int REGS_SOFTMAX = 112, REGS_OUTPUT = 64, REGS_OTHER = 64;
-    static_assert(4 * TILES * (REGS_SOFTMAX + REGS_OUTPUT) + (WARPS - 8 * TILES) * REGS_OTHER <= WARPS * 80, "register budget");
+    static constexpr int REGS_LAUNCH = 80;
+    static_assert(4 * TILES * (REGS_SOFTMAX + REGS_OUTPUT) + (WARPS - 8 * TILES) * REGS_OTHER <= WARPS * REGS_LAUNCH, "register budget");
     static constexpr int SUM_BYTES = 3 * TILES * CT_BM * 4;   // row sums of three items
     static constexpr int SMEM = 1024 + Q_BUFFERS * TILES * CT_Q_BYTES + 2 * CT_SLOTS * CT_KV_BYTES + TILES * CT_STAGE_BYTES + SUM_BYTES + CT_BAR_BYTES;
     static constexpr int PER_SM = TILES == 1 ? 2 : 1;
@@ -1057,6 +1058,12 @@ template <bool F16, bool MASK, int TILES>
 static int launch_cross_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const CrossTileParams& p, int sms, cudaStream_t stream) {
     using Sz = CrossTileSizes<TILES>;
     auto kern = cross_tile_kernel<F16, MASK, TILES>;
+    // the budget above is of the registers that the compiler gave the kernel: with fewer an increase would wait for good
+    static const int regs = [&] {
+        cudaFuncAttributes fa = {};
+        return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
+    }();
+    if (regs < Sz::REGS_LAUNCH) return fail(SVDQ_ERR_CUDA, "cross_attention: built with %d registers a thread, %d needed", regs, Sz::REGS_LAUNCH);
     static std::atomic<uint64_t> attr_done{0};
     if (int rc = ensure_dynamic_smem(kern, Sz::SMEM + CT_TABLE_BYTES, attr_done)) return rc;
     cudaLaunchConfig_t cfg = {};
